@@ -285,6 +285,90 @@ int gdn_decode_sm100_state16(const void* q, const void* k, const void* v,
                              int dv, int head_map, float scale, int in_dtype,
                              int out_dtype, void* stream);
 
+/* ---- 8-bit key/value cache ------------------------------------------------
+ * A paged K/V cache in 8 bits: writing new tokens, reading tokens back, and
+ * attention over it.  No counterpart in the reference, which attends over
+ * dense 16-bit K and V (src/attn_sm75.cu:107-112) and keeps no cache.
+ *   k_cache, v_cache : [n_blocks][Hkv][block_size][D] e4m3 codes (one byte, the
+ *           format with a largest value of 448 and no infinities)
+ *   k_scale, v_scale : [n_blocks][Hkv] fp32 powers of two 2^e, -40 <= e <= 40;
+ *           the value of a code is code * scale
+ *   block_table : [B][max_blocks] device int32; token p of sequence b is slot
+ *           p % block_size of block block_table[b][p / block_size].  Entries past
+ *           a sequence's last block are not read.  Sequences may share blocks
+ *           that no call writes.
+ *   seq_lens : [B] device int32, tokens of each sequence in the cache
+ *   block_size 16, 32, 64 or 128; D 64, 128 or 256.  Caches 16-byte aligned.
+ * Nothing needs to be initialised: a block's first token sets its scale, and
+ * codes behind a sequence's last token are neither read as values nor written.
+ * Offsets, lengths and block ids are checked on the device before they are
+ * used: what is outside is skipped (a sequence whose offsets or length do not
+ * fit, the tokens of a block whose id lies outside the pool) and
+ * b200lab_device_status() then returns B200LAB_ERR_INVALID. */
+
+/* Writes a batch's new tokens, the last n_b of each sequence's seq_lens[b]:
+ *   k, v : token-major [total_tokens][Hkv][D], in_dtype F16, BF16 or F32, with
+ *          the given strides (in elements) of a token and of a head, channels
+ *          contiguous; so K and V may be slices of a fused projection.  Base
+ *          pointers 16-byte aligned, strides multiples of 16 bytes.
+ *   seq_lens counts the new tokens too.
+ *   cu_seqlens : [B+1] device int32 prefix sums of the n_b; NULL: one token a
+ *          sequence (total_tokens == B, max_seqlen 1), and a sequence with
+ *          seq_lens[b] <= 0 is a padding entry, of which nothing is written.
+ *   max_seqlen : the most new tokens a sequence has (bounds the grid).
+ * The scale of a (block, head) is the smallest power of two in range with
+ * max |x| <= 448 * scale over the finite values written to it; a block begun by
+ * an earlier call keeps its scale unless the new tokens need a larger one, to
+ * which its codes are then rounded (exactly, but for those that become
+ * subnormal).  Codes are rounded to nearest even; infinities and values above
+ * 448 * 2^40 become +-448 * scale, NaN stays NaN.  A block that is written
+ * belongs to one sequence of the call. */
+int kv8_append_sm100(const void* k, long long k_stride_token, long long k_stride_head,
+                     const void* v, long long v_stride_token, long long v_stride_head,
+                     void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                     const int* block_table, const int* seq_lens, const int* cu_seqlens,
+                     int max_seqlen, int total_tokens, int B, int max_blocks, int n_blocks,
+                     int block_size, int Hkv, int D, int in_dtype, void* stream);
+
+/* Reads the first cu_seqlens[b+1] - cu_seqlens[b] tokens of each sequence back:
+ *   k, v : [total_tokens][Hkv][D] contiguous, out_dtype F16, BF16 or F32, 16-byte
+ *          aligned; packed as attn_fwd_sm100_varlen takes them, which is how the
+ *          queries of a long prompt attend over a cached context.
+ * code * scale is exact in BF16 and F32 and rounded in F16 (values above 65504
+ * become infinite).  Rows behind the last sequence are left as they were. */
+int kv8_read_sm100(const void* k_cache, const void* v_cache, const float* k_scale,
+                   const float* v_scale, const int* block_table, const int* cu_seqlens,
+                   int max_seqlen, int total_tokens, void* k, void* v, int B, int max_blocks,
+                   int n_blocks, int block_size, int Hkv, int D, int out_dtype, void* stream);
+
+/* Softmax attention of each sequence's last tokens over the cache:
+ *   O = softmax(scale * Q K^T [+mask]) V [* sigmoid(G)]
+ *   Q : token-major [total_q][Hq][D], dtype F16 or BF16, with the given strides
+ *       (in elements, multiples of 8) of a token and of a head; 16-byte aligned.
+ *   G : gate like Q with its own strides, or NULL.
+ *   O : [total_q][Hq][D] contiguous, 16-byte aligned.
+ *   seq_lens : keys of each sequence, its query tokens' own among them.
+ *   cu_seqlens_q : [B+1] device int32 prefix sums of the query tokens n_b; NULL:
+ *       one token a sequence (total_q == B, max_seqlen_q 1).
+ *   causal: query i of n_b sees the keys j <= i + seq_lens[b] - n_b.  A row that
+ *       sees no key (seq_lens[b] == 0, a padding entry) is written as 0.  Rows
+ *       behind the last sequence are left as they were.
+ * GQA as attn_fwd_sm100.  Any number of query tokens is right, but the kernel is
+ * made for few: it reads the cache once for every 8..32 rows of a kv group
+ * (16 at D = 256), so the queries of a long prompt are faster through
+ * kv8_read_sm100 and attn_fwd_sm100_varlen.  Calls that may overlap need
+ * workspaces of their own. */
+int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long long q_stride_head,
+                       const void* G, long long g_stride_token, long long g_stride_head,
+                       const void* k_cache, const void* v_cache, const float* k_scale,
+                       const float* v_scale, const int* block_table, const int* seq_lens,
+                       const int* cu_seqlens_q, int max_seqlen_q, int total_q, void* O, int B,
+                       int max_blocks, int n_blocks, int block_size, int Hq, int Hkv, int D,
+                       float scale, int causal, int dtype, void* workspace, size_t ws_bytes,
+                       void* stream);
+/* Its workspace in bytes (independent of lengths and batch), on the current device. */
+size_t attn_fwd_sm100_kv8_workspace(int Hq, int Hkv, int max_seqlen_q, int D);
+
 /* ---- utilities ----------------------------------------------------------- */
 /* Message for a status code (static storage). */
 const char* b200lab_strerror(int status);

@@ -11,6 +11,9 @@ Entry points (reference interface each replaces, cookys/turing-sm75):
 * :func:`attn_fwd`     -- flash_attn_sm75_wmma / _ffma  (src/attn_sm75.cu:107-375)
 * :func:`gdn_prefill`  -- gdn_wmma_kernel, gdn_prep/apply (src/gdn_sm75.cu:361-574, 896-1073)
 * :func:`gdn_decode`   -- token-serial gdn_occ*_kernel at T=1 (src/gdn_sm75.cu:722-789)
+
+Without a counterpart there: the paged 8-bit key/value cache (:func:`kv8_append`,
+:func:`kv8_read`, :func:`attn_fwd_kv8`).
 """
 from __future__ import annotations
 
@@ -40,6 +43,7 @@ EXPORTED = (
     "gdn_prefill_sm100_fused", "gdn_prefill_sm100_varlen", "gdn_prefill_sm100_fused_varlen",
     "gdn_decode_sm100", "gdn_decode_sm100_state16", "gdn_decode_sm100_fused",
     "gdn_decode_sm100_slots",
+    "kv8_append_sm100", "kv8_read_sm100", "attn_fwd_sm100_kv8", "attn_fwd_sm100_kv8_workspace",
     "b200lab_strerror", "b200lab_device_status", "b200lab_version", "b200lab_launch_count",
     "b200lab_watchdog_selftest",
 )
@@ -103,6 +107,16 @@ def lib() -> ctypes.CDLL:
         L.gdn_decode_sm100_fused.argtypes = [vp] * 9 + [ci] * 6 + [cf, ci, ci, vp]
         L.gdn_decode_sm100_state16.restype = ci
         L.gdn_decode_sm100_state16.argtypes = [vp] * 6 + [ci, vp] + [ci] * 6 + [cf, ci, ci, vp]
+        ll = ctypes.c_longlong
+        L.kv8_append_sm100.restype = ci
+        L.kv8_append_sm100.argtypes = [vp, ll, ll, vp, ll, ll] + [vp] * 7 + [ci] * 9 + [vp]
+        L.kv8_read_sm100.restype = ci
+        L.kv8_read_sm100.argtypes = [vp] * 6 + [ci] * 2 + [vp] * 2 + [ci] * 7 + [vp]
+        L.attn_fwd_sm100_kv8.restype = ci
+        L.attn_fwd_sm100_kv8.argtypes = ([vp, ll, ll, vp, ll, ll] + [vp] * 7 + [ci] * 2 + [vp] + [ci] * 7 +
+                                         [cf, ci, ci, vp, sz, vp])
+        L.attn_fwd_sm100_kv8_workspace.restype = sz
+        L.attn_fwd_sm100_kv8_workspace.argtypes = [ci] * 4
         L.b200lab_strerror.restype = ctypes.c_char_p
         L.b200lab_strerror.argtypes = [ci]
         L.b200lab_device_status.restype = ci
@@ -448,6 +462,189 @@ def gdn_decode_slots(q, k, v, g_log, beta, state_pool, slots, *, scale: float | 
                                       int(head_map), float(scale), _dtype_code(q), _dtype_code(out),
                                       _stream(stream))
     _check(st, "gdn_decode_sm100_slots")
+    return out
+
+
+# ---- 8-bit key/value cache -------------------------------------------------
+class _On:
+    """Makes `device` current and `stream` (None: the device's current one) the stream that new
+    tensors belong to, where they are not already; .ptr is the stream's handle."""
+
+    __slots__ = ("ptr", "_ctx")
+
+    def __init__(self, device, stream):
+        cuda = _torch().cuda
+        self._ctx = []
+        if cuda.current_device() != device.index:
+            self._ctx.append(cuda.device(device))
+        cur = cuda.current_stream(device)
+        if stream is None:
+            stream = cur
+        elif stream.device != device:
+            raise ValueError("stream belongs to another device than the tensors")
+        elif stream != cur:
+            self._ctx.append(cuda.stream(stream))
+        self.ptr = stream.cuda_stream
+
+    def __enter__(self):
+        for c in self._ctx:
+            c.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        for c in reversed(self._ctx):
+            c.__exit__(*exc)
+        return False
+
+
+def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
+    """Checks of the cache's tensors; returns (n_blocks, Hkv, block_size, D)."""
+    torch = _torch()
+    dev = k_cache.device
+    if dev.type != "cuda":
+        raise ValueError("k_cache must be a CUDA tensor (no CPU path)")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache and v_cache must be [n_blocks, Hkv, block_size, D], alike")
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+        raise TypeError("k_cache and v_cache must be float8_e4m3fn")
+    if k_scale.shape != k_cache.shape[:2] or v_scale.shape != k_cache.shape[:2]:
+        raise ValueError("k_scale and v_scale must be [n_blocks, Hkv]")
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise TypeError("k_scale and v_scale must be float32")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32:
+        raise ValueError("block_table must be int32 [B, max_blocks]")
+    for t in (k_cache, v_cache, k_scale, v_scale, block_table):
+        if not t.is_contiguous():
+            raise ValueError("the cache, its scales and the block table must be contiguous")
+        if t.device != dev:
+            raise ValueError("the cache, its scales and the block table must be on one device")
+    return k_cache.shape
+
+
+def _kv8_ints(t, n, name, dev):
+    torch = _torch()
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
+    return t.data_ptr()
+
+
+def _rows(t, shape, name, dev):
+    """Checks of a token-major [total, H, D] tensor with contiguous channels; (pointer, strides)."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on the cache's device")
+    st, sh, sd = t.stride()
+    if sd != 1:
+        raise ValueError(f"{name} must have contiguous channels")
+    return t.data_ptr(), st, sh
+
+
+def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *, cu_seqlens=None,
+               max_seqlen: int = 1, stream=None) -> None:
+    """Write a batch's new tokens into the paged 8-bit cache (in place).  k, v [total,Hkv,D]
+    (fp16/bf16/fp32; strided views of a fused projection are taken as they are); k_cache, v_cache
+    [n_blocks,Hkv,block_size,D] float8_e4m3fn; k_scale, v_scale [n_blocks,Hkv] fp32 powers of two;
+    block_table int32 [B,max_blocks]; seq_lens int32 [B], the new tokens counted; cu_seqlens int32
+    [B+1] of the new tokens (None: one a sequence, seq_lens <= 0 marking padding) with max_seqlen
+    the most of one sequence."""
+    n_blocks, Hkv, block_size, D = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
+    dev = k_cache.device
+    B, max_blocks = block_table.shape
+    total = k.shape[0]
+    if v.dtype != k.dtype:
+        raise TypeError("k and v must share a dtype")
+    kp, kt, kh = _rows(k, (total, Hkv, D), "k", dev)
+    vp, vt, vh = _rows(v, (total, Hkv, D), "v", dev)
+    lens = _kv8_ints(seq_lens, B, "seq_lens", dev)
+    cu = 0 if cu_seqlens is None else _kv8_ints(cu_seqlens, B + 1, "cu_seqlens", dev)
+    code = _dtype_code(k)
+    if total == 0 and cu_seqlens is not None:
+        return
+    with _On(dev, stream) as on:
+        st = lib().kv8_append_sm100(kp, kt, kh, vp, vt, vh, k_cache.data_ptr(), v_cache.data_ptr(),
+                                    k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), lens, cu,
+                                    int(max_seqlen), total, B, max_blocks, n_blocks, block_size, Hkv, D, code, on.ptr)
+    _check(st, "kv8_append_sm100")
+
+
+def kv8_read(k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, max_seqlen: int, total_tokens: int, *,
+             out_dtype=None, k_out=None, v_out=None, stream=None):
+    """Read the first cu_seqlens[b+1] - cu_seqlens[b] tokens of each sequence back from the 8-bit
+    cache, packed [total_tokens,Hkv,D] in out_dtype (fp16/bf16/fp32, default bf16).  Returns (k, v)."""
+    torch = _torch()
+    n_blocks, Hkv, block_size, D = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
+    dev = k_cache.device
+    B, max_blocks = block_table.shape
+    cu = _kv8_ints(cu_seqlens, B + 1, "cu_seqlens", dev)
+    shape = (int(total_tokens), Hkv, D)
+    with _On(dev, stream) as on:
+        outs = []
+        for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+            if t is None:
+                t = torch.empty(shape, dtype=out_dtype or torch.bfloat16, device=dev)
+            elif t.shape != shape or t.device != dev or not t.is_contiguous() or t.dtype != (out_dtype or t.dtype):
+                raise ValueError(f"{name} must be contiguous {list(shape)} of out_dtype on the cache's device")
+            outs.append(t)
+        if outs[0].dtype != outs[1].dtype:
+            raise TypeError("k_out and v_out must share a dtype")
+        if shape[0] > 0:
+            st = lib().kv8_read_sm100(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                      block_table.data_ptr(), cu, int(max_seqlen), shape[0], outs[0].data_ptr(),
+                                      outs[1].data_ptr(), B, max_blocks, n_blocks, block_size, Hkv, D,
+                                      _dtype_code(outs[0]), on.ptr)
+            _check(st, "kv8_read_sm100")
+    return outs[0], outs[1]
+
+
+def attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q=1, D=128) -> int:
+    """Workspace bytes of attn_fwd_kv8 (independent of batch and lengths)."""
+    return int(lib().attn_fwd_sm100_kv8_workspace(Hq, Hkv, int(max_seqlen_q), D))
+
+
+def attn_fwd_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *, cu_seqlens_q=None,
+                 max_seqlen_q: int = 1, gate=None, scale: float | None = None, causal: bool = True, out=None,
+                 workspace=None, stream=None):
+    """Attention of each sequence's last tokens over the paged 8-bit cache (their own keys already
+    appended).  q [total_q,Hq,D] fp16/bf16, gate like q or None (out * sigmoid(gate)), both possibly
+    strided views; cu_seqlens_q int32 [B+1] (None: one token a sequence) with max_seqlen_q the most of
+    one sequence; the cache as in :func:`kv8_append`.  Returns [total_q,Hq,D]; rows that see no key are 0."""
+    torch = _torch()
+    n_blocks, Hkv, block_size, D = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
+    dev = k_cache.device
+    B, max_blocks = block_table.shape
+    total, Hq = q.shape[0], q.shape[1]
+    shape = (total, Hq, D)
+    qp, qt, qh = _rows(q, shape, "q", dev)
+    gp, gt, gh = 0, 0, 0
+    if gate is not None:
+        if gate.dtype != q.dtype:
+            raise TypeError("gate must have q's dtype")
+        gp, gt, gh = _rows(gate, shape, "gate", dev)
+    lens = _kv8_ints(seq_lens, B, "seq_lens", dev)
+    cu = 0 if cu_seqlens_q is None else _kv8_ints(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
+    code = _dtype_code(q)
+    if out is not None and (out.shape != shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev):
+        raise ValueError("out must be contiguous, like q, on the cache's device")
+    if workspace is not None and (not workspace.is_contiguous() or workspace.device != dev):
+        raise ValueError("workspace must be contiguous, on the cache's device")
+    if scale is None:
+        scale = 1.0 / (D ** 0.5)
+    with _On(dev, stream) as on:
+        if out is None:
+            out = torch.empty(shape, dtype=q.dtype, device=dev)
+        if total == 0 and cu_seqlens_q is not None:
+            return out
+        if workspace is None:
+            # at least a byte, so that wrong sizes reach the library's own checks
+            workspace = torch.empty(max(1, attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q, D)), dtype=torch.uint8,
+                                    device=dev)
+        st = lib().attn_fwd_sm100_kv8(qp, qt, qh, gp, gt, gh, k_cache.data_ptr(), v_cache.data_ptr(),
+                                      k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), lens, cu,
+                                      int(max_seqlen_q), total, out.data_ptr(), B, max_blocks, n_blocks, block_size,
+                                      Hq, Hkv, D, float(scale), int(bool(causal)), code, workspace.data_ptr(),
+                                      workspace.numel() * workspace.element_size(), on.ptr)
+    _check(st, "attn_fwd_sm100_kv8")
     return out
 
 

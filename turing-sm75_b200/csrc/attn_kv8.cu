@@ -1,0 +1,968 @@
+// attn_kv8.cu -- softmax attention of a batch's last tokens over the paged 8-bit key/value cache
+// (layout and number format: kv8.cuh).
+//
+// No counterpart in the reference, which attends over dense 16-bit K and V
+// (src/attn_sm75.cu:107-112); same softmax semantics as attn_fwd_sm100.
+//
+// Mathematics.  For a query row r and key j, with the codes c and the scales sK, sV of j's block:
+//   x = scale log2(e) sK (q . cK) + log2(sV),  p = 2^(x - m),  O = sum p cV,  l = sum p / sV,
+// m a running maximum of x, and o = O / l.  The scale of V rides in the exponent of the weights,
+// so codes are multiplied as they are, whatever the blocks' scales.  (Scales are 2^e, |e| <= 40:
+// a weight that underflows to 0 in p counts less than 2^-46 of l.)
+//
+// What bounds it: the bytes of the cache; a code is used by the few rows of its kv group only
+// (2 x rows flop a byte).  Everything follows from streaming them:
+//   * The batch's work is cut into equal runs of 64-key tiles, one run a CTA, whatever the lengths
+//     are (the tiles of all (sequence, kv-head, row tile) segments are numbered through on the
+//     device).  A segment that lies in one run is written out by its CTA; one that is cut leaves
+//     fp32 partial sums in the workspace, two at most a CTA, and a second kernel joins them.
+//   * A warp has a ring of its own of 16-key pieces of K and V, filled by TMA, whose next pieces
+//     are requested across segment borders, so that the loads never pause.
+//   * Products are mma.sync m16n8k16 with the KEYS (S^T = K Q^T) and the CHANNELS (O^T = V^T P^T)
+//     on the 16-row side and 8 query rows on the 8-column side: a kv group of 1..8 rows fills one
+//     column tile, a code is converted to fp16 (exactly) once for all column tiles, and P^T
+//     turns from result into operand by a register transpose (movmatrix).
+//   * The channel and key order inside a product is free: each thread takes 32 consecutive channels
+//     of a K row (two 16-byte shared loads, conflict-free under the TMA swizzle) and 16 of four V
+//     rows, whose bytes it pairs by key with one PRMT for two conversions.
+//   * Q is brought to fp16 with a power of two a row: exact, as bf16 and fp16 both have at most 11
+//     significant bits (below 2^-29 of the row's largest value, bits are lost).
+#include "errwords.h"
+#include "kv8.cuh"
+
+namespace b200 {
+namespace {
+
+__device__ int g_err_attn_kv8 = 0;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kPiece = 16;                // keys a warp takes at a time
+constexpr int kTile = kPiece * kWarps;    // keys a CTA takes at a time
+constexpr int kMaxGrid = 2048;            // more CTAs than any sm_100 part has resident here
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.f;              // the running maximum is moved when x exceeds it by 2^8
+
+// Ring of one warp: kDepth pieces of K and V, 16 to 24 KB, so that two CTAs fit an SM.
+template <int D, int NT> struct Ring {
+    static constexpr int kBytes = 2 * kPiece * D;   // a piece of K, then one of V
+    static constexpr int kDepth = D == 256 ? (NT == 1 ? 3 : 2) : D == 128 ? 5 : 10;
+};
+
+struct PieceMeta {
+    float ks;   // scale of K
+    float lv;   // log2 of the scale of V
+    float iv;   // 1 / scale of V
+    int ok;     // 0: the block id lies outside the pool
+};
+
+struct Args {
+    const void* q;
+    const void* g;  // gate or null
+    void* o;
+    long long q_st, q_sh, g_st, g_sh;  // strides of a token and of a head
+    const int* table;
+    const int* lens;
+    const int* cu;  // null: one query token a sequence
+    const float* k_scale;
+    const float* v_scale;
+    float* part;    // [grid][2][rows][D] sums, [grid][2][rows] (m, l)
+    int* meta;      // [grid][4]
+    int max_seqlen_q, total_q, B, max_blocks, n_blocks, log2P, Hq, Hkv, group, causal;
+    float scale;
+};
+
+// ---- the plan: sequences -> segments -> 64-key tiles ------------------------------------------
+struct Seq {
+    int n, L, t0;      // query tokens, keys, first packed token
+    int tiles, rts;    // key tiles and row tiles
+    __device__ __forceinline__ long long units(int Hkv) const { return (long long)tiles * rts * Hkv; }
+};
+
+// A sequence whose offsets or length are outside what the call was given has no tiles and is reported.
+template <int NT> __device__ __forceinline__ Seq load_seq(const Args& a, int b, bool report) {
+    Seq s;
+    s.L = a.lens[b];
+    s.t0 = a.cu ? a.cu[b] : b;
+    const long long n = a.cu ? (long long)a.cu[b + 1] - s.t0 : 1;
+    s.tiles = s.rts = s.n = 0;
+    if (n == 0) return s;
+    if (s.t0 < 0 || n < 0 || s.t0 + n > a.total_q || n > a.max_seqlen_q || s.L < 0 ||
+        s.L > ((long long)a.max_blocks << a.log2P)) {
+        if (report) atomicExch(&g_err_attn_kv8, B200LAB_ERR_INVALID);
+        return s;
+    }
+    s.n = (int)n;
+    s.tiles = max(1, (s.L + kTile - 1) / kTile);  // a sequence without keys has a tile, to write its zeros
+    s.rts = (s.n * a.group + 8 * NT - 1) / (8 * NT);
+    return s;
+}
+
+// A place in the numbered tiles: sequence, kv-head, row tile, key tile; `left` tiles of the CTA's
+// run from here on.
+template <int NT> struct Cursor {
+    Seq s;
+    int b, h, rt, tile;
+    long long left;
+    __device__ __forceinline__ int run() const { return (int)min((long long)(s.tiles - tile), left); }
+    // to the first tile of the next segment
+    __device__ __forceinline__ void next(const Args& a) {
+        left -= run();
+        if (left <= 0) return;
+        tile = 0;
+        if (++rt < s.rts) return;
+        rt = 0;
+        if (++h < a.Hkv) return;
+        h = 0;
+        do {
+            s = load_seq<NT>(a, ++b, false);
+        } while (s.tiles == 0);  // ends: tiles are left
+    }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int D, int NT> struct Smem {
+    static constexpr int kRow = D == 128 ? 128 : 64;  // channels joined at a time
+    alignas(1024) uint8_t ring[kWarps][Ring<D, NT>::kDepth][Ring<D, NT>::kBytes];
+    alignas(16) float join[kWarps][8][kRow + 4];
+    uint2 qfrag[NT > 1 ? NT : 1][NT > 1 ? D / 16 : 1][32];
+    PieceMeta piece[kWarps][Ring<D, NT>::kDepth];
+    float m[kWarps][8 * NT], l[kWarps][8 * NT];
+    float qscale[8 * NT];
+    uint64_t full[kWarps][Ring<D, NT>::kDepth];
+    long long total[kWarps];
+    long long first_unit;
+    int first_b;
+    int abort;
+};
+
+// The factor that brings a part's sums from its own maximum m to the common one M.  A part without
+// scores counts nothing, one whose scores are all NaN (l is NaN) everything.
+__device__ __forceinline__ float part_weight(float m, float l, float M) {
+    return m == -INFINITY && l == l ? 0.f : ex2(m - M);
+}
+
+// One output value of a row: the gate, and the rounding to the output type.
+template <typename T> __device__ __forceinline__ float gated(float o, float g) { return o / (1.f + __expf(-g)); }
+
+// Row n of a row tile -> query token of the sequence and head of the group.
+__device__ __forceinline__ void row_place(int row, int group, int& i, int& hg) {
+    i = row / group;
+    hg = row - i * group;
+}
+
+// kPer consecutive output channels of one row.
+template <typename T, int kPer>
+__device__ __forceinline__ void store_row(const Args& a, size_t token, int head, int D, int d0, const float (&x)[kPer]) {
+    float y[kPer];
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) y[u] = x[u];
+    if (a.g) {
+        const T* g = static_cast<const T*>(a.g) + token * a.g_st + (size_t)head * a.g_sh + d0;
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) y[u] = gated<T>(y[u], Elem<T>::to_f(g[u]));
+    }
+    T* o = static_cast<T*>(a.o) + (token * a.Hq + head) * (size_t)D + d0;
+    if constexpr (kPer % 8 == 0) {
+#pragma unroll
+        for (int u = 0; u < kPer; u += 8) {
+            uint4 w;
+            w.x = Elem<T>::pack2(y[u], y[u + 1]);
+            w.y = Elem<T>::pack2(y[u + 2], y[u + 3]);
+            w.z = Elem<T>::pack2(y[u + 4], y[u + 5]);
+            w.w = Elem<T>::pack2(y[u + 6], y[u + 7]);
+            *reinterpret_cast<uint4*>(o + u) = w;
+        }
+    } else {
+        static_assert(kPer == 4, "");
+        *reinterpret_cast<uint2*>(o) = make_uint2(Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3]));
+    }
+}
+
+// Where the words of a thread's K row lie: the 128-byte swizzle (64-byte at D = 64) of the TMA box,
+// 16-byte chunk index XOR row.
+template <int D> __device__ __forceinline__ int chunk_at(int row, int chunk) {
+    if constexpr (D == 64) {
+        return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+    } else {
+        return row * 128 + ((chunk ^ (row & 7)) << 4);
+    }
+}
+
+// The key that row i (mod 8) of a product stands for.  At D = 64, where a row is half a line of
+// banks, this order keeps the K loads (rows i and i + 1 of the product) and the V loads (rows 0, 2,
+// 4, 6, or 1, 3, 5, 7) free of bank conflicts; wider rows need none.
+template <int D> __device__ __forceinline__ int key_of(int i) {
+    return D == 64 ? (int)((0x65742130u >> (4 * i)) & 7u) : i;
+}
+
+// One query row's channels of this thread, as the operand of Q K^T: f[ks] holds the channels that
+// word ks of the thread's K row holds.  The row is scaled by a power of two to a largest magnitude
+// in [2^14, 2^15); returned is the inverse factor, NaN for a row that is not finite (its scores then
+// are NaN, as in exact arithmetic some would be).  q null: a row of zeros.
+template <int D, typename T>
+__device__ __forceinline__ float load_q(const T* q, int t, uint32_t (&f)[D / 16][2]) {
+    constexpr int kBoxes = D > 128 ? 2 : 1, kDims = D == 64 ? 16 : 32;  // channels a thread has in a box
+    uint4 raw[kBoxes][kDims / 8];
+    float amax = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int box = 0; box < kBoxes; ++box)
+#pragma unroll
+        for (int c = 0; c < kDims / 8; ++c) {
+            raw[box][c] = q ? *reinterpret_cast<const uint4*>(q + box * 128 + t * kDims + c * 8) : make_uint4(0, 0, 0, 0);
+            const T* e = reinterpret_cast<const T*>(&raw[box][c]);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float x = fabsf(Elem<T>::to_f(e[u]));
+                finite = finite && x <= 3.402823466e38f;
+                amax = fmaxf(amax, x);
+            }
+        }
+#pragma unroll
+    for (int m = 1; m <= 2; m <<= 1) {  // the four threads of a row
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
+        finite = __shfl_xor_sync(0xffffffffu, (int)finite, m) && finite;
+    }
+    const uint32_t field = min(268u - min(__float_as_uint(amax) >> 23, 254u), 227u);
+    const float to = finite ? __uint_as_float(field << 23) : 0.f;
+#pragma unroll
+    for (int box = 0; box < kBoxes; ++box)
+#pragma unroll
+        for (int c = 0; c < kDims / 8; ++c) {
+            const T* e = reinterpret_cast<const T*>(&raw[box][c]);
+            float x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = finite ? Elem<T>::to_f(e[u]) * to : 0.f;
+            const int ks = box * (kDims / 4) + 2 * c;
+            f[ks][0] = pack_h2(x[0], x[1]);
+            f[ks][1] = pack_h2(x[2], x[3]);
+            f[ks + 1][0] = pack_h2(x[4], x[5]);
+            f[ks + 1][1] = pack_h2(x[6], x[7]);
+        }
+    return finite ? __uint_as_float((254u - field) << 23) : __uint_as_float(0x7fc00000u);
+}
+
+// The pieces of one warp in the order it takes them, requested ahead of their use.
+template <int D, int NT> struct Producer {
+    Cursor<NT> c;
+    int k;        // next tile of the segment, from c.tile
+    int block;    // lane i: of tile c.tile + (k & ~31) + i
+    float ks, vs;
+
+    // Requests the next piece into a ring slot; false: none is left.
+    __device__ __forceinline__ bool issue(const Args& a, const CUtensorMap* mk, const CUtensorMap* mv, uint8_t* slot,
+                                          PieceMeta* meta, uint64_t* bar, int warp, int lane) {
+        for (;;) {
+            if (c.left <= 0) return false;
+            if (k < c.run() && (c.tile + k) * kTile + warp * kPiece < c.s.L) break;
+            c.next(a);
+            k = 0;
+        }
+        if ((k & 31) == 0) {  // the block ids and scales of the next 32 tiles, one a lane
+            const int pos = (c.tile + k + lane) * kTile + warp * kPiece;
+            block = -1;
+            ks = vs = 0.f;
+            if (k + lane < c.run() && pos < c.s.L) {
+                block = a.table[(size_t)c.b * a.max_blocks + (pos >> a.log2P)];
+                if (block < 0 || block >= a.n_blocks) {
+                    atomicExch(&g_err_attn_kv8, B200LAB_ERR_INVALID);
+                    block = -1;
+                } else {
+                    ks = a.k_scale[(size_t)block * a.Hkv + c.h];
+                    vs = fminf(fmaxf(a.v_scale[(size_t)block * a.Hkv + c.h], kKv8MinScale), kKv8MaxScale);
+                }
+            }
+        }
+        const int blk = __shfl_sync(0xffffffffu, block, k & 31);
+        const float pks = __shfl_sync(0xffffffffu, ks, k & 31), pvs = __shfl_sync(0xffffffffu, vs, k & 31);
+        if (lane == 0) {
+            PieceMeta m;
+            m.ks = pks;
+            const uint32_t bits = __float_as_uint(pvs);
+            const float mant = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+            m.lv = (float)((int)(bits >> 23) - 127) + (mant == 1.f ? 0.f : log2f(mant));
+            m.iv = 1.f / pvs;
+            m.ok = blk >= 0;
+            *meta = m;
+            if (blk >= 0) {
+                const int row = ((c.tile + k) * kTile + warp * kPiece) & ((1 << a.log2P) - 1);
+                const int bh = blk * a.Hkv + c.h;
+                mbar_arrive_expect_tx(bar, Ring<D, NT>::kBytes);
+                constexpr int kBox = D > 128 ? 128 : D;
+#pragma unroll
+                for (int box = 0; box < D / kBox; ++box) {
+                    tma_load_3d(slot + box * kPiece * kBox, mk, bar, box * kBox, row, bh);
+                    tma_load_3d(slot + kPiece * D + box * kPiece * kBox, mv, bar, box * kBox, row, bh);
+                }
+            } else {
+                mbar_arrive(bar);
+            }
+        }
+        ++k;
+        return true;
+    }
+};
+
+template <int D, int NT, typename T>
+__global__ void __launch_bounds__(kThreads, 2)
+    attn_kv8_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const Args a) {
+    constexpr int kRows = 8 * NT, kDepth = Ring<D, NT>::kDepth;
+    constexpr int kBox = D > 128 ? 128 : D, kBoxes = D / kBox;
+    extern __shared__ uint8_t smem_raw[];
+    Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int g = lane >> 2, t = lane & 3;
+
+    if (tid == 0) {
+        prefetch_tmap(&mapK);
+        prefetch_tmap(&mapV);
+        sm.abort = 0;
+    }
+    if (lane == 0) {
+        for (int i = 0; i < kDepth; ++i) mbar_init(&sm.full[warp][i], 1);
+        fence_barrier_init();
+    }
+    grid_dependency_wait();
+    allow_dependent_launch();
+
+    // ---- this CTA's run of tiles: thread i adds up the sequences of its share, the thread whose
+    // share holds the run's first tile finds its sequence
+    const int share = (a.B + kThreads - 1) / kThreads;
+    const int b0 = min(a.B, tid * share), b1 = min(a.B, b0 + share);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += load_seq<NT>(a, b, blockIdx.x == 0).units(a.Hkv);
+    long long upto = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffu, upto, m);
+        if (lane >= m) upto += other;
+    }
+    if (lane == 31) sm.total[warp] = upto;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) upto += sm.total[w];
+        total += sm.total[w];
+    }
+    const long long G = min((long long)gridDim.x, total);
+    if (blockIdx.x >= G) {
+        if (tid == 0) a.meta[4 * blockIdx.x] = -1;
+        return;
+    }
+    const long long u0 = blockIdx.x * total / G, u1 = (blockIdx.x + 1) * total / G;
+    if (upto - mine <= u0 && u0 < upto) {
+        long long at = upto - mine;
+        int b = b0;
+        for (;; ++b) {
+            const long long n = load_seq<NT>(a, b, false).units(a.Hkv);
+            if (u0 < at + n) break;
+            at += n;
+        }
+        sm.first_b = b;
+        sm.first_unit = at;
+    }
+    __syncthreads();
+
+    Cursor<NT> cur;
+    cur.b = sm.first_b;
+    cur.s = load_seq<NT>(a, cur.b, false);
+    {
+        const long long local = u0 - sm.first_unit;
+        const long long seg = local / cur.s.tiles;
+        cur.tile = (int)(local - seg * cur.s.tiles);
+        cur.h = (int)(seg / cur.s.rts);
+        cur.rt = (int)(seg - (long long)cur.h * cur.s.rts);
+        cur.left = u1 - u0;
+    }
+
+    Producer<D, NT> pro;
+    pro.c = cur;
+    pro.k = 0;
+    int put = 0, got = 0, slot = 0;  // pieces requested and taken, the next one's slot
+    uint32_t phase = 0;
+    bool alive = true;
+    for (; put < kDepth; ++put)
+        if (!pro.issue(a, &mapK, &mapV, sm.ring[warp][put], &sm.piece[warp][put], &sm.full[warp][put], warp, lane)) break;
+
+    bool has_tail = false;  // whether the run's last segment goes on in the next CTA's
+    while (cur.left > 0) {
+        const int run = cur.run();
+        const Seq& s = cur.s;
+        const int row0 = cur.rt * kRows, rows = min(kRows, s.n * a.group - row0);
+
+        // ---- Q
+        uint32_t qf[NT == 1 ? D / 16 : 1][2];
+        float qs[NT][2];  // score factors of this thread's two columns of each column tile
+        {
+            const float to_log2 = a.scale * kLog2e;
+            if constexpr (NT == 1) {
+                const T* q = nullptr;
+                if (g < rows) {
+                    int i, hg;
+                    row_place(row0 + g, a.group, i, hg);
+                    q = static_cast<const T*>(a.q) + (size_t)(s.t0 + i) * a.q_st + (size_t)(cur.h * a.group + hg) * a.q_sh;
+                }
+                const float f = load_q<D, T>(q, t, qf) * to_log2;
+                qs[0][0] = __shfl_sync(0xffffffffu, f, 8 * t);
+                qs[0][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+            } else {
+                for (int nt = warp; nt < NT; nt += kWarps) {
+                    const T* q = nullptr;
+                    if (nt * 8 + g < rows) {
+                        int i, hg;
+                        row_place(row0 + nt * 8 + g, a.group, i, hg);
+                        q = static_cast<const T*>(a.q) + (size_t)(s.t0 + i) * a.q_st +
+                            (size_t)(cur.h * a.group + hg) * a.q_sh;
+                    }
+                    uint32_t f[D / 16][2];
+                    const float x = load_q<D, T>(q, t, f) * to_log2;
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) sm.qfrag[nt][ks][lane] = make_uint2(f[ks][0], f[ks][1]);
+                    if (t == 0) sm.qscale[nt * 8 + g] = x;
+                }
+                __syncthreads();  // read again only after the joins below, which end with one too
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    qs[nt][0] = sm.qscale[nt * 8 + 2 * t];
+                    qs[nt][1] = sm.qscale[nt * 8 + 2 * t + 1];
+                }
+            }
+        }
+        float m[NT][2], l[NT][2], o[NT][D / 16][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+        }
+        // the first key that some row of this row tile does not see
+        const int all_see = a.causal ? s.L - s.n + row0 / a.group + 1 : s.L;
+
+        for (int k = 0; k < run; ++k) {
+            const int base = (cur.tile + k) * kTile + warp * kPiece;
+            if (base >= s.L) break;
+            if (alive)  // agreed by the warp: every lane goes the same way on
+                alive = __all_sync(0xffffffffu, mbar_wait(&sm.full[warp][slot], phase, &sm.abort, &g_err_attn_kv8));
+            if (alive) {
+                const PieceMeta meta = sm.piece[warp][slot];
+                const uint8_t* ks_ = sm.ring[warp][slot];
+                const uint8_t* vs_ = ks_ + kPiece * D;
+                if (meta.ok) {
+                    // ---- S^T = K Q^T (16 keys x 8 rows a column tile), two partial sums to shorten the chain
+                    float sc[NT][2][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[nt][0][i] = sc[nt][1][i] = 0.f;
+                    const int kr = key_of<D>(g);
+#pragma unroll
+                    for (int box = 0; box < kBoxes; ++box) {
+                        const uint8_t* kb = ks_ + box * kPiece * kBox;
+                        constexpr int kChunks = D == 64 ? 1 : 2;
+#pragma unroll
+                        for (int c = 0; c < kChunks; ++c) {
+                            const int chunk = kChunks * t + c;
+                            const uint4 lo = *reinterpret_cast<const uint4*>(kb + chunk_at<D>(kr, chunk));
+                            const uint4 hi = *reinterpret_cast<const uint4*>(kb + chunk_at<D>(kr + 8, chunk));
+                            const uint32_t w0[4] = {lo.x, lo.y, lo.z, lo.w}, w1[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int ks = (box * kChunks + c) * 4 + j;
+                                const uint32_t a0 = kv8_decode2(w0[j]), a1 = kv8_decode2(w1[j]);
+                                const uint32_t a2 = kv8_decode2_hi(w0[j]), a3 = kv8_decode2_hi(w1[j]);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    if constexpr (NT == 1) {
+                                        mma(sc[nt][ks & 1], a0, a1, a2, a3, qf[ks][0], qf[ks][1]);
+                                    } else {
+                                        const uint2 qb = sm.qfrag[nt][ks][lane];
+                                        mma(sc[nt][ks & 1], a0, a1, a2, a3, qb.x, qb.y);
+                                    }
+                                }
+                            }
+                        }
+                    }
+                    // ---- softmax over the piece: thread (g, t) has keys key(g), key(g) + 8 of rows 2t, 2t + 1
+                    const bool edge = base + kPiece > all_see;  // some key of the piece is masked for some row
+                    uint32_t pb[NT][2];
+                    bool moved = false;
+                    float mx[NT][2];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            sc[nt][0][i] = fmaf(sc[nt][0][i] + sc[nt][1][i], qs[nt][i & 1] * meta.ks, meta.lv);
+                        if (edge) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int key = base + kr + (i >> 1) * 8;
+                                const int row = row0 + nt * 8 + 2 * t + (i & 1);
+                                const int sees = a.causal ? s.L - s.n + row / a.group + 1 : s.L;
+                                if (key >= min(sees, s.L)) sc[nt][0][i] = -INFINITY;
+                            }
+                        }
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float x = fmaxf(sc[nt][0][c], sc[nt][0][c + 2]);
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                            mx[nt][c] = x;
+                            moved |= x > m[nt][c] + kLazy;
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                const float to = fmaxf(m[nt][c], mx[nt][c]);
+                                const float f = to == -INFINITY ? 1.f : ex2(m[nt][c] - to);
+                                m[nt][c] = to;
+                                l[nt][c] *= f;
+#pragma unroll
+                                for (int i = 0; i < D / 16; ++i) {
+                                    o[nt][i][c] *= f;
+                                    o[nt][i][c + 2] *= f;
+                                }
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
+                        const float m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+                        const float p0 = ex2(sc[nt][0][0] - m0), p1 = ex2(sc[nt][0][1] - m1);
+                        const float p2 = ex2(sc[nt][0][2] - m0), p3 = ex2(sc[nt][0][3] - m1);
+                        l[nt][0] = fmaf(p0 + p2, meta.iv, l[nt][0]);
+                        l[nt][1] = fmaf(p1 + p3, meta.iv, l[nt][1]);
+                        // the weights are rounded to fp16 (2^-11 relative; the sum l is not, its rounding
+                        // errors would not cancel theirs)
+                        pb[nt][0] = transpose8x8(pack_h2(p0, p1));
+                        pb[nt][1] = transpose8x8(pack_h2(p2, p3));
+                    }
+                    // ---- O^T += V^T P^T: product rows are channels, k index i stands for key key(i)
+                    const int r[4] = {key_of<D>(2 * t), key_of<D>(2 * t + 1), key_of<D>(2 * t) + 8, key_of<D>(2 * t + 1) + 8};
+                    constexpr int kWords = kBox / 32;  // of a thread in a V row
+                    uint32_t w[kBoxes][4][kWords];
+#pragma unroll
+                    for (int box = 0; box < kBoxes; ++box)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const uint8_t* vb = vs_ + box * kPiece * kBox;
+                            if constexpr (D == 64) {
+                                const uint2 x = *reinterpret_cast<const uint2*>(vb + chunk_at<D>(r[q], g >> 1) + (g & 1) * 8);
+                                w[box][q][0] = x.x, w[box][q][1] = x.y;
+                            } else {
+                                const uint4 x = *reinterpret_cast<const uint4*>(vb + chunk_at<D>(r[q], g));
+                                w[box][q][0] = x.x, w[box][q][1] = x.y, w[box][q][2] = x.z, w[box][q][3] = x.w;
+                            }
+                        }
+                    if (edge) {
+                        // Behind the sequence's last key lies whatever was there: its codes count as 0, as
+                        // 0 * NaN is NaN.  A NaN that some rows see must not reach the rows that do not: it
+                        // is taken out of the product, and what it meets there becomes NaN by itself.
+                        uint32_t nan = 0;
+#pragma unroll
+                        for (int box = 0; box < kBoxes; ++box)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                                for (int j = 0; j < kWords; ++j) {
+                                    if (base + r[q] >= s.L) w[box][q][j] = 0;
+                                    nan |= ((w[box][q][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                                }
+                        if (__any_sync(0xffffffffu, nan != 0)) {
+#pragma unroll 1
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const int row = row0 + nt * 8 + g;
+                                const int sees = min(a.causal ? s.L - s.n + row / a.group + 1 : s.L, s.L);
+                                uint32_t vis[2];
+#pragma unroll
+                                for (int q = 0; q < 2; ++q)
+                                    vis[q] = pack_h2(base + r[2 * q] < sees ? 1.f : 0.f, base + r[2 * q + 1] < sees ? 1.f : 0.f);
+#pragma unroll
+                                for (int i = 0; i < D / 16; ++i) {
+                                    const int box = i / (kBox / 16), j = (i % (kBox / 16)) >> 1;
+                                    uint32_t f[4];
+#pragma unroll
+                                    for (int q = 0; q < 4; ++q) {
+                                        const uint32_t at = ((w[box][q][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                                        f[q] = (at >> 7) * 0x38u;  // 1.0 where a NaN is
+                                    }
+                                    const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+                                    const uint32_t x = __byte_perm(f[0], f[1], sel), y = __byte_perm(f[2], f[3], sel);
+                                    float hit[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma(hit, kv8_decode2(x), kv8_decode2_hi(x), kv8_decode2(y), kv8_decode2_hi(y), vis[0], vis[1]);
+#pragma unroll
+                                    for (int n2 = 0; n2 < NT; ++n2)
+#pragma unroll
+                                        for (int c = 0; c < 4; ++c)
+                                            if (n2 == nt && hit[c] > 0.f) o[n2][i][c] = __uint_as_float(0x7fc00000u);
+                                }
+                            }
+#pragma unroll
+                            for (int box = 0; box < kBoxes; ++box)
+#pragma unroll
+                                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                                    for (int j = 0; j < kWords; ++j) {
+                                        const uint32_t at = ((w[box][q][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                                        w[box][q][j] &= ~((at >> 7) * 0xffu);
+                                    }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const int box = i / (kBox / 16), j = (i % (kBox / 16)) >> 1;
+                        const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+                        const uint32_t x = __byte_perm(w[box][0][j], w[box][1][j], sel);
+                        const uint32_t y = __byte_perm(w[box][2][j], w[box][3][j], sel);
+                        const uint32_t a0 = kv8_decode2(x), a1 = kv8_decode2_hi(x);
+                        const uint32_t a2 = kv8_decode2(y), a3 = kv8_decode2_hi(y);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma(o[nt][i], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                    }
+                }
+                ++got;
+                __syncwarp();  // every lane has read the slot
+                if (pro.issue(a, &mapK, &mapV, sm.ring[warp][slot], &sm.piece[warp][slot], &sm.full[warp][slot], warp, lane))
+                    ++put;
+            }
+            if (++slot == kDepth) slot = 0, phase ^= 1;
+        }
+
+        // ---- join the warps' sums
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int x = 4; x <= 16; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+                if (g == 0) {
+                    sm.m[warp][nt * 8 + 2 * t + c] = m[nt][c];
+                    sm.l[warp][nt * 8 + 2 * t + c] = l[nt][c];
+                }
+            }
+        __syncthreads();
+        const bool whole = cur.tile == 0 && run == s.tiles;
+        const int part = blockIdx.x * 2 + (cur.tile == 0 ? 1 : 0);
+        constexpr int kRow = Smem<D, NT>::kRow, kPer = kRow / 16;
+        const int jr = tid >> 4, jd = (tid & 15) * kPer;  // this thread's row of a column tile, and channels
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float f[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int n = nt * 8 + 2 * t + c;
+                float M = sm.m[0][n];
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sm.m[w][n]);
+                f[c] = part_weight(m[nt][c], l[nt][c], M);
+            }
+#pragma unroll
+            for (int d = 0; d < D / kRow; ++d) {
+                // rows 2t, 2t + 1; this thread's channels of a box are contiguous, two a product row pair
+                constexpr int kOwn = kBox / 8;  // channels a thread has in a box
+                if constexpr (kRow == kBox) {
+#pragma unroll
+                    for (int i = 0; i < kOwn / 2; i += 2) {
+                        const float(&x)[4] = o[nt][d * (kBox / 16) + i];
+                        const float(&y)[4] = o[nt][d * (kBox / 16) + i + 1];
+                        *reinterpret_cast<float4*>(&sm.join[warp][2 * t][kOwn * g + 2 * i]) =
+                            make_float4(x[0] * f[0], x[2] * f[0], y[0] * f[0], y[2] * f[0]);
+                        *reinterpret_cast<float4*>(&sm.join[warp][2 * t + 1][kOwn * g + 2 * i]) =
+                            make_float4(x[1] * f[1], x[3] * f[1], y[1] * f[1], y[3] * f[1]);
+                    }
+                } else {
+                    // half a box: the threads g of that half
+                    if ((g >> 2) == (d & 1)) {
+#pragma unroll
+                        for (int i = 0; i < kOwn / 2; i += 2) {
+                            const float(&x)[4] = o[nt][(d >> 1) * (kBox / 16) + i];
+                            const float(&y)[4] = o[nt][(d >> 1) * (kBox / 16) + i + 1];
+                            *reinterpret_cast<float4*>(&sm.join[warp][2 * t][kOwn * (g & 3) + 2 * i]) =
+                                make_float4(x[0] * f[0], x[2] * f[0], y[0] * f[0], y[2] * f[0]);
+                            *reinterpret_cast<float4*>(&sm.join[warp][2 * t + 1][kOwn * (g & 3) + 2 * i]) =
+                                make_float4(x[1] * f[1], x[3] * f[1], y[1] * f[1], y[3] * f[1]);
+                        }
+                    }
+                }
+                __syncthreads();
+                const int n = nt * 8 + jr;
+                if (n < rows) {
+                    float M = sm.m[0][n];
+#pragma unroll
+                    for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sm.m[w][n]);
+                    float sum = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w)
+                        sum += sm.l[w][n] * part_weight(sm.m[w][n], sm.l[w][n], M);
+                    float x[kPer];
+#pragma unroll
+                    for (int u = 0; u < kPer; ++u) x[u] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+                        for (int u = 0; u < kPer; ++u) x[u] += sm.join[w][jr][jd + u];
+                    if (whole) {
+                        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key: 0
+#pragma unroll
+                        for (int u = 0; u < kPer; ++u) x[u] *= inv;
+                        int i, hg;
+                        row_place(row0 + n, a.group, i, hg);
+                        store_row<T, kPer>(a, (size_t)(s.t0 + i), cur.h * a.group + hg, D, d * kRow + jd, x);
+                    } else {
+                        float* p = a.part + ((size_t)part * kRows + n) * D + d * kRow + jd;
+#pragma unroll
+                        for (int u = 0; u < kPer; u += 4)
+                            *reinterpret_cast<float4*>(p + u) = make_float4(x[u], x[u + 1], x[u + 2], x[u + 3]);
+                        if (d == 0 && jd == 0)
+                            reinterpret_cast<float2*>(a.part + (size_t)gridDim.x * 2 * kRows * D)[(size_t)part * kRows + n] =
+                                make_float2(M, sum);
+                    }
+                }
+                __syncthreads();
+            }
+        }
+        if (cur.tile == 0 && run < s.tiles) {
+            has_tail = true;
+            if (tid == 0) {
+                const long long end = u1 - cur.left + s.tiles;  // the segment's end
+                a.meta[4 * blockIdx.x] = (int)((end * G - 1) / total);  // the CTA whose run holds its last tile
+                a.meta[4 * blockIdx.x + 1] = cur.b;
+                a.meta[4 * blockIdx.x + 2] = cur.h;
+                a.meta[4 * blockIdx.x + 3] = cur.rt;
+            }
+        }
+        cur.next(a);
+    }
+    if (!has_tail && tid == 0) a.meta[4 * blockIdx.x] = -1;
+    if (!alive) {
+        // a wait gave up: let the copies in flight land (again for a limited time) before the CTA's
+        // shared memory is given back
+        const unsigned long long began = globaltimer_ns();
+        for (; got < put; ++got) {
+            const int i = got % kDepth;
+            while (!mbar_test(&sm.full[warp][i], (got / kDepth) & 1))
+                if (globaltimer_ns() - began > kWaitLimitNs) return;
+        }
+    }
+}
+
+// Joins the segments that were cut.  Block (c, n): row n of the segment whose first part CTA c left;
+// its other parts are the first ones of the CTAs c + 1 .. last.  The 8 warps share the parts.
+template <int D, int NT, typename T>
+__global__ void __launch_bounds__(256) attn_kv8_join_kernel(const Args a, int grid) {
+    constexpr int kRows = 8 * NT, kVec = D / 32;  // channels of a lane
+    __shared__ float weight[kMaxGrid];
+    __shared__ float red[8], acc[8][D];
+    grid_dependency_wait();
+    allow_dependent_launch();
+    const int c = blockIdx.x, n = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int last = a.meta[4 * c];
+    if (last < 0) return;
+    const int b = a.meta[4 * c + 1], h = a.meta[4 * c + 2], rt = a.meta[4 * c + 3];
+    const Seq s = load_seq<NT>(a, b, false);
+    const int row = rt * kRows + n;
+    if (row >= s.n * a.group) return;
+    const int parts = last - c + 1;
+    const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)grid * 2 * kRows * D);
+    auto at = [&](int p) { return (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * kRows + n; };
+    float M = -INFINITY;
+    for (int p = tid; p < parts; p += 256) {
+        const float x = ml[at(p)].x;
+        weight[p] = x;
+        M = fmaxf(M, x);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    if (lane == 0) red[warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) M = fmaxf(M, red[w]);
+    __syncthreads();
+    float sum = 0.f;
+    for (int p = tid; p < parts; p += 256) {
+        const float lp = ml[at(p)].y, f = part_weight(weight[p], lp, M);
+        weight[p] = f;
+        sum += lp * f;
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (lane == 0) red[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += red[w];
+    float x[kVec];
+#pragma unroll
+    for (int u = 0; u < kVec; ++u) x[u] = 0.f;
+#pragma unroll 4
+    for (int p = warp; p < parts; p += 8) {
+        const float f = weight[p];
+        const float* src = a.part + at(p) * D + lane * kVec;
+        float y[kVec];
+#pragma unroll
+        for (int u = 0; u < kVec; u += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(src + u);
+            y[u] = v.x;
+            y[u + 1] = v.y;
+        }
+#pragma unroll
+        for (int u = 0; u < kVec; ++u) x[u] = fmaf(f, y[u], x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kVec; ++u) acc[warp][lane * kVec + u] = x[u];
+    __syncthreads();
+    if (tid < D / 4) {
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) y[u] += acc[w][tid * 4 + u];
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) y[u] *= inv;
+        int i, hg;
+        row_place(row, a.group, i, hg);
+        store_row<T, 4>(a, (size_t)(s.t0 + i), h * a.group + hg, D, tid * 4, y);
+    }
+}
+
+// Column tiles of 8 query rows a CTA works on at once: as many as the rows of a kv group fill, up
+// to what the sums leave registers for.  Rows beyond take further passes over the keys.
+int column_tiles(int rows, int D) {
+    const int most = D == 256 ? 2 : 4;
+    return rows <= 8 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
+}
+
+int plan_grid() {
+    const int g = 2 * device_sm_count();
+    return g < kMaxGrid ? g : kMaxGrid;
+}
+
+size_t workspace_bytes(int nt, int D) {
+    const size_t rows = (size_t)plan_grid() * 2 * 8 * nt;
+    return rows * D * 4 + rows * 8 + (size_t)plan_grid() * 16;
+}
+
+template <int D, int NT, typename T>
+int launch(Args a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, cudaStream_t st) {
+    const int grid = plan_grid();
+    const size_t rows = (size_t)grid * 2 * 8 * NT;
+    a.part = static_cast<float*>(ws);
+    a.meta = reinterpret_cast<int*>(a.part + rows * D + rows * 2);
+    constexpr size_t smem = sizeof(Smem<D, NT>) + 1024;
+    auto kern = attn_kv8_kernel<D, NT, T>;
+    B200_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    int rc = kv8_launch(kern, dim3(grid), kThreads, smem, st, mk, mv, a);
+    if (rc != B200LAB_OK) return rc;
+    const long long used = (long long)a.group * a.max_seqlen_q;
+    const int y = (int)(used < 8 * NT ? used : 8 * NT);
+    return kv8_launch(attn_kv8_join_kernel<D, NT, T>, dim3(grid, y), 256, 0, st, a, grid);
+}
+
+template <int D, typename T>
+int launch_rows(int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, cudaStream_t st) {
+    if (nt == 1) return launch<D, 1, T>(a, mk, mv, ws, st);
+    if (nt == 2) return launch<D, 2, T>(a, mk, mv, ws, st);
+    if constexpr (D < 256) return launch<D, 4, T>(a, mk, mv, ws, st);
+    return B200LAB_ERR_UNSUPPORTED;
+}
+
+template <typename T>
+int launch_d(int D, int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, cudaStream_t st) {
+    switch (D) {
+        case 64: return launch_rows<64, T>(nt, a, mk, mv, ws, st);
+        case 128: return launch_rows<128, T>(nt, a, mk, mv, ws, st);
+        default: return launch_rows<256, T>(nt, a, mk, mv, ws, st);
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace b200
+
+B200_DEFINE_ERR_TAKER(attn_kv8, b200::g_err_attn_kv8)
+
+extern "C" size_t attn_fwd_sm100_kv8_workspace(int Hq, int Hkv, int max_seqlen_q, int D) {
+    if (Hq < 1 || Hkv < 1 || Hq % Hkv || max_seqlen_q < 1 || (D != 64 && D != 128 && D != 256)) return 0;
+    const long long rows = (long long)(Hq / Hkv) * max_seqlen_q;
+    return b200::workspace_bytes(b200::column_tiles(rows < 64 ? (int)rows : 64, D), D);
+}
+
+extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long long q_stride_head, const void* G,
+                                  long long g_stride_token, long long g_stride_head, const void* k_cache,
+                                  const void* v_cache, const float* k_scale, const float* v_scale,
+                                  const int* block_table, const int* seq_lens, const int* cu_seqlens_q,
+                                  int max_seqlen_q, int total_q, void* O, int B, int max_blocks, int n_blocks,
+                                  int block_size, int Hq, int Hkv, int D, float scale, int causal, int dtype,
+                                  void* workspace, size_t ws_bytes, void* stream) {
+    using namespace b200;
+    if (!Q || !O || !seq_lens) return B200LAB_ERR_INVALID;
+    int rc = kv8_check_cache(k_cache, v_cache, k_scale, v_scale, block_table, B, max_blocks, n_blocks, block_size, Hkv, D);
+    if (rc != B200LAB_OK) return rc;
+    if (Hq < 1 || Hq % Hkv || max_seqlen_q < 1 || total_q < 1) return B200LAB_ERR_INVALID;
+    if (!cu_seqlens_q && (max_seqlen_q != 1 || total_q != B)) return B200LAB_ERR_INVALID;
+    if (dtype != B200LAB_F16 && dtype != B200LAB_BF16) return B200LAB_ERR_INVALID;
+    if (causal != 0 && causal != 1) return B200LAB_ERR_INVALID;
+    if (!(scale > 0.f) || scale > 3.402823466e38f) return B200LAB_ERR_INVALID;
+    if (!aligned16(Q) || !aligned16(O) || !aligned16(workspace)) return B200LAB_ERR_INVALID;
+    if (q_stride_token < 0 || q_stride_head < 0 || q_stride_token % 8 || q_stride_head % 8) return B200LAB_ERR_INVALID;
+    if (G && (g_stride_token < 0 || g_stride_head < 0)) return B200LAB_ERR_INVALID;
+    const int most = max_seqlen_q < total_q ? max_seqlen_q : total_q;
+    const long long rows = (long long)(Hq / Hkv) * most;
+    if (rows > 0x40000000LL) return B200LAB_ERR_UNSUPPORTED;
+    const int nt = column_tiles((int)rows, D);
+    if (!workspace || ws_bytes < workspace_bytes(nt, D)) return B200LAB_ERR_WORKSPACE;
+    rc = check_device_sm100();
+    if (rc != B200LAB_OK) return rc;
+    Args a;
+    a.q = Q, a.g = G, a.o = O;
+    a.q_st = q_stride_token, a.q_sh = q_stride_head, a.g_st = g_stride_token, a.g_sh = g_stride_head;
+    a.table = block_table, a.lens = seq_lens, a.cu = cu_seqlens_q;
+    a.k_scale = k_scale, a.v_scale = v_scale;
+    a.max_seqlen_q = most, a.total_q = total_q, a.B = B, a.max_blocks = max_blocks, a.n_blocks = n_blocks;
+    a.log2P = kv8_log2_block(block_size), a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv, a.causal = causal;
+    a.scale = scale;
+    // the cache as [n_blocks * Hkv][block_size][D] bytes; a box is 16 tokens of up to 128 channels
+    CUtensorMap mk, mv;
+    const uint32_t box = D > 128 ? 128 : (uint32_t)D;
+    const CUtensorMapSwizzle swizzle = D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    for (int side = 0; side < 2; ++side) {
+        rc = make_tmap_3d(side ? &mv : &mk, side ? v_cache : k_cache, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)D,
+                          (uint64_t)block_size, (uint64_t)n_blocks * Hkv, box, kPiece, swizzle);
+        if (rc != B200LAB_OK) return rc;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, a, mk, mv, workspace, st)
+                                : launch_d<__nv_bfloat16>(D, nt, a, mk, mv, workspace, st);
+}

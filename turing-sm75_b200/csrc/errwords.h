@@ -8,6 +8,8 @@ int take_err_attn();
 int take_err_attn_gated();
 int take_err_gdn_prefill();
 int take_err_gdn_decode();
+int take_err_kv8_cache();
+int take_err_attn_kv8();
 int take_err_watchdog();
 }  // namespace b200
 

@@ -136,7 +136,8 @@ extern "C" int b200lab_device_status(void* stream) {
         return B200LAB_ERR_CUDA;
     int worst = B200LAB_OK;
     const int words[] = {b200::take_err_attn(), b200::take_err_attn_gated(), b200::take_err_gdn_prefill(),
-                         b200::take_err_gdn_decode(), b200::take_err_watchdog()};
+                         b200::take_err_gdn_decode(), b200::take_err_kv8_cache(), b200::take_err_attn_kv8(),
+                         b200::take_err_watchdog()};
     for (int w : words) {
         if (w == B200LAB_ERR_CUDA) return B200LAB_ERR_CUDA;
         if (w != B200LAB_OK) worst = w;
