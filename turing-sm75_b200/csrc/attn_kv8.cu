@@ -16,7 +16,7 @@
 //     are (the tiles of all (sequence, kv-head, row tile) segments are numbered through on the
 //     device).  A segment that lies in one run is written out by its CTA; one that is cut leaves
 //     fp32 partial sums in the workspace, two at most a CTA, and a second kernel joins them.
-//   * A warp has a ring of its own of 16-key pieces of K and V, filled by TMA, whose next pieces
+//   * A warp has a ring of its own of 16- or 32-key pieces of K and V, filled by TMA, whose next pieces
 //     are requested across segment borders, so that the loads never pause.
 //   * Products are mma.sync m16n8k16 with the KEYS (S^T = K Q^T) and the CHANNELS (O^T = V^T P^T)
 //     on the 16-row side and 8 query rows on the 8-column side: a kv group of 1..8 rows fills one
@@ -37,23 +37,27 @@ __device__ int g_err_attn_kv8 = 0;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kPiece = 16;                // keys a warp takes at a time
-constexpr int kTile = kPiece * kWarps;    // keys a CTA takes at a time
+constexpr int kGroup = 16;                // keys of one product
 constexpr int kMaxGrid = 2048;            // more CTAs than any sm_100 part has resident here
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;              // the running maximum is moved when x exceeds it by 2^8
 
-// Ring of one warp: kDepth pieces of K and V, 16 to 24 KB, so that two CTAs fit an SM.
-template <int D, int NT> struct Ring {
-    static constexpr int kBytes = 2 * kPiece * D;   // a piece of K, then one of V
-    static constexpr int kDepth = D == 256 ? (NT == 1 ? 3 : 2) : D == 128 ? 5 : 10;
+// What a variant's CTA works on and holds; kCtas of them fill an SM's registers and shared memory.
+template <int D, int NT> struct Cfg {
+    static constexpr int kH = NT == 1 && D <= 128 ? 2 : 1;  // groups of a piece, the keys a warp takes at a time
+    static constexpr int kPiece = kGroup * kH;
+    static constexpr int kTile = kPiece * kWarps;           // keys a CTA takes at a time
+    static constexpr int kBytes = 2 * kPiece * D;           // a piece of K, then one of V
+    static constexpr int kCtas = NT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : 2;
+    static constexpr int kDepth = (D == 64 ? (NT == 1 ? 5 : 10) : D == 128 ? (NT == 1 ? 4 : 5) : (NT == 1 ? 3 : 2)) / kH;
+    static constexpr int kRow = 64;                         // channels joined at a time
 };
 
-struct PieceMeta {
+struct GroupMeta {
     float ks;   // scale of K
     float lv;   // log2 of the scale of V
     float iv;   // 1 / scale of V
-    int ok;     // 0: the block id lies outside the pool
+    int ok;     // 0: no key of the group is in the sequence, or its block id lies outside the pool
 };
 
 struct Args {
@@ -69,6 +73,7 @@ struct Args {
     float* part;    // [grid][2][rows][D] sums, [grid][2][rows] (m, l)
     int* meta;      // [grid][4]
     int max_seqlen_q, total_q, B, max_blocks, n_blocks, log2P, Hq, Hkv, group, causal;
+    int box_rows;   // tokens a TMA box holds: the piece's, or the block's where that is less
     float scale;
 };
 
@@ -80,7 +85,7 @@ struct Seq {
 };
 
 // A sequence whose offsets or length are outside what the call was given has no tiles and is reported.
-template <int NT> __device__ __forceinline__ Seq load_seq(const Args& a, int b, bool report) {
+template <int D, int NT> __device__ __forceinline__ Seq load_seq(const Args& a, int b, bool report) {
     Seq s;
     s.L = a.lens[b];
     s.t0 = a.cu ? a.cu[b] : b;
@@ -93,6 +98,7 @@ template <int NT> __device__ __forceinline__ Seq load_seq(const Args& a, int b, 
         return s;
     }
     s.n = (int)n;
+    constexpr int kTile = Cfg<D, NT>::kTile;
     s.tiles = max(1, (s.L + kTile - 1) / kTile);  // a sequence without keys has a tile, to write its zeros
     s.rts = (s.n * a.group + 8 * NT - 1) / (8 * NT);
     return s;
@@ -100,7 +106,7 @@ template <int NT> __device__ __forceinline__ Seq load_seq(const Args& a, int b, 
 
 // A place in the numbered tiles: sequence, kv-head, row tile, key tile; `left` tiles of the CTA's
 // run from here on.
-template <int NT> struct Cursor {
+template <int D, int NT> struct Cursor {
     Seq s;
     int b, h, rt, tile;
     long long left;
@@ -115,7 +121,7 @@ template <int NT> struct Cursor {
         if (++h < a.Hkv) return;
         h = 0;
         do {
-            s = load_seq<NT>(a, ++b, false);
+            s = load_seq<D, NT>(a, ++b, false);
         } while (s.tiles == 0);  // ends: tiles are left
     }
 };
@@ -145,14 +151,14 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
 }
 
 template <int D, int NT> struct Smem {
-    static constexpr int kRow = D == 128 ? 128 : 64;  // channels joined at a time
-    alignas(1024) uint8_t ring[kWarps][Ring<D, NT>::kDepth][Ring<D, NT>::kBytes];
+    static constexpr int kRow = Cfg<D, NT>::kRow;
+    alignas(1024) uint8_t ring[kWarps][Cfg<D, NT>::kDepth][Cfg<D, NT>::kBytes];
     alignas(16) float join[kWarps][8][kRow + 4];
     uint2 qfrag[NT > 1 ? NT : 1][NT > 1 ? D / 16 : 1][32];
-    PieceMeta piece[kWarps][Ring<D, NT>::kDepth];
+    GroupMeta meta[kWarps][Cfg<D, NT>::kDepth][Cfg<D, NT>::kH];
     float m[kWarps][8 * NT], l[kWarps][8 * NT];
     float qscale[8 * NT];
-    uint64_t full[kWarps][Ring<D, NT>::kDepth];
+    uint64_t full[kWarps][Cfg<D, NT>::kDepth];
     long long total[kWarps];
     long long first_unit;
     int first_b;
@@ -268,58 +274,69 @@ __device__ __forceinline__ float load_q(const T* q, int t, uint32_t (&f)[D / 16]
 
 // The pieces of one warp in the order it takes them, requested ahead of their use.
 template <int D, int NT> struct Producer {
-    Cursor<NT> c;
+    using C = Cfg<D, NT>;
+    Cursor<D, NT> c;
     int k;        // next tile of the segment, from c.tile
-    int block;    // lane i: of tile c.tile + (k & ~31) + i
-    float ks, vs;
+    int block;    // lane i: of group i of the next 32 / kH pieces
+    float ks, lv, iv;
 
     // Requests the next piece into a ring slot; false: none is left.
     __device__ __forceinline__ bool issue(const Args& a, const CUtensorMap* mk, const CUtensorMap* mv, uint8_t* slot,
-                                          PieceMeta* meta, uint64_t* bar, int warp, int lane) {
+                                          GroupMeta* meta, uint64_t* bar, int warp, int lane) {
         for (;;) {
             if (c.left <= 0) return false;
-            if (k < c.run() && (c.tile + k) * kTile + warp * kPiece < c.s.L) break;
+            if (k < c.run() && (c.tile + k) * C::kTile + warp * C::kPiece < c.s.L) break;
             c.next(a);
             k = 0;
         }
-        if ((k & 31) == 0) {  // the block ids and scales of the next 32 tiles, one a lane
-            const int pos = (c.tile + k + lane) * kTile + warp * kPiece;
+        constexpr int kAhead = 32 / C::kH;
+        if ((k & (kAhead - 1)) == 0) {  // the block ids and scales of the next pieces, a group a lane
+            const int pos = (c.tile + k + lane / C::kH) * C::kTile + warp * C::kPiece + (lane % C::kH) * kGroup;
             block = -1;
-            ks = vs = 0.f;
-            if (k + lane < c.run() && pos < c.s.L) {
+            ks = lv = iv = 0.f;
+            if (k + lane / C::kH < c.run() && pos < c.s.L) {
                 block = a.table[(size_t)c.b * a.max_blocks + (pos >> a.log2P)];
                 if (block < 0 || block >= a.n_blocks) {
                     atomicExch(&g_err_attn_kv8, B200LAB_ERR_INVALID);
                     block = -1;
                 } else {
                     ks = a.k_scale[(size_t)block * a.Hkv + c.h];
-                    vs = fminf(fmaxf(a.v_scale[(size_t)block * a.Hkv + c.h], kKv8MinScale), kKv8MaxScale);
+                    const float vs = fminf(fmaxf(a.v_scale[(size_t)block * a.Hkv + c.h], kKv8MinScale), kKv8MaxScale);
+                    lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);
+                    if (__float_as_uint(vs) & 0x7fffffu) lv = log2f(vs);  // not a power of two
+                    iv = 1.f / vs;
                 }
             }
         }
-        const int blk = __shfl_sync(0xffffffffu, block, k & 31);
-        const float pks = __shfl_sync(0xffffffffu, ks, k & 31), pvs = __shfl_sync(0xffffffffu, vs, k & 31);
-        if (lane == 0) {
-            PieceMeta m;
-            m.ks = pks;
-            const uint32_t bits = __float_as_uint(pvs);
-            const float mant = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
-            m.lv = (float)((int)(bits >> 23) - 127) + (mant == 1.f ? 0.f : log2f(mant));
-            m.iv = 1.f / pvs;
-            m.ok = blk >= 0;
-            *meta = m;
-            if (blk >= 0) {
-                const int row = ((c.tile + k) * kTile + warp * kPiece) & ((1 << a.log2P) - 1);
-                const int bh = blk * a.Hkv + c.h;
-                mbar_arrive_expect_tx(bar, Ring<D, NT>::kBytes);
-                constexpr int kBox = D > 128 ? 128 : D;
+        const int first = (k & (kAhead - 1)) * C::kH;  // lane of the piece's first group
+        int blk[C::kH];
 #pragma unroll
-                for (int box = 0; box < D / kBox; ++box) {
-                    tma_load_3d(slot + box * kPiece * kBox, mk, bar, box * kBox, row, bh);
-                    tma_load_3d(slot + kPiece * D + box * kPiece * kBox, mv, bar, box * kBox, row, bh);
-                }
+        for (int u = 0; u < C::kH; ++u) blk[u] = __shfl_sync(0xffffffffu, block, first + u);
+        if (lane - first >= 0 && lane - first < C::kH) meta[lane - first] = GroupMeta{ks, lv, iv, block >= 0};
+        __syncwarp();  // before lane 0's arrival, which the readers wait for
+        if (lane == 0) {
+            constexpr int kBox = D > 128 ? 128 : D;
+            const int step = a.box_rows / kGroup;  // groups of a box, all of one block
+            int boxes = 0;
+#pragma unroll
+            for (int u = 0; u < C::kH; ++u) boxes += u % step == 0 && blk[u] >= 0;
+            if (boxes) {
+                mbar_arrive_expect_tx(bar, boxes * a.box_rows * 2 * D);
             } else {
                 mbar_arrive(bar);
+            }
+            const int pos = (c.tile + k) * C::kTile + warp * C::kPiece;
+#pragma unroll
+            for (int u = 0; u < C::kH; ++u) {
+                if (u % step != 0 || blk[u] < 0) continue;
+                const int row = (pos + u * kGroup) & ((1 << a.log2P) - 1);
+                const int bh = blk[u] * a.Hkv + c.h;
+#pragma unroll
+                for (int box = 0; box < D / kBox; ++box) {
+                    uint8_t* dst = slot + (box * C::kPiece + u * kGroup) * kBox;
+                    tma_load_3d(dst, mk, bar, box * kBox, row, bh);
+                    tma_load_3d(dst + C::kPiece * D, mv, bar, box * kBox, row, bh);
+                }
             }
         }
         ++k;
@@ -327,10 +344,66 @@ template <int D, int NT> struct Producer {
     }
 };
 
+// The codes of V of a group that some row does not see whole, before their product.  Behind the
+// sequence's last key lies whatever was there: its codes count as 0, as 0 * NaN is NaN.  A NaN that
+// some rows see must not reach the rows that do not: it is taken out of the product, and the sums of
+// the rows that see it become NaN here.
+//   w: this thread's codes of the keys r[0..3] of the group; row: row g of the first column tile
+template <int D, int NT, int kBoxes, int kWords>
+__device__ __forceinline__ void take_out_masked(const Args& a, const Seq& s, uint32_t (&w)[kBoxes][4][kWords],
+                                                float (&o)[NT][D / 16][4], const int (&r)[4], int base, bool ok, int row) {
+    uint32_t nan = 0;
+#pragma unroll
+    for (int box = 0; box < kBoxes; ++box)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {
+                if (base + r[q] >= s.L || !ok) w[box][q][j] = 0;
+                nan |= ((w[box][q][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            }
+    if (!__any_sync(0xffffffffu, nan != 0)) return;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int sees = min(a.causal ? s.L - s.n + (row + nt * 8) / a.group + 1 : s.L, s.L);
+        uint32_t vis[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            vis[q] = pack_h2(base + r[2 * q] < sees ? 1.f : 0.f, base + r[2 * q + 1] < sees ? 1.f : 0.f);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const int box = i / (2 * kWords), j = (i % (2 * kWords)) >> 1;
+            uint32_t f[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t at = ((w[box][q][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                f[q] = (at >> 7) * 0x38u;  // 1.0 where a NaN is
+            }
+            const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+            const uint32_t x = __byte_perm(f[0], f[1], sel), y = __byte_perm(f[2], f[3], sel);
+            float hit[4] = {0.f, 0.f, 0.f, 0.f};
+            mma(hit, kv8_decode2(x), kv8_decode2_hi(x), kv8_decode2(y), kv8_decode2_hi(y), vis[0], vis[1]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (hit[c] > 0.f) o[nt][i][c] = __uint_as_float(0x7fc00000u);
+        }
+    }
+#pragma unroll
+    for (int box = 0; box < kBoxes; ++box)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {
+                const uint32_t at = ((w[box][q][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                w[box][q][j] &= ~((at >> 7) * 0xffu);
+            }
+}
+
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
     attn_kv8_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const Args a) {
-    constexpr int kRows = 8 * NT, kDepth = Ring<D, NT>::kDepth;
+    using C = Cfg<D, NT>;
+    constexpr int kRows = 8 * NT, kDepth = C::kDepth, kH = C::kH, kPiece = C::kPiece, kTile = C::kTile;
     constexpr int kBox = D > 128 ? 128 : D, kBoxes = D / kBox;
     extern __shared__ uint8_t smem_raw[];
     Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -346,15 +419,17 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int i = 0; i < kDepth; ++i) mbar_init(&sm.full[warp][i], 1);
         fence_barrier_init();
     }
+    // Launched early, but lets the join kernel start only as its CTAs end (the default): a join CTA that
+    // waits on an SM keeps the next call's CTA from starting there (B64 16k, calls back to back: 580 us
+    // with the trigger here, 350 without).
     grid_dependency_wait();
-    allow_dependent_launch();
 
     // ---- this CTA's run of tiles: thread i adds up the sequences of its share, the thread whose
     // share holds the run's first tile finds its sequence
     const int share = (a.B + kThreads - 1) / kThreads;
     const int b0 = min(a.B, tid * share), b1 = min(a.B, b0 + share);
     long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += load_seq<NT>(a, b, blockIdx.x == 0).units(a.Hkv);
+    for (int b = b0; b < b1; ++b) mine += load_seq<D, NT>(a, b, blockIdx.x == 0).units(a.Hkv);
     long long upto = mine;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -379,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         long long at = upto - mine;
         int b = b0;
         for (;; ++b) {
-            const long long n = load_seq<NT>(a, b, false).units(a.Hkv);
+            const long long n = load_seq<D, NT>(a, b, false).units(a.Hkv);
             if (u0 < at + n) break;
             at += n;
         }
@@ -388,9 +463,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncthreads();
 
-    Cursor<NT> cur;
+    Cursor<D, NT> cur;
     cur.b = sm.first_b;
-    cur.s = load_seq<NT>(a, cur.b, false);
+    cur.s = load_seq<D, NT>(a, cur.b, false);
     {
         const long long local = u0 - sm.first_unit;
         const long long seg = local / cur.s.tiles;
@@ -407,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint32_t phase = 0;
     bool alive = true;
     for (; put < kDepth; ++put)
-        if (!pro.issue(a, &mapK, &mapV, sm.ring[warp][put], &sm.piece[warp][put], &sm.full[warp][put], warp, lane)) break;
+        if (!pro.issue(a, &mapK, &mapV, sm.ring[warp][put], sm.meta[warp][put], &sm.full[warp][put], warp, lane)) break;
 
     bool has_tail = false;  // whether the run's last segment goes on in the next CTA's
     while (cur.left > 0) {
@@ -470,24 +545,38 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (alive)  // agreed by the warp: every lane goes the same way on
                 alive = __all_sync(0xffffffffu, mbar_wait(&sm.full[warp][slot], phase, &sm.abort, &g_err_attn_kv8));
             if (alive) {
-                const PieceMeta meta = sm.piece[warp][slot];
                 const uint8_t* ks_ = sm.ring[warp][slot];
                 const uint8_t* vs_ = ks_ + kPiece * D;
-                if (meta.ok) {
-                    // ---- S^T = K Q^T (16 keys x 8 rows a column tile), two partial sums to shorten the chain
-                    float sc[NT][2][4];
+                GroupMeta meta[kH];
+                bool whole_piece = true;
+#pragma unroll
+                for (int u = 0; u < kH; ++u) {
+                    meta[u] = sm.meta[warp][slot][u];
+                    whole_piece = whole_piece && meta[u].ok;
+                }
+                // ---- S^T = K Q^T (16 keys x 8 rows a group and column tile); a lone group has two partial
+                // sums, to shorten the chain of products
+                constexpr int kAcc = kH == 1 ? 2 : 1;
+                float sc[kH][NT][kAcc][4];
+#pragma unroll
+                for (int u = 0; u < kH; ++u)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[nt][0][i] = sc[nt][1][i] = 0.f;
-                    const int kr = key_of<D>(g);
+                        for (int i = 0; i < 4; ++i) {
+                            sc[u][nt][0][i] = 0.f;
+                            sc[u][nt][kAcc - 1][i] = 0.f;
+                        }
+                const int kr = key_of<D>(g);
 #pragma unroll
-                    for (int box = 0; box < kBoxes; ++box) {
-                        const uint8_t* kb = ks_ + box * kPiece * kBox;
-                        constexpr int kChunks = D == 64 ? 1 : 2;
+                for (int box = 0; box < kBoxes; ++box) {
+                    constexpr int kChunks = D == 64 ? 1 : 2;
 #pragma unroll
-                        for (int c = 0; c < kChunks; ++c) {
-                            const int chunk = kChunks * t + c;
+                    for (int c = 0; c < kChunks; ++c) {
+                        const int chunk = kChunks * t + c;
+#pragma unroll
+                        for (int u = 0; u < kH; ++u) {
+                            const uint8_t* kb = ks_ + (box * kPiece + u * kGroup) * kBox;
                             const uint4 lo = *reinterpret_cast<const uint4*>(kb + chunk_at<D>(kr, chunk));
                             const uint4 hi = *reinterpret_cast<const uint4*>(kb + chunk_at<D>(kr + 8, chunk));
                             const uint32_t w0[4] = {lo.x, lo.y, lo.z, lo.w}, w1[4] = {hi.x, hi.y, hi.z, hi.w};
@@ -499,83 +588,97 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) {
                                     if constexpr (NT == 1) {
-                                        mma(sc[nt][ks & 1], a0, a1, a2, a3, qf[ks][0], qf[ks][1]);
+                                        mma(sc[u][nt][ks & (kAcc - 1)], a0, a1, a2, a3, qf[ks][0], qf[ks][1]);
                                     } else {
                                         const uint2 qb = sm.qfrag[nt][ks][lane];
-                                        mma(sc[nt][ks & 1], a0, a1, a2, a3, qb.x, qb.y);
+                                        mma(sc[u][nt][ks & (kAcc - 1)], a0, a1, a2, a3, qb.x, qb.y);
                                     }
                                 }
                             }
                         }
                     }
-                    // ---- softmax over the piece: thread (g, t) has keys key(g), key(g) + 8 of rows 2t, 2t + 1
-                    const bool edge = base + kPiece > all_see;  // some key of the piece is masked for some row
-                    uint32_t pb[NT][2];
-                    bool moved = false;
-                    float mx[NT][2];
+                }
+                // ---- softmax over the piece: thread (g, t) has keys key(g), key(g) + 8 of each group and rows
+                // 2t, 2t + 1
+                const bool edge = base + kPiece > all_see || !whole_piece;  // some key is masked for some row
+                bool moved = false;
+                float mx[NT][2];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
+                for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            sc[nt][0][i] = fmaf(sc[nt][0][i] + sc[nt][1][i], qs[nt][i & 1] * meta.ks, meta.lv);
+                    for (int u = 0; u < kH; ++u) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = kAcc == 2 ? sc[u][nt][0][i] + sc[u][nt][kAcc - 1][i] : sc[u][nt][0][i];
+                            sc[u][nt][0][i] = fmaf(x, qs[nt][i & 1] * meta[u].ks, meta[u].lv);
+                        }
                         if (edge) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const int key = base + kr + (i >> 1) * 8;
+                                const int key = base + u * kGroup + kr + (i >> 1) * 8;
                                 const int row = row0 + nt * 8 + 2 * t + (i & 1);
                                 const int sees = a.causal ? s.L - s.n + row / a.group + 1 : s.L;
-                                if (key >= min(sees, s.L)) sc[nt][0][i] = -INFINITY;
-                            }
-                        }
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float x = fmaxf(sc[nt][0][c], sc[nt][0][c + 2]);
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                            mx[nt][c] = x;
-                            moved |= x > m[nt][c] + kLazy;
-                        }
-                    }
-                    if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                const float to = fmaxf(m[nt][c], mx[nt][c]);
-                                const float f = to == -INFINITY ? 1.f : ex2(m[nt][c] - to);
-                                m[nt][c] = to;
-                                l[nt][c] *= f;
-#pragma unroll
-                                for (int i = 0; i < D / 16; ++i) {
-                                    o[nt][i][c] *= f;
-                                    o[nt][i][c + 2] *= f;
-                                }
+                                if (key >= min(sees, s.L) || !meta[u].ok) sc[u][nt][0][i] = -INFINITY;
                             }
                         }
                     }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float x = fmaxf(sc[0][nt][0][c], sc[0][nt][0][c + 2]);
+#pragma unroll
+                        for (int u = 1; u < kH; ++u) x = fmaxf(x, fmaxf(sc[u][nt][0][c], sc[u][nt][0][c + 2]));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        mx[nt][c] = x;
+                        moved |= x > m[nt][c] + kLazy;
+                    }
+                }
+                if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
-                        const float m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-                        const float p0 = ex2(sc[nt][0][0] - m0), p1 = ex2(sc[nt][0][1] - m1);
-                        const float p2 = ex2(sc[nt][0][2] - m0), p3 = ex2(sc[nt][0][3] - m1);
-                        l[nt][0] = fmaf(p0 + p2, meta.iv, l[nt][0]);
-                        l[nt][1] = fmaf(p1 + p3, meta.iv, l[nt][1]);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float to = fmaxf(m[nt][c], mx[nt][c]);
+                            const float f = to == -INFINITY ? 1.f : ex2(m[nt][c] - to);
+                            m[nt][c] = to;
+                            l[nt][c] *= f;
+#pragma unroll
+                            for (int i = 0; i < D / 16; ++i) {
+                                o[nt][i][c] *= f;
+                                o[nt][i][c + 2] *= f;
+                            }
+                        }
+                    }
+                }
+                uint32_t pb[kH][NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
+                    const float m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+                    for (int u = 0; u < kH; ++u) {
+                        const float p0 = ex2(sc[u][nt][0][0] - m0), p1 = ex2(sc[u][nt][0][1] - m1);
+                        const float p2 = ex2(sc[u][nt][0][2] - m0), p3 = ex2(sc[u][nt][0][3] - m1);
+                        l[nt][0] = fmaf(p0 + p2, meta[u].iv, l[nt][0]);
+                        l[nt][1] = fmaf(p1 + p3, meta[u].iv, l[nt][1]);
                         // the weights are rounded to fp16 (2^-11 relative; the sum l is not, its rounding
                         // errors would not cancel theirs)
-                        pb[nt][0] = transpose8x8(pack_h2(p0, p1));
-                        pb[nt][1] = transpose8x8(pack_h2(p2, p3));
+                        pb[u][nt][0] = transpose8x8(pack_h2(p0, p1));
+                        pb[u][nt][1] = transpose8x8(pack_h2(p2, p3));
                     }
-                    // ---- O^T += V^T P^T: product rows are channels, k index i stands for key key(i)
-                    const int r[4] = {key_of<D>(2 * t), key_of<D>(2 * t + 1), key_of<D>(2 * t) + 8, key_of<D>(2 * t + 1) + 8};
-                    constexpr int kWords = kBox / 32;  // of a thread in a V row
+                }
+                // ---- O^T += V^T P^T: product rows are channels, k index i stands for key key(i)
+                const int r[4] = {key_of<D>(2 * t), key_of<D>(2 * t + 1), key_of<D>(2 * t) + 8, key_of<D>(2 * t + 1) + 8};
+                constexpr int kWords = kBox / 32;  // of a thread in a V row
+#pragma unroll
+                for (int u = 0; u < kH; ++u) {
                     uint32_t w[kBoxes][4][kWords];
 #pragma unroll
                     for (int box = 0; box < kBoxes; ++box)
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            const uint8_t* vb = vs_ + box * kPiece * kBox;
+                            const uint8_t* vb = vs_ + (box * kPiece + u * kGroup) * kBox;
                             if constexpr (D == 64) {
                                 const uint2 x = *reinterpret_cast<const uint2*>(vb + chunk_at<D>(r[q], g >> 1) + (g & 1) * 8);
                                 w[box][q][0] = x.x, w[box][q][1] = x.y;
@@ -584,60 +687,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                                 w[box][q][0] = x.x, w[box][q][1] = x.y, w[box][q][2] = x.z, w[box][q][3] = x.w;
                             }
                         }
-                    if (edge) {
-                        // Behind the sequence's last key lies whatever was there: its codes count as 0, as
-                        // 0 * NaN is NaN.  A NaN that some rows see must not reach the rows that do not: it
-                        // is taken out of the product, and what it meets there becomes NaN by itself.
-                        uint32_t nan = 0;
-#pragma unroll
-                        for (int box = 0; box < kBoxes; ++box)
-#pragma unroll
-                            for (int q = 0; q < 4; ++q)
-#pragma unroll
-                                for (int j = 0; j < kWords; ++j) {
-                                    if (base + r[q] >= s.L) w[box][q][j] = 0;
-                                    nan |= ((w[box][q][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                                }
-                        if (__any_sync(0xffffffffu, nan != 0)) {
-#pragma unroll 1
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const int row = row0 + nt * 8 + g;
-                                const int sees = min(a.causal ? s.L - s.n + row / a.group + 1 : s.L, s.L);
-                                uint32_t vis[2];
-#pragma unroll
-                                for (int q = 0; q < 2; ++q)
-                                    vis[q] = pack_h2(base + r[2 * q] < sees ? 1.f : 0.f, base + r[2 * q + 1] < sees ? 1.f : 0.f);
-#pragma unroll
-                                for (int i = 0; i < D / 16; ++i) {
-                                    const int box = i / (kBox / 16), j = (i % (kBox / 16)) >> 1;
-                                    uint32_t f[4];
-#pragma unroll
-                                    for (int q = 0; q < 4; ++q) {
-                                        const uint32_t at = ((w[box][q][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                                        f[q] = (at >> 7) * 0x38u;  // 1.0 where a NaN is
-                                    }
-                                    const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
-                                    const uint32_t x = __byte_perm(f[0], f[1], sel), y = __byte_perm(f[2], f[3], sel);
-                                    float hit[4] = {0.f, 0.f, 0.f, 0.f};
-                                    mma(hit, kv8_decode2(x), kv8_decode2_hi(x), kv8_decode2(y), kv8_decode2_hi(y), vis[0], vis[1]);
-#pragma unroll
-                                    for (int n2 = 0; n2 < NT; ++n2)
-#pragma unroll
-                                        for (int c = 0; c < 4; ++c)
-                                            if (n2 == nt && hit[c] > 0.f) o[n2][i][c] = __uint_as_float(0x7fc00000u);
-                                }
-                            }
-#pragma unroll
-                            for (int box = 0; box < kBoxes; ++box)
-#pragma unroll
-                                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                                    for (int j = 0; j < kWords; ++j) {
-                                        const uint32_t at = ((w[box][q][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                                        w[box][q][j] &= ~((at >> 7) * 0xffu);
-                                    }
-                        }
-                    }
+                    if (edge) take_out_masked<D, NT>(a, s, w, o, r, base + u * kGroup, meta[u].ok, row0 + g);
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) {
                         const int box = i / (kBox / 16), j = (i % (kBox / 16)) >> 1;
@@ -647,12 +697,12 @@ __global__ void __launch_bounds__(kThreads, 2)
                         const uint32_t a0 = kv8_decode2(x), a1 = kv8_decode2_hi(x);
                         const uint32_t a2 = kv8_decode2(y), a3 = kv8_decode2_hi(y);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma(o[nt][i], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                        for (int nt = 0; nt < NT; ++nt) mma(o[nt][i], a0, a1, a2, a3, pb[u][nt][0], pb[u][nt][1]);
                     }
                 }
                 ++got;
                 __syncwarp();  // every lane has read the slot
-                if (pro.issue(a, &mapK, &mapV, sm.ring[warp][slot], &sm.piece[warp][slot], &sm.full[warp][slot], warp, lane))
+                if (pro.issue(a, &mapK, &mapV, sm.ring[warp][slot], sm.meta[warp][slot], &sm.full[warp][slot], warp, lane))
                     ++put;
             }
             if (++slot == kDepth) slot = 0, phase ^= 1;
@@ -688,30 +738,17 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
 #pragma unroll
             for (int d = 0; d < D / kRow; ++d) {
-                // rows 2t, 2t + 1; this thread's channels of a box are contiguous, two a product row pair
-                constexpr int kOwn = kBox / 8;  // channels a thread has in a box
-                if constexpr (kRow == kBox) {
+                // rows 2t, 2t + 1; a thread has kOwn consecutive channels of a box, kRow / kOwn threads a join
+                constexpr int kOwn = kBox / 8, kSharers = kRow / kOwn, kJoins = kBox / kRow;
+                if (g / kSharers == d % kJoins) {
 #pragma unroll
                     for (int i = 0; i < kOwn / 2; i += 2) {
-                        const float(&x)[4] = o[nt][d * (kBox / 16) + i];
-                        const float(&y)[4] = o[nt][d * (kBox / 16) + i + 1];
-                        *reinterpret_cast<float4*>(&sm.join[warp][2 * t][kOwn * g + 2 * i]) =
+                        const float(&x)[4] = o[nt][(d / kJoins) * (kBox / 16) + i];
+                        const float(&y)[4] = o[nt][(d / kJoins) * (kBox / 16) + i + 1];
+                        *reinterpret_cast<float4*>(&sm.join[warp][2 * t][kOwn * (g % kSharers) + 2 * i]) =
                             make_float4(x[0] * f[0], x[2] * f[0], y[0] * f[0], y[2] * f[0]);
-                        *reinterpret_cast<float4*>(&sm.join[warp][2 * t + 1][kOwn * g + 2 * i]) =
+                        *reinterpret_cast<float4*>(&sm.join[warp][2 * t + 1][kOwn * (g % kSharers) + 2 * i]) =
                             make_float4(x[1] * f[1], x[3] * f[1], y[1] * f[1], y[3] * f[1]);
-                    }
-                } else {
-                    // half a box: the threads g of that half
-                    if ((g >> 2) == (d & 1)) {
-#pragma unroll
-                        for (int i = 0; i < kOwn / 2; i += 2) {
-                            const float(&x)[4] = o[nt][(d >> 1) * (kBox / 16) + i];
-                            const float(&y)[4] = o[nt][(d >> 1) * (kBox / 16) + i + 1];
-                            *reinterpret_cast<float4*>(&sm.join[warp][2 * t][kOwn * (g & 3) + 2 * i]) =
-                                make_float4(x[0] * f[0], x[2] * f[0], y[0] * f[0], y[2] * f[0]);
-                            *reinterpret_cast<float4*>(&sm.join[warp][2 * t + 1][kOwn * (g & 3) + 2 * i]) =
-                                make_float4(x[1] * f[1], x[3] * f[1], y[1] * f[1], y[3] * f[1]);
-                        }
                     }
                 }
                 __syncthreads();
@@ -789,7 +826,7 @@ __global__ void __launch_bounds__(256) attn_kv8_join_kernel(const Args a, int gr
     const int last = a.meta[4 * c];
     if (last < 0) return;
     const int b = a.meta[4 * c + 1], h = a.meta[4 * c + 2], rt = a.meta[4 * c + 3];
-    const Seq s = load_seq<NT>(a, b, false);
+    const Seq s = load_seq<D, NT>(a, b, false);
     const int row = rt * kRows + n;
     if (row >= s.n * a.group) return;
     const int parts = last - c + 1;
@@ -863,19 +900,26 @@ int column_tiles(int rows, int D) {
     return rows <= 8 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
 }
 
-int plan_grid() {
-    const int g = 2 * device_sm_count();
+int piece_keys(int D, int nt) {
+    return nt > 1 || D == 256 ? kGroup : D == 64 ? Cfg<64, 1>::kPiece : Cfg<128, 1>::kPiece;
+}
+static_assert(Cfg<256, 1>::kH == 1 && Cfg<64, 2>::kH == 1 && Cfg<128, 2>::kH == 1 && Cfg<64, 4>::kH == 1, "piece_keys");
+
+int plan_grid(int D, int nt, int sms) {
+    const int ctas = nt == 1 ? (D == 64 ? Cfg<64, 1>::kCtas : D == 128 ? Cfg<128, 1>::kCtas : Cfg<256, 1>::kCtas)
+                   : nt == 2 ? (D == 64 ? Cfg<64, 2>::kCtas : D == 128 ? Cfg<128, 2>::kCtas : Cfg<256, 2>::kCtas)
+                             : (D == 64 ? Cfg<64, 4>::kCtas : Cfg<128, 4>::kCtas);
+    const int g = ctas * sms;
     return g < kMaxGrid ? g : kMaxGrid;
 }
 
-size_t workspace_bytes(int nt, int D) {
-    const size_t rows = (size_t)plan_grid() * 2 * 8 * nt;
-    return rows * D * 4 + rows * 8 + (size_t)plan_grid() * 16;
+size_t workspace_bytes(int nt, int D, int sms) {
+    const size_t grid = plan_grid(D, nt, sms), rows = grid * 2 * 8 * nt;
+    return rows * D * 4 + rows * 8 + grid * 16;
 }
 
 template <int D, int NT, typename T>
-int launch(Args a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, cudaStream_t st) {
-    const int grid = plan_grid();
+int launch(Args a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid, cudaStream_t st) {
     const size_t rows = (size_t)grid * 2 * 8 * NT;
     a.part = static_cast<float*>(ws);
     a.meta = reinterpret_cast<int*>(a.part + rows * D + rows * 2);
@@ -890,19 +934,20 @@ int launch(Args a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, cudaS
 }
 
 template <int D, typename T>
-int launch_rows(int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, cudaStream_t st) {
-    if (nt == 1) return launch<D, 1, T>(a, mk, mv, ws, st);
-    if (nt == 2) return launch<D, 2, T>(a, mk, mv, ws, st);
-    if constexpr (D < 256) return launch<D, 4, T>(a, mk, mv, ws, st);
+int launch_rows(int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid, cudaStream_t st) {
+    if (nt == 1) return launch<D, 1, T>(a, mk, mv, ws, grid, st);
+    if (nt == 2) return launch<D, 2, T>(a, mk, mv, ws, grid, st);
+    if constexpr (D < 256) return launch<D, 4, T>(a, mk, mv, ws, grid, st);
     return B200LAB_ERR_UNSUPPORTED;
 }
 
 template <typename T>
-int launch_d(int D, int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, cudaStream_t st) {
+int launch_d(int D, int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid,
+             cudaStream_t st) {
     switch (D) {
-        case 64: return launch_rows<64, T>(nt, a, mk, mv, ws, st);
-        case 128: return launch_rows<128, T>(nt, a, mk, mv, ws, st);
-        default: return launch_rows<256, T>(nt, a, mk, mv, ws, st);
+        case 64: return launch_rows<64, T>(nt, a, mk, mv, ws, grid, st);
+        case 128: return launch_rows<128, T>(nt, a, mk, mv, ws, grid, st);
+        default: return launch_rows<256, T>(nt, a, mk, mv, ws, grid, st);
     }
 }
 
@@ -916,7 +961,7 @@ B200_DEFINE_ERR_TAKER(attn_kv8, b200::g_err_attn_kv8)
 extern "C" size_t attn_fwd_sm100_kv8_workspace(int Hq, int Hkv, int max_seqlen_q, int D) {
     if (Hq < 1 || Hkv < 1 || Hq % Hkv || max_seqlen_q < 1 || (D != 64 && D != 128 && D != 256)) return 0;
     const long long rows = (long long)(Hq / Hkv) * max_seqlen_q;
-    return b200::workspace_bytes(b200::column_tiles(rows < 64 ? (int)rows : 64, D), D);
+    return b200::workspace_bytes(b200::column_tiles(rows < 64 ? (int)rows : 64, D), D, b200::device_sm_count());
 }
 
 extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long long q_stride_head, const void* G,
@@ -942,7 +987,8 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     const long long rows = (long long)(Hq / Hkv) * most;
     if (rows > 0x40000000LL) return B200LAB_ERR_UNSUPPORTED;
     const int nt = column_tiles((int)rows, D);
-    if (!workspace || ws_bytes < workspace_bytes(nt, D)) return B200LAB_ERR_WORKSPACE;
+    const int sms = device_sm_count(), grid = plan_grid(D, nt, sms);
+    if (!workspace || ws_bytes < workspace_bytes(nt, D, sms)) return B200LAB_ERR_WORKSPACE;
     rc = check_device_sm100();
     if (rc != B200LAB_OK) return rc;
     Args a;
@@ -953,16 +999,18 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     a.max_seqlen_q = most, a.total_q = total_q, a.B = B, a.max_blocks = max_blocks, a.n_blocks = n_blocks;
     a.log2P = kv8_log2_block(block_size), a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv, a.causal = causal;
     a.scale = scale;
-    // the cache as [n_blocks * Hkv][block_size][D] bytes; a box is 16 tokens of up to 128 channels
+    // the cache as [n_blocks * Hkv][block_size][D] bytes; a box is box_rows tokens of up to 128 channels
     CUtensorMap mk, mv;
     const uint32_t box = D > 128 ? 128 : (uint32_t)D;
+    const int piece = piece_keys(D, nt);
+    a.box_rows = block_size < piece ? block_size : piece;
     const CUtensorMapSwizzle swizzle = D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
     for (int side = 0; side < 2; ++side) {
         rc = make_tmap_3d(side ? &mv : &mk, side ? v_cache : k_cache, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)D,
-                          (uint64_t)block_size, (uint64_t)n_blocks * Hkv, box, kPiece, swizzle);
+                          (uint64_t)block_size, (uint64_t)n_blocks * Hkv, box, (uint32_t)a.box_rows, swizzle);
         if (rc != B200LAB_OK) return rc;
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, a, mk, mv, workspace, st)
-                                : launch_d<__nv_bfloat16>(D, nt, a, mk, mv, workspace, st);
+    return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, a, mk, mv, workspace, grid, st)
+                                : launch_d<__nv_bfloat16>(D, nt, a, mk, mv, workspace, grid, st);
 }
