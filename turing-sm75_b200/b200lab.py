@@ -466,43 +466,10 @@ def gdn_decode_slots(q, k, v, g_log, beta, state_pool, slots, *, scale: float | 
 
 
 # ---- 8-bit key/value cache -------------------------------------------------
-class _On:
-    """Makes `device` current and `stream` (None: the device's current one) the stream that new
-    tensors belong to, where they are not already; .ptr is the stream's handle."""
-
-    __slots__ = ("ptr", "_ctx")
-
-    def __init__(self, device, stream):
-        cuda = _torch().cuda
-        self._ctx = []
-        if cuda.current_device() != device.index:
-            self._ctx.append(cuda.device(device))
-        cur = cuda.current_stream(device)
-        if stream is None:
-            stream = cur
-        elif stream.device != device:
-            raise ValueError("stream belongs to another device than the tensors")
-        elif stream != cur:
-            self._ctx.append(cuda.stream(stream))
-        self.ptr = stream.cuda_stream
-
-    def __enter__(self):
-        for c in self._ctx:
-            c.__enter__()
-        return self
-
-    def __exit__(self, *exc):
-        for c in reversed(self._ctx):
-            c.__exit__(*exc)
-        return False
-
-
-def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
-    """Checks of the cache's tensors; returns (n_blocks, Hkv, block_size, D)."""
+# These calls are made once a layer and token, so the checks are kept cheap: one condition over all
+# tensors, and the search for what it was only once it fails.
+def _kv8_refuse(k_cache, v_cache, k_scale, v_scale, block_table):
     torch = _torch()
-    dev = k_cache.device
-    if dev.type != "cuda":
-        raise ValueError("k_cache must be a CUDA tensor (no CPU path)")
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError("k_cache and v_cache must be [n_blocks, Hkv, block_size, D], alike")
     if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
@@ -513,17 +480,27 @@ def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
         raise TypeError("k_scale and v_scale must be float32")
     if block_table.dim() != 2 or block_table.dtype != torch.int32:
         raise ValueError("block_table must be int32 [B, max_blocks]")
-    for t in (k_cache, v_cache, k_scale, v_scale, block_table):
-        if not t.is_contiguous():
-            raise ValueError("the cache, its scales and the block table must be contiguous")
-        if t.device != dev:
-            raise ValueError("the cache, its scales and the block table must be on one device")
-    return k_cache.shape
+    raise ValueError("the cache, its scales and the block table must be contiguous CUDA tensors on one device")
+
+
+def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
+    """Checks of the cache's tensors; returns ((n_blocks, Hkv, block_size, D), device index)."""
+    torch = _torch()
+    shape, dev, e4m3 = k_cache.shape, k_cache.get_device(), torch.float8_e4m3fn
+    if dev < 0:
+        raise ValueError("k_cache must be a CUDA tensor (no CPU path)")
+    if not (len(shape) == 4 and v_cache.shape == shape and k_cache.dtype is e4m3 and v_cache.dtype is e4m3
+            and k_scale.shape == shape[:2] and v_scale.shape == shape[:2] and k_scale.dtype is torch.float32
+            and v_scale.dtype is torch.float32 and block_table.dtype is torch.int32 and block_table.dim() == 2
+            and v_cache.get_device() == dev and k_scale.get_device() == dev and v_scale.get_device() == dev
+            and block_table.get_device() == dev and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and k_scale.is_contiguous() and v_scale.is_contiguous() and block_table.is_contiguous()):
+        _kv8_refuse(k_cache, v_cache, k_scale, v_scale, block_table)
+    return shape, dev
 
 
 def _kv8_ints(t, n, name, dev):
-    torch = _torch()
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.device != dev:
+    if t.dtype is not _torch().int32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != dev:
         raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
     return t.data_ptr()
 
@@ -532,12 +509,32 @@ def _rows(t, shape, name, dev):
     """Checks of a token-major [total, H, D] tensor with contiguous channels; (pointer, strides)."""
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if t.device != dev:
+    if t.get_device() != dev:
         raise ValueError(f"{name} must be on the cache's device")
     st, sh, sd = t.stride()
     if sd != 1:
         raise ValueError(f"{name} must have contiguous channels")
     return t.data_ptr(), st, sh
+
+
+def _enter(dev, stream):
+    """(handle of the stream to launch on, context that makes device `dev` and that stream the
+    current ones, so that new tensors belong to them, or None where they are already)."""
+    torch = _torch()
+    if torch.cuda.current_device() == dev:
+        cur = torch._C._cuda_getCurrentRawStream(dev)  # torch.cuda.current_stream takes 2 us for it
+        if stream is None or stream.cuda_stream == cur:
+            return cur, None
+    elif stream is None:
+        stream = torch.cuda.current_stream(dev)
+    if stream.device_index != dev:
+        raise ValueError("stream belongs to another device than the tensors")
+    return stream.cuda_stream, torch.cuda.stream(stream)  # sets the device too
+
+
+def _entered(ctx, f, *args, **kw):
+    with ctx:
+        return f(*args, **kw)
 
 
 def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *, cu_seqlens=None,
@@ -548,24 +545,27 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, 
     block_table int32 [B,max_blocks]; seq_lens int32 [B], the new tokens counted; cu_seqlens int32
     [B+1] of the new tokens (None: one a sequence, seq_lens <= 0 marking padding) with max_seqlen
     the most of one sequence."""
-    n_blocks, Hkv, block_size, D = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
-    dev = k_cache.device
+    (n_blocks, Hkv, block_size, D), dev = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
     B, max_blocks = block_table.shape
     total = k.shape[0]
-    if v.dtype != k.dtype:
+    if v.dtype is not k.dtype:
         raise TypeError("k and v must share a dtype")
-    kp, kt, kh = _rows(k, (total, Hkv, D), "k", dev)
-    vp, vt, vh = _rows(v, (total, Hkv, D), "v", dev)
+    shape = (total, Hkv, D)
+    kp, kt, kh = _rows(k, shape, "k", dev)
+    vp, vt, vh = _rows(v, shape, "v", dev)
     lens = _kv8_ints(seq_lens, B, "seq_lens", dev)
-    cu = 0 if cu_seqlens is None else _kv8_ints(cu_seqlens, B + 1, "cu_seqlens", dev)
+    cu = None if cu_seqlens is None else _kv8_ints(cu_seqlens, B + 1, "cu_seqlens", dev)
     code = _dtype_code(k)
-    if total == 0 and cu_seqlens is not None:
+    if total == 0 and cu is not None:
         return
-    with _On(dev, stream) as on:
-        st = lib().kv8_append_sm100(kp, kt, kh, vp, vt, vh, k_cache.data_ptr(), v_cache.data_ptr(),
-                                    k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), lens, cu,
-                                    int(max_seqlen), total, B, max_blocks, n_blocks, block_size, Hkv, D, code, on.ptr)
-    _check(st, "kv8_append_sm100")
+    ptr, ctx = _enter(dev, stream)
+    args = (kp, kt, kh, vp, vt, vh, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            block_table.data_ptr(), lens, cu, int(max_seqlen), total, B, max_blocks, n_blocks, block_size, Hkv, D,
+            code, ptr)
+    f = lib().kv8_append_sm100
+    st = f(*args) if ctx is None else _entered(ctx, f, *args)
+    if st != OK:
+        raise B200LabError(st, "kv8_append_sm100")
 
 
 def kv8_read(k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, max_seqlen: int, total_tokens: int, *,
@@ -573,33 +573,40 @@ def kv8_read(k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, max_se
     """Read the first cu_seqlens[b+1] - cu_seqlens[b] tokens of each sequence back from the 8-bit
     cache, packed [total_tokens,Hkv,D] in out_dtype (fp16/bf16/fp32, default bf16).  Returns (k, v)."""
     torch = _torch()
-    n_blocks, Hkv, block_size, D = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
-    dev = k_cache.device
+    (n_blocks, Hkv, block_size, D), dev = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
     B, max_blocks = block_table.shape
     cu = _kv8_ints(cu_seqlens, B + 1, "cu_seqlens", dev)
     shape = (int(total_tokens), Hkv, D)
-    with _On(dev, stream) as on:
-        outs = []
+    ptr, ctx = _enter(dev, stream)
+    if ctx is not None:
+        return _entered(ctx, kv8_read, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, max_seqlen,
+                        total_tokens, out_dtype=out_dtype, k_out=k_out, v_out=v_out)
+    if k_out is None and v_out is None:
+        k_out = k_scale.new_empty(shape, dtype=out_dtype or torch.bfloat16)
+        v_out = torch.empty_like(k_out)
+    else:
+        if k_out is None or v_out is None:
+            raise ValueError("k_out and v_out go together")
         for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-            if t is None:
-                t = torch.empty(shape, dtype=out_dtype or torch.bfloat16, device=dev)
-            elif t.shape != shape or t.device != dev or not t.is_contiguous() or t.dtype != (out_dtype or t.dtype):
+            if (t.shape != shape or t.get_device() != dev or not t.is_contiguous() or t.dtype is not k_out.dtype
+                    or t.dtype is not (out_dtype or t.dtype)):
                 raise ValueError(f"{name} must be contiguous {list(shape)} of out_dtype on the cache's device")
-            outs.append(t)
-        if outs[0].dtype != outs[1].dtype:
-            raise TypeError("k_out and v_out must share a dtype")
-        if shape[0] > 0:
-            st = lib().kv8_read_sm100(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                      block_table.data_ptr(), cu, int(max_seqlen), shape[0], outs[0].data_ptr(),
-                                      outs[1].data_ptr(), B, max_blocks, n_blocks, block_size, Hkv, D,
-                                      _dtype_code(outs[0]), on.ptr)
-            _check(st, "kv8_read_sm100")
-    return outs[0], outs[1]
+    if shape[0] > 0:
+        st = lib().kv8_read_sm100(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                  block_table.data_ptr(), cu, int(max_seqlen), shape[0], k_out.data_ptr(),
+                                  v_out.data_ptr(), B, max_blocks, n_blocks, block_size, Hkv, D, _dtype_code(k_out),
+                                  ptr)
+        if st != OK:
+            raise B200LabError(st, "kv8_read_sm100")
+    return k_out, v_out
 
 
 def attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q=1, D=128) -> int:
-    """Workspace bytes of attn_fwd_kv8 (independent of batch and lengths)."""
+    """Workspace bytes of attn_fwd_kv8 (independent of batch and lengths) on the current device."""
     return int(lib().attn_fwd_sm100_kv8_workspace(Hq, Hkv, int(max_seqlen_q), D))
+
+
+_kv8_workspace = {}  # (device, Hq, Hkv, max_seqlen_q, D) -> 16-bit values of a workspace
 
 
 def attn_fwd_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *, cu_seqlens_q=None,
@@ -609,42 +616,49 @@ def attn_fwd_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *
     appended).  q [total_q,Hq,D] fp16/bf16, gate like q or None (out * sigmoid(gate)), both possibly
     strided views; cu_seqlens_q int32 [B+1] (None: one token a sequence) with max_seqlen_q the most of
     one sequence; the cache as in :func:`kv8_append`.  Returns [total_q,Hq,D]; rows that see no key are 0."""
-    torch = _torch()
-    n_blocks, Hkv, block_size, D = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
-    dev = k_cache.device
+    (n_blocks, Hkv, block_size, D), dev = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
     B, max_blocks = block_table.shape
     total, Hq = q.shape[0], q.shape[1]
     shape = (total, Hq, D)
     qp, qt, qh = _rows(q, shape, "q", dev)
-    gp, gt, gh = 0, 0, 0
+    gp = None
+    gt = gh = 0
     if gate is not None:
-        if gate.dtype != q.dtype:
+        if gate.dtype is not q.dtype:
             raise TypeError("gate must have q's dtype")
         gp, gt, gh = _rows(gate, shape, "gate", dev)
     lens = _kv8_ints(seq_lens, B, "seq_lens", dev)
-    cu = 0 if cu_seqlens_q is None else _kv8_ints(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
+    cu = None if cu_seqlens_q is None else _kv8_ints(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
     code = _dtype_code(q)
-    if out is not None and (out.shape != shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev):
+    ptr, ctx = _enter(dev, stream)
+    if ctx is not None:
+        return _entered(ctx, attn_fwd_kv8, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
+                        cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q, gate=gate, scale=scale, causal=causal,
+                        out=out, workspace=workspace)
+    if out is None:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError("out must be contiguous, like q, on the cache's device")
-    if workspace is not None and (not workspace.is_contiguous() or workspace.device != dev):
-        raise ValueError("workspace must be contiguous, on the cache's device")
-    if scale is None:
-        scale = 1.0 / (D ** 0.5)
-    with _On(dev, stream) as on:
-        if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=dev)
-        if total == 0 and cu_seqlens_q is not None:
-            return out
-        if workspace is None:
-            # at least a byte, so that wrong sizes reach the library's own checks
-            workspace = torch.empty(max(1, attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q, D)), dtype=torch.uint8,
-                                    device=dev)
-        st = lib().attn_fwd_sm100_kv8(qp, qt, qh, gp, gt, gh, k_cache.data_ptr(), v_cache.data_ptr(),
-                                      k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), lens, cu,
-                                      int(max_seqlen_q), total, out.data_ptr(), B, max_blocks, n_blocks, block_size,
-                                      Hq, Hkv, D, float(scale), int(bool(causal)), code, workspace.data_ptr(),
-                                      workspace.numel() * workspace.element_size(), on.ptr)
-    _check(st, "attn_fwd_sm100_kv8")
+    if total == 0 and cu is not None:
+        return out
+    if workspace is None:
+        key = (dev, Hq, Hkv, max_seqlen_q, D)
+        n = _kv8_workspace.get(key)
+        if n is None:  # at least a value, so that wrong sizes reach the library's own checks
+            n = _kv8_workspace[key] = max(1, attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q, D) // 2)
+        workspace = out.new_empty(n)
+        ws_bytes = n * out.element_size()
+    else:
+        if not workspace.is_contiguous() or workspace.get_device() != dev:
+            raise ValueError("workspace must be contiguous, on the cache's device")
+        ws_bytes = workspace.numel() * workspace.element_size()
+    st = lib().attn_fwd_sm100_kv8(qp, qt, qh, gp, gt, gh, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                                  v_scale.data_ptr(), block_table.data_ptr(), lens, cu, int(max_seqlen_q), total,
+                                  out.data_ptr(), B, max_blocks, n_blocks, block_size, Hq, Hkv, D,
+                                  D ** -0.5 if scale is None else float(scale), 1 if causal else 0, code,
+                                  workspace.data_ptr(), ws_bytes, ptr)
+    if st != OK:
+        raise B200LabError(st, "attn_fwd_sm100_kv8")
     return out
 
 

@@ -38,7 +38,7 @@ __device__ int g_err_attn_kv8 = 0;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kGroup = 16;                // keys of one product
-constexpr int kMaxGrid = 2048;            // more CTAs than any sm_100 part has resident here
+constexpr int kMaxGrid = 2048;            // CTAs of a call at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;              // the running maximum is moved when x exceeds it by 2^8
 
@@ -51,13 +51,12 @@ template <int D, int NT> struct Cfg {
     static constexpr int kCtas = NT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : 2;
     static constexpr int kDepth = (D == 64 ? (NT == 1 ? 5 : 10) : D == 128 ? (NT == 1 ? 4 : 5) : (NT == 1 ? 3 : 2)) / kH;
     static constexpr int kRow = 64;                         // channels joined at a time
+    static constexpr int kStart = 2;                        // what a segment's start and end cost, in tiles
 };
 
-struct GroupMeta {
-    float ks;   // scale of K
-    float lv;   // log2 of the scale of V
-    float iv;   // 1 / scale of V
-    int ok;     // 0: no key of the group is in the sequence, or its block id lies outside the pool
+struct GroupMeta {  // of 16 keys
+    float ks, vs;   // scales of K and V
+    int ok;         // 0: no key of the group is in the sequence, or its block id lies outside the pool
 };
 
 struct Args {
@@ -81,7 +80,10 @@ struct Args {
 struct Seq {
     int n, L, t0;      // query tokens, keys, first packed token
     int tiles, rts;    // key tiles and row tiles
-    __device__ __forceinline__ long long units(int Hkv) const { return (long long)tiles * rts * Hkv; }
+    // in the numbering of the plan, where a segment counts kStart tiles more than it has
+    template <int kStart> __device__ __forceinline__ long long units(int Hkv) const {
+        return tiles ? (long long)(tiles + kStart) * rts * Hkv : 0;
+    }
 };
 
 // A sequence whose offsets or length are outside what the call was given has no tiles and is reported.
@@ -104,18 +106,21 @@ template <int D, int NT> __device__ __forceinline__ Seq load_seq(const Args& a, 
     return s;
 }
 
-// A place in the numbered tiles: sequence, kv-head, row tile, key tile; `left` tiles of the CTA's
-// run from here on.
+// A place in the numbered tiles: sequence, kv-head, row tile, key tile (negative: in the kStart units
+// that stand for the segment's start); `left` units of the CTA's run from here on.
 template <int D, int NT> struct Cursor {
     Seq s;
     int b, h, rt, tile;
     long long left;
-    __device__ __forceinline__ int run() const { return (int)min((long long)(s.tiles - tile), left); }
-    // to the first tile of the next segment
+    // the CTA's tiles of this segment: [first, first + count), none where count <= 0
+    __device__ __forceinline__ int span() const { return (int)min((long long)(s.tiles - tile), left); }
+    __device__ __forceinline__ int first() const { return max(tile, 0); }
+    __device__ __forceinline__ int count() const { return tile + span() - first(); }
+    // to the next segment
     __device__ __forceinline__ void next(const Args& a) {
-        left -= run();
+        left -= span();
         if (left <= 0) return;
-        tile = 0;
+        tile = -Cfg<D, NT>::kStart;
         if (++rt < s.rts) return;
         rt = 0;
         if (++h < a.Hkv) return;
@@ -123,6 +128,22 @@ template <int D, int NT> struct Cursor {
         do {
             s = load_seq<D, NT>(a, ++b, false);
         } while (s.tiles == 0);  // ends: tiles are left
+    }
+};
+
+// The units [0, total) dealt to G CTAs: total % G CTAs have one more than the others.
+struct Deal {
+    long long each, more;
+    __device__ __forceinline__ Deal(long long total, int G) {
+        // 32-bit division, a fraction of the 64-bit one's time, wherever it does
+        each = total <= 0x7fffffffLL ? (long long)((uint32_t)total / (uint32_t)G) : total / G;
+        more = total - each * G;
+    }
+    __device__ __forceinline__ long long start(int c) const { return c * each + min((long long)c, more); }
+    __device__ __forceinline__ int holder(long long unit) const {
+        const long long big = more * (each + 1);  // units of the CTAs that have one more
+        if (unit < big) return (int)(unit / (each + 1));
+        return (int)(more + (unit - big) / each);
     }
 };
 
@@ -160,8 +181,7 @@ template <int D, int NT> struct Smem {
     float qscale[8 * NT];
     uint64_t full[kWarps][Cfg<D, NT>::kDepth];
     long long total[kWarps];
-    long long first_unit;
-    int first_b;
+    Cursor<D, NT> first;
     int abort;
 };
 
@@ -272,39 +292,40 @@ __device__ __forceinline__ float load_q(const T* q, int t, uint32_t (&f)[D / 16]
     return finite ? __uint_as_float((254u - field) << 23) : __uint_as_float(0x7fc00000u);
 }
 
+// 4 bytes global -> shared without waiting, and this thread's arrival at `bar` once its copies are
+// complete (which the barrier's count includes).
+__device__ __forceinline__ void copy_word(void* smem, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void arrive_when_copied(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // The pieces of one warp in the order it takes them, requested ahead of their use.
 template <int D, int NT> struct Producer {
     using C = Cfg<D, NT>;
     Cursor<D, NT> c;
-    int k;        // next tile of the segment, from c.tile
+    int k;        // next tile of the segment, from c.first()
     int block;    // lane i: of group i of the next 32 / kH pieces
-    float ks, lv, iv;
 
     // Requests the next piece into a ring slot; false: none is left.
     __device__ __forceinline__ bool issue(const Args& a, const CUtensorMap* mk, const CUtensorMap* mv, uint8_t* slot,
                                           GroupMeta* meta, uint64_t* bar, int warp, int lane) {
         for (;;) {
             if (c.left <= 0) return false;
-            if (k < c.run() && (c.tile + k) * C::kTile + warp * C::kPiece < c.s.L) break;
+            if (k < c.count() && (c.first() + k) * C::kTile + warp * C::kPiece < c.s.L) break;
             c.next(a);
             k = 0;
         }
         constexpr int kAhead = 32 / C::kH;
-        if ((k & (kAhead - 1)) == 0) {  // the block ids and scales of the next pieces, a group a lane
-            const int pos = (c.tile + k + lane / C::kH) * C::kTile + warp * C::kPiece + (lane % C::kH) * kGroup;
+        if ((k & (kAhead - 1)) == 0) {  // the block ids of the next pieces, a group a lane
+            const int pos = (c.first() + k + lane / C::kH) * C::kTile + warp * C::kPiece + (lane % C::kH) * kGroup;
             block = -1;
-            ks = lv = iv = 0.f;
-            if (k + lane / C::kH < c.run() && pos < c.s.L) {
+            if (k + lane / C::kH < c.count() && pos < c.s.L) {
                 block = a.table[(size_t)c.b * a.max_blocks + (pos >> a.log2P)];
                 if (block < 0 || block >= a.n_blocks) {
                     atomicExch(&g_err_attn_kv8, B200LAB_ERR_INVALID);
                     block = -1;
-                } else {
-                    ks = a.k_scale[(size_t)block * a.Hkv + c.h];
-                    const float vs = fminf(fmaxf(a.v_scale[(size_t)block * a.Hkv + c.h], kKv8MinScale), kKv8MaxScale);
-                    lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);
-                    if (__float_as_uint(vs) & 0x7fffffu) lv = log2f(vs);  // not a power of two
-                    iv = 1.f / vs;
                 }
             }
         }
@@ -312,8 +333,20 @@ template <int D, int NT> struct Producer {
         int blk[C::kH];
 #pragma unroll
         for (int u = 0; u < C::kH; ++u) blk[u] = __shfl_sync(0xffffffffu, block, first + u);
-        if (lane - first >= 0 && lane - first < C::kH) meta[lane - first] = GroupMeta{ks, lv, iv, block >= 0};
-        __syncwarp();  // before lane 0's arrival, which the readers wait for
+        // the scales come as copies of their own, so that nothing here waits for them: each of the lanes
+        // that hold the piece's groups arrives at the barrier once its two words are there
+        if (lane >= first && lane < first + C::kH) {
+            GroupMeta* m = meta + (lane - first);
+            m->ok = block >= 0;
+            if (block >= 0) {
+                const size_t bh = (size_t)block * a.Hkv + c.h;
+                copy_word(&m->ks, a.k_scale + bh);
+                copy_word(&m->vs, a.v_scale + bh);
+            } else {
+                m->ks = m->vs = 1.f;
+            }
+            arrive_when_copied(bar);
+        }
         if (lane == 0) {
             constexpr int kBox = D > 128 ? 128 : D;
             const int step = a.box_rows / kGroup;  // groups of a box, all of one block
@@ -325,7 +358,7 @@ template <int D, int NT> struct Producer {
             } else {
                 mbar_arrive(bar);
             }
-            const int pos = (c.tile + k) * C::kTile + warp * C::kPiece;
+            const int pos = (c.first() + k) * C::kTile + warp * C::kPiece;
 #pragma unroll
             for (int u = 0; u < C::kH; ++u) {
                 if (u % step != 0 || blk[u] < 0) continue;
@@ -339,6 +372,7 @@ template <int D, int NT> struct Producer {
                 }
             }
         }
+        __syncwarp();  // every lane sees m->ok
         ++k;
         return true;
     }
@@ -416,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
         sm.abort = 0;
     }
     if (lane == 0) {
-        for (int i = 0; i < kDepth; ++i) mbar_init(&sm.full[warp][i], 1);
+        for (int i = 0; i < kDepth; ++i) mbar_init(&sm.full[warp][i], 1 + kH);  // the copies, a lane a group's scales
         fence_barrier_init();
     }
     // Launched early, but lets the join kernel start only as its CTAs end (the default): a join CTA that
@@ -429,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
     const int share = (a.B + kThreads - 1) / kThreads;
     const int b0 = min(a.B, tid * share), b1 = min(a.B, b0 + share);
     long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += load_seq<D, NT>(a, b, blockIdx.x == 0).units(a.Hkv);
+    for (int b = b0; b < b1; ++b) mine += load_seq<D, NT>(a, b, blockIdx.x == 0).units<Cfg<D, NT>::kStart>(a.Hkv);
     long long upto = mine;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -444,36 +478,36 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
         if (w < warp) upto += sm.total[w];
         total += sm.total[w];
     }
-    const long long G = min((long long)gridDim.x, total);
-    if (blockIdx.x >= G) {
+    const int G = (int)min((long long)gridDim.x, total);
+    if ((int)blockIdx.x >= G) {
         if (tid == 0) a.meta[4 * blockIdx.x] = -1;
         return;
     }
-    const long long u0 = blockIdx.x * total / G, u1 = (blockIdx.x + 1) * total / G;
+    const Deal deal(total, G);
+    const long long u0 = deal.start(blockIdx.x), u1 = deal.start(blockIdx.x + 1);
     if (upto - mine <= u0 && u0 < upto) {
         long long at = upto - mine;
         int b = b0;
+        Seq s;
         for (;; ++b) {
-            const long long n = load_seq<D, NT>(a, b, false).units(a.Hkv);
+            s = load_seq<D, NT>(a, b, false);
+            const long long n = s.units<C::kStart>(a.Hkv);
             if (u0 < at + n) break;
             at += n;
         }
-        sm.first_b = b;
-        sm.first_unit = at;
+        // the segment and the tile in it; a sequence's units fit 32 bits nearly always
+        const long long local = u0 - at;
+        const int per = s.tiles + C::kStart;
+        const long long seg = local <= 0x7fffffffLL ? (long long)((uint32_t)local / (uint32_t)per) : local / per;
+        sm.first.s = s;
+        sm.first.b = b;
+        sm.first.tile = (int)(local - seg * per) - C::kStart;
+        sm.first.h = (int)(seg / s.rts);
+        sm.first.rt = (int)(seg - (long long)sm.first.h * s.rts);
+        sm.first.left = u1 - u0;
     }
     __syncthreads();
-
-    Cursor<D, NT> cur;
-    cur.b = sm.first_b;
-    cur.s = load_seq<D, NT>(a, cur.b, false);
-    {
-        const long long local = u0 - sm.first_unit;
-        const long long seg = local / cur.s.tiles;
-        cur.tile = (int)(local - seg * cur.s.tiles);
-        cur.h = (int)(seg / cur.s.rts);
-        cur.rt = (int)(seg - (long long)cur.h * cur.s.rts);
-        cur.left = u1 - u0;
-    }
+    Cursor<D, NT> cur = sm.first;
 
     Producer<D, NT> pro;
     pro.c = cur;
@@ -485,8 +519,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
         if (!pro.issue(a, &mapK, &mapV, sm.ring[warp][put], sm.meta[warp][put], &sm.full[warp][put], warp, lane)) break;
 
     bool has_tail = false;  // whether the run's last segment goes on in the next CTA's
-    while (cur.left > 0) {
-        const int run = cur.run();
+    for (; cur.left > 0; cur.next(a)) {
+        const int first = cur.first(), run = cur.count();
+        if (run <= 0) continue;  // the cut lies in the segment's start: the next CTA has it
         const Seq& s = cur.s;
         const int row0 = cur.rt * kRows, rows = min(kRows, s.n * a.group - row0);
 
@@ -540,19 +575,28 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
         const int all_see = a.causal ? s.L - s.n + row0 / a.group + 1 : s.L;
 
         for (int k = 0; k < run; ++k) {
-            const int base = (cur.tile + k) * kTile + warp * kPiece;
+            const int base = (first + k) * kTile + warp * kPiece;
             if (base >= s.L) break;
             if (alive)  // agreed by the warp: every lane goes the same way on
                 alive = __all_sync(0xffffffffu, mbar_wait(&sm.full[warp][slot], phase, &sm.abort, &g_err_attn_kv8));
             if (alive) {
                 const uint8_t* ks_ = sm.ring[warp][slot];
                 const uint8_t* vs_ = ks_ + kPiece * D;
-                GroupMeta meta[kH];
-                bool whole_piece = true;
+                // scale of K, log2 and inverse of the scale of V: powers of two, whose exponents are read off
+                // (a scale that is none takes the long way)
+                float gk[kH], gl[kH], gi[kH];
+                bool ok[kH], whole_piece = true;
 #pragma unroll
                 for (int u = 0; u < kH; ++u) {
-                    meta[u] = sm.meta[warp][slot][u];
-                    whole_piece = whole_piece && meta[u].ok;
+                    const GroupMeta m = sm.meta[warp][slot][u];
+                    const float v = fminf(fmaxf(m.vs, kKv8MinScale), kKv8MaxScale);
+                    const uint32_t bits = __float_as_uint(v);
+                    gk[u] = m.ks;
+                    gl[u] = (float)((int)(bits >> 23) - 127);
+                    gi[u] = __uint_as_float((254u << 23) - bits);
+                    if (bits & 0x7fffffu) gl[u] = log2f(v), gi[u] = 1.f / v;
+                    ok[u] = m.ok;
+                    whole_piece = whole_piece && m.ok;
                 }
                 // ---- S^T = K Q^T (16 keys x 8 rows a group and column tile); a lone group has two partial
                 // sums, to shorten the chain of products
@@ -610,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float x = kAcc == 2 ? sc[u][nt][0][i] + sc[u][nt][kAcc - 1][i] : sc[u][nt][0][i];
-                            sc[u][nt][0][i] = fmaf(x, qs[nt][i & 1] * meta[u].ks, meta[u].lv);
+                            sc[u][nt][0][i] = fmaf(x, qs[nt][i & 1] * gk[u], gl[u]);
                         }
                         if (edge) {
 #pragma unroll
@@ -618,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                                 const int key = base + u * kGroup + kr + (i >> 1) * 8;
                                 const int row = row0 + nt * 8 + 2 * t + (i & 1);
                                 const int sees = a.causal ? s.L - s.n + row / a.group + 1 : s.L;
-                                if (key >= min(sees, s.L) || !meta[u].ok) sc[u][nt][0][i] = -INFINITY;
+                                if (key >= min(sees, s.L) || !ok[u]) sc[u][nt][0][i] = -INFINITY;
                             }
                         }
                     }
@@ -660,8 +704,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                     for (int u = 0; u < kH; ++u) {
                         const float p0 = ex2(sc[u][nt][0][0] - m0), p1 = ex2(sc[u][nt][0][1] - m1);
                         const float p2 = ex2(sc[u][nt][0][2] - m0), p3 = ex2(sc[u][nt][0][3] - m1);
-                        l[nt][0] = fmaf(p0 + p2, meta[u].iv, l[nt][0]);
-                        l[nt][1] = fmaf(p1 + p3, meta[u].iv, l[nt][1]);
+                        l[nt][0] = fmaf(p0 + p2, gi[u], l[nt][0]);
+                        l[nt][1] = fmaf(p1 + p3, gi[u], l[nt][1]);
                         // the weights are rounded to fp16 (2^-11 relative; the sum l is not, its rounding
                         // errors would not cancel theirs)
                         pb[u][nt][0] = transpose8x8(pack_h2(p0, p1));
@@ -687,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                                 w[box][q][0] = x.x, w[box][q][1] = x.y, w[box][q][2] = x.z, w[box][q][3] = x.w;
                             }
                         }
-                    if (edge) take_out_masked<D, NT>(a, s, w, o, r, base + u * kGroup, meta[u].ok, row0 + g);
+                    if (edge) take_out_masked<D, NT>(a, s, w, o, r, base + u * kGroup, ok[u], row0 + g);
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) {
                         const int box = i / (kBox / 16), j = (i % (kBox / 16)) >> 1;
@@ -721,8 +765,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                 }
             }
         __syncthreads();
-        const bool whole = cur.tile == 0 && run == s.tiles;
-        const int part = blockIdx.x * 2 + (cur.tile == 0 ? 1 : 0);
+        const bool whole = first == 0 && run == s.tiles;
+        const int part = blockIdx.x * 2 + (first == 0 ? 1 : 0);
         constexpr int kRow = Smem<D, NT>::kRow, kPer = kRow / 16;
         const int jr = tid >> 4, jd = (tid & 15) * kPer;  // this thread's row of a column tile, and channels
 #pragma unroll
@@ -788,17 +832,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                 __syncthreads();
             }
         }
-        if (cur.tile == 0 && run < s.tiles) {
+        if (first == 0 && run < s.tiles) {
             has_tail = true;
             if (tid == 0) {
-                const long long end = u1 - cur.left + s.tiles;  // the segment's end
-                a.meta[4 * blockIdx.x] = (int)((end * G - 1) / total);  // the CTA whose run holds its last tile
-                a.meta[4 * blockIdx.x + 1] = cur.b;
-                a.meta[4 * blockIdx.x + 2] = cur.h;
-                a.meta[4 * blockIdx.x + 3] = cur.rt;
+                const long long end = u1 - cur.left + (s.tiles - cur.tile);  // the segment's end
+                a.meta[4 * blockIdx.x] = deal.holder(end - 1);  // the CTA whose run holds its last tile
+                a.meta[4 * blockIdx.x + 1] = s.t0;
+                a.meta[4 * blockIdx.x + 2] = cur.h * a.group;
+                a.meta[4 * blockIdx.x + 3] = row0 | rows << 24;
             }
         }
-        cur.next(a);
     }
     if (!has_tail && tid == 0) a.meta[4 * blockIdx.x] = -1;
     if (!alive) {
@@ -813,83 +856,90 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
     }
 }
 
-// Joins the segments that were cut.  Block (c, n): row n of the segment whose first part CTA c left;
-// its other parts are the first ones of the CTAs c + 1 .. last.  The 8 warps share the parts.
+// Joins the segments that were cut.  Block (c, y): rows y * per_block .. of the segment whose first
+// part CTA c left; its other parts are the first ones of the CTAs c + 1 .. last.  8 / per_block warps
+// share the parts of a row, each with a maximum of its own, so that all loads of a warp are under way
+// at once behind the one of the segment's description.
+constexpr int kJoinAhead = 4;  // parts a warp loads at a time
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(256) attn_kv8_join_kernel(const Args a, int grid) {
+__global__ void __launch_bounds__(256) attn_kv8_join_kernel(const Args a, int grid, int per_block) {
     constexpr int kRows = 8 * NT, kVec = D / 32;  // channels of a lane
-    __shared__ float weight[kMaxGrid];
-    __shared__ float red[8], acc[8][D];
+    __shared__ float acc[8][D];
+    __shared__ float2 stat[8];
     grid_dependency_wait();
     allow_dependent_launch();
-    const int c = blockIdx.x, n = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int last = a.meta[4 * c];
+    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int4 d = reinterpret_cast<const int4*>(a.meta)[c];
+    const int last = d.x, row0 = d.w & 0xffffff, rows = d.w >> 24;
     if (last < 0) return;
-    const int b = a.meta[4 * c + 1], h = a.meta[4 * c + 2], rt = a.meta[4 * c + 3];
-    const Seq s = load_seq<D, NT>(a, b, false);
-    const int row = rt * kRows + n;
-    if (row >= s.n * a.group) return;
-    const int parts = last - c + 1;
+    const int sharers = 8 / per_block;
+    const int n = blockIdx.y * per_block + warp / sharers;
+    const int parts = n < rows ? last - c + 1 : 0;
     const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)grid * 2 * kRows * D);
-    auto at = [&](int p) { return (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * kRows + n; };
-    float M = -INFINITY;
-    for (int p = tid; p < parts; p += 256) {
-        const float x = ml[at(p)].x;
-        weight[p] = x;
-        M = fmaxf(M, x);
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-    if (lane == 0) red[warp] = M;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, red[w]);
-    __syncthreads();
-    float sum = 0.f;
-    for (int p = tid; p < parts; p += 256) {
-        const float lp = ml[at(p)].y, f = part_weight(weight[p], lp, M);
-        weight[p] = f;
-        sum += lp * f;
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    if (lane == 0) red[warp] = sum;
-    __syncthreads();
-    sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) sum += red[w];
-    float x[kVec];
+    float M = -INFINITY, sum = 0.f, x[kVec];
 #pragma unroll
     for (int u = 0; u < kVec; ++u) x[u] = 0.f;
-#pragma unroll 4
-    for (int p = warp; p < parts; p += 8) {
-        const float f = weight[p];
-        const float* src = a.part + at(p) * D + lane * kVec;
-        float y[kVec];
+    for (int p0 = warp % sharers; p0 < parts; p0 += sharers * kJoinAhead) {
+        float2 st[kJoinAhead];
+        float y[kJoinAhead][kVec];
 #pragma unroll
-        for (int u = 0; u < kVec; u += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(src + u);
-            y[u] = v.x;
-            y[u + 1] = v.y;
+        for (int i = 0; i < kJoinAhead; ++i) {
+            const int p = p0 + i * sharers;
+            st[i] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int u = 0; u < kVec; ++u) y[i][u] = 0.f;
+            if (p < parts) {
+                const size_t at = (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * kRows + n;
+                st[i] = ml[at];
+                const float* src = a.part + at * D + lane * kVec;
+#pragma unroll
+                for (int u = 0; u < kVec; u += 2) {
+                    const float2 v = *reinterpret_cast<const float2*>(src + u);
+                    y[i][u] = v.x;
+                    y[i][u + 1] = v.y;
+                }
+            }
         }
+        float to = M;
 #pragma unroll
-        for (int u = 0; u < kVec; ++u) x[u] = fmaf(f, y[u], x[u]);
+        for (int i = 0; i < kJoinAhead; ++i) to = fmaxf(to, st[i].x);
+        const float f = part_weight(M, sum, to);
+        sum *= f;
+#pragma unroll
+        for (int u = 0; u < kVec; ++u) x[u] *= f;
+#pragma unroll
+        for (int i = 0; i < kJoinAhead; ++i) {
+            const float w = part_weight(st[i].x, st[i].y, to);
+            sum = fmaf(w, st[i].y, sum);
+#pragma unroll
+            for (int u = 0; u < kVec; ++u) x[u] = fmaf(w, y[i][u], x[u]);
+        }
+        M = to;
     }
+    if (lane == 0) stat[warp] = make_float2(M, sum);
 #pragma unroll
     for (int u = 0; u < kVec; ++u) acc[warp][lane * kVec + u] = x[u];
     __syncthreads();
-    if (tid < D / 4) {
-        float y[4] = {0.f, 0.f, 0.f, 0.f};
+    // the warps' sums of each row, 4 channels a thread
+    for (int i = threadIdx.x; i < per_block * (D / 4); i += 256) {
+        const int r = i / (D / 4), ch = (i % (D / 4)) * 4;
+        const int m = blockIdx.y * per_block + r;
+        if (m >= rows) continue;
+        float all = -INFINITY;
+        for (int w = r * sharers; w < (r + 1) * sharers; ++w) all = fmaxf(all, stat[w].x);
+        float y[4] = {0.f, 0.f, 0.f, 0.f}, s = 0.f;
+        for (int w = r * sharers; w < (r + 1) * sharers; ++w) {
+            const float f = part_weight(stat[w].x, stat[w].y, all);
+            s = fmaf(f, stat[w].y, s);
 #pragma unroll
-        for (int w = 0; w < 8; ++w)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) y[u] += acc[w][tid * 4 + u];
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            for (int u = 0; u < 4; ++u) y[u] = fmaf(f, acc[w][ch + u], y[u]);
+        }
+        const float inv = s == 0.f ? 0.f : 1.f / s;
 #pragma unroll
         for (int u = 0; u < 4; ++u) y[u] *= inv;
-        int i, hg;
-        row_place(row, a.group, i, hg);
-        store_row<T, 4>(a, (size_t)(s.t0 + i), h * a.group + hg, D, tid * 4, y);
+        int token, hg;
+        row_place(row0 + m, a.group, token, hg);
+        store_row<T, 4>(a, (size_t)(d.y + token), d.z + hg, D, ch, y);
     }
 }
 
@@ -919,35 +969,47 @@ size_t workspace_bytes(int nt, int D, int sms) {
 }
 
 template <int D, int NT, typename T>
-int launch(Args a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid, cudaStream_t st) {
+int launch(Args a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid, int device,
+           cudaStream_t st) {
     const size_t rows = (size_t)grid * 2 * 8 * NT;
     a.part = static_cast<float*>(ws);
     a.meta = reinterpret_cast<int*>(a.part + rows * D + rows * 2);
     constexpr size_t smem = sizeof(Smem<D, NT>) + 1024;
     auto kern = attn_kv8_kernel<D, NT, T>;
-    B200_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<unsigned long long> ready{0};  // devices whose limit is raised
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (!bit || !(ready.load(std::memory_order_relaxed) & bit)) {
+        B200_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
     int rc = kv8_launch(kern, dim3(grid), kThreads, smem, st, mk, mv, a);
     if (rc != B200LAB_OK) return rc;
     const long long used = (long long)a.group * a.max_seqlen_q;
-    const int y = (int)(used < 8 * NT ? used : 8 * NT);
-    return kv8_launch(attn_kv8_join_kernel<D, NT, T>, dim3(grid, y), 256, 0, st, a, grid);
+    const int rows_used = (int)(used < 8 * NT ? used : 8 * NT);
+    // Rows a block joins: eight, a warp each, where a segment is cut into two or three parts (many
+    // segments, or few tiles), down to one with eight warps on its parts where segments are few.
+    const int parts = grid / (a.B < grid / a.Hkv ? a.B * a.Hkv : grid) + 2;
+    const int per_block = parts <= 4 ? 8 : parts <= 8 ? 4 : parts <= 16 ? 2 : 1;
+    return kv8_launch(attn_kv8_join_kernel<D, NT, T>, dim3(grid, (rows_used + per_block - 1) / per_block), 256, 0, st, a,
+                      grid, per_block);
 }
 
 template <int D, typename T>
-int launch_rows(int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid, cudaStream_t st) {
-    if (nt == 1) return launch<D, 1, T>(a, mk, mv, ws, grid, st);
-    if (nt == 2) return launch<D, 2, T>(a, mk, mv, ws, grid, st);
-    if constexpr (D < 256) return launch<D, 4, T>(a, mk, mv, ws, grid, st);
+int launch_rows(int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid, int device,
+           cudaStream_t st) {
+    if (nt == 1) return launch<D, 1, T>(a, mk, mv, ws, grid, device, st);
+    if (nt == 2) return launch<D, 2, T>(a, mk, mv, ws, grid, device, st);
+    if constexpr (D < 256) return launch<D, 4, T>(a, mk, mv, ws, grid, device, st);
     return B200LAB_ERR_UNSUPPORTED;
 }
 
 template <typename T>
 int launch_d(int D, int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid,
-             cudaStream_t st) {
+             int device, cudaStream_t st) {
     switch (D) {
-        case 64: return launch_rows<64, T>(nt, a, mk, mv, ws, grid, st);
-        case 128: return launch_rows<128, T>(nt, a, mk, mv, ws, grid, st);
-        default: return launch_rows<256, T>(nt, a, mk, mv, ws, grid, st);
+        case 64: return launch_rows<64, T>(nt, a, mk, mv, ws, grid, device, st);
+        case 128: return launch_rows<128, T>(nt, a, mk, mv, ws, grid, device, st);
+        default: return launch_rows<256, T>(nt, a, mk, mv, ws, grid, device, st);
     }
 }
 
@@ -985,12 +1047,12 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     if (G && (g_stride_token < 0 || g_stride_head < 0)) return B200LAB_ERR_INVALID;
     const int most = max_seqlen_q < total_q ? max_seqlen_q : total_q;
     const long long rows = (long long)(Hq / Hkv) * most;
-    if (rows > 0x40000000LL) return B200LAB_ERR_UNSUPPORTED;
+    if (rows > 0xffffffLL) return B200LAB_ERR_UNSUPPORTED;  // 24 bits in a segment's description
     const int nt = column_tiles((int)rows, D);
-    const int sms = device_sm_count(), grid = plan_grid(D, nt, sms);
+    const Kv8Device dev = kv8_device();
+    const int sms = dev.sms > 0 ? dev.sms : device_sm_count(), grid = plan_grid(D, nt, sms);
     if (!workspace || ws_bytes < workspace_bytes(nt, D, sms)) return B200LAB_ERR_WORKSPACE;
-    rc = check_device_sm100();
-    if (rc != B200LAB_OK) return rc;
+    if (dev.status != B200LAB_OK) return dev.status;
     Args a;
     a.q = Q, a.g = G, a.o = O;
     a.q_st = q_stride_token, a.q_sh = q_stride_head, a.g_st = g_stride_token, a.g_sh = g_stride_head;
@@ -1011,6 +1073,6 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
         if (rc != B200LAB_OK) return rc;
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, a, mk, mv, workspace, grid, st)
-                                : launch_d<__nv_bfloat16>(D, nt, a, mk, mv, workspace, grid, st);
+    return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, a, mk, mv, workspace, grid, dev.ordinal, st)
+                                : launch_d<__nv_bfloat16>(D, nt, a, mk, mv, workspace, grid, dev.ordinal, st);
 }

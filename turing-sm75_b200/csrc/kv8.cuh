@@ -13,6 +13,8 @@
 
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace b200 {
@@ -66,6 +68,29 @@ inline int kv8_check_cache(const void* k_cache, const void* v_cache, const float
     // positions and lengths are 32-bit
     if ((long long)max_blocks * block_size > 0x40000000LL) return B200LAB_ERR_UNSUPPORTED;
     return B200LAB_OK;
+}
+
+// What the launches need to know of the current device, asked of the runtime once a device: its
+// ordinal (-1 on an error), whether it is an sm_100 part, its SMs.
+struct Kv8Device {
+    int ordinal, sms;
+    int status;
+};
+inline Kv8Device kv8_device() {
+    constexpr int kMost = 64;
+    static std::atomic<int> seen[kMost];  // 0: not asked yet, else 2 * SMs + (an sm_100 part)
+    Kv8Device d = {-1, 0, B200LAB_ERR_CUDA};
+    if (cudaGetDevice(&d.ordinal) != cudaSuccess) return d;
+    int v = d.ordinal < kMost ? seen[d.ordinal].load(std::memory_order_relaxed) : 0;
+    if (v == 0) {
+        const int rc = check_device_sm100();
+        if (rc == B200LAB_ERR_CUDA) return d;
+        v = 2 * device_sm_count() + (rc == B200LAB_OK);
+        if (d.ordinal < kMost) seen[d.ordinal].store(v, std::memory_order_relaxed);
+    }
+    d.sms = v >> 1;
+    d.status = (v & 1) ? B200LAB_OK : B200LAB_ERR_DEVICE;
+    return d;
 }
 
 // Launches `kern` with programmatic stream serialisation: every kernel of this cache waits

@@ -302,7 +302,7 @@ extern "C" int kv8_append_sm100(const void* k, long long k_stride_token, long lo
     a.items_per_seq = (int)(touched < max_blocks ? touched : max_blocks);
     a.items = 2LL * B * a.items_per_seq * Hkv;
     if (a.items > 0x7fffffffLL) return B200LAB_ERR_UNSUPPORTED;
-    rc = check_device_sm100();
+    rc = kv8_device().status;
     if (rc != B200LAB_OK) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const long long values = (long long)(most < block_size ? most : block_size) * D;
@@ -337,7 +337,7 @@ extern "C" int kv8_read_sm100(const void* k_cache, const void* v_cache, const fl
     const long long per_cta = (long long)kReadThreads * kReadVecs;
     const long long grid = (a.vecs + per_cta - 1) / per_cta;
     if (grid > 0x7fffffffLL) return B200LAB_ERR_UNSUPPORTED;
-    rc = check_device_sm100();
+    rc = kv8_device().status;
     if (rc != B200LAB_OK) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const dim3 g((unsigned)grid);
