@@ -48,8 +48,8 @@ template <int D, int NT> struct Cfg {
     static constexpr int kPiece = kGroup * kH;
     static constexpr int kTile = kPiece * kWarps;           // keys a CTA takes at a time
     static constexpr int kBytes = 2 * kPiece * D;           // a piece of K, then one of V
-    static constexpr int kCtas = NT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : 2;
-    static constexpr int kDepth = (D == 64 ? (NT == 1 ? 5 : 10) : D == 128 ? (NT == 1 ? 4 : 5) : (NT == 1 ? 3 : 2)) / kH;
+    static constexpr int kCtas = NT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : NT == 2 && D <= 128 ? 3 : 2;
+    static constexpr int kDepth = (D == 64 ? (NT == 1 ? 5 : NT == 2 ? 6 : 10) : D == 128 ? (NT == 1 ? 4 : NT == 2 ? 3 : 5) : (NT == 1 ? 3 : 2)) / kH;
     static constexpr int kRow = 64;                         // channels joined at a time
     static constexpr int kStart = 2;                        // what a segment's start and end cost, in tiles
 };
@@ -110,10 +110,9 @@ template <int D, int NT> __device__ __forceinline__ Seq load_seq(const Args& a, 
 // that stand for the segment's start); `left` units of the CTA's run from here on.
 template <int D, int NT> struct Cursor {
     Seq s;
-    int b, h, rt, tile;
-    long long left;
+    int b, h, rt, tile, left;  // (a CTA's run fits 32 bits: 2^31 tiles would take it hours)
     // the CTA's tiles of this segment: [first, first + count), none where count <= 0
-    __device__ __forceinline__ int span() const { return (int)min((long long)(s.tiles - tile), left); }
+    __device__ __forceinline__ int span() const { return min(s.tiles - tile, left); }
     __device__ __forceinline__ int first() const { return max(tile, 0); }
     __device__ __forceinline__ int count() const { return tile + span() - first(); }
     // to the next segment
@@ -191,40 +190,38 @@ __device__ __forceinline__ float part_weight(float m, float l, float M) {
     return m == -INFINITY && l == l ? 0.f : ex2(m - M);
 }
 
-// One output value of a row: the gate, and the rounding to the output type.
-template <typename T> __device__ __forceinline__ float gated(float o, float g) { return o / (1.f + __expf(-g)); }
-
 // Row n of a row tile -> query token of the sequence and head of the group.
 __device__ __forceinline__ void row_place(int row, int group, int& i, int& hg) {
     i = row / group;
     hg = row - i * group;
 }
 
-// kPer consecutive output channels of one row.
-template <typename T, int kPer>
-__device__ __forceinline__ void store_row(const Args& a, size_t token, int head, int D, int d0, const float (&x)[kPer]) {
-    float y[kPer];
-#pragma unroll
-    for (int u = 0; u < kPer; ++u) y[u] = x[u];
-    if (a.g) {
+// kPer consecutive channels of a row: the gate's, and the gated outputs' store.
+template <typename T, int kPer> struct Channels {
+    T v[kPer];
+    __device__ __forceinline__ void load_gate(const Args& a, size_t token, int head, int d0) {
         const T* g = static_cast<const T*>(a.g) + token * a.g_st + (size_t)head * a.g_sh + d0;
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) y[u] = gated<T>(y[u], Elem<T>::to_f(g[u]));
+        for (int u = 0; u < kPer; ++u) v[u] = g[u];
     }
-    T* o = static_cast<T*>(a.o) + (token * a.Hq + head) * (size_t)D + d0;
-    if constexpr (kPer % 8 == 0) {
+};
+template <typename T, int kPer>
+__device__ __forceinline__ void store_row(const Args& a, size_t token, int head, int D, int d0, const float (&x)[kPer],
+                                          const Channels<T, kPer>& gate) {
+    float y[kPer];
 #pragma unroll
-        for (int u = 0; u < kPer; u += 8) {
-            uint4 w;
-            w.x = Elem<T>::pack2(y[u], y[u + 1]);
-            w.y = Elem<T>::pack2(y[u + 2], y[u + 3]);
-            w.z = Elem<T>::pack2(y[u + 4], y[u + 5]);
-            w.w = Elem<T>::pack2(y[u + 6], y[u + 7]);
-            *reinterpret_cast<uint4*>(o + u) = w;
-        }
+    for (int u = 0; u < kPer; ++u) y[u] = a.g ? x[u] / (1.f + __expf(-Elem<T>::to_f(gate.v[u]))) : x[u];
+    uint32_t w[kPer / 2];
+#pragma unroll
+    for (int u = 0; u < kPer; u += 2) w[u / 2] = Elem<T>::pack2(y[u], y[u + 1]);
+    uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + (token * a.Hq + head) * (size_t)D + d0);
+    if constexpr (kPer == 8) {
+        *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if constexpr (kPer == 4) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
     } else {
-        static_assert(kPer == 4, "");
-        *reinterpret_cast<uint2*>(o) = make_uint2(Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3]));
+        static_assert(kPer == 2, "");
+        *o = w[0];
     }
 }
 
@@ -396,7 +393,7 @@ __device__ __forceinline__ void take_out_masked(const Args& a, const Seq& s, uin
                 if (base + r[q] >= s.L || !ok) w[box][q][j] = 0;
                 nan |= ((w[box][q][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
             }
-    if (!__any_sync(0xffffffffu, nan != 0)) return;
+    if (__builtin_expect(!__any_sync(0xffffffffu, nan != 0), 1)) return;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int sees = min(a.causal ? s.L - s.n + (row + nt * 8) / a.group + 1 : s.L, s.L);
@@ -463,7 +460,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
     const int share = (a.B + kThreads - 1) / kThreads;
     const int b0 = min(a.B, tid * share), b1 = min(a.B, b0 + share);
     long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += load_seq<D, NT>(a, b, blockIdx.x == 0).units<Cfg<D, NT>::kStart>(a.Hkv);
+    Seq own;  // the last of the share: with up to 128 sequences, the only one
+    for (int b = b0; b < b1; ++b) {
+        own = load_seq<D, NT>(a, b, blockIdx.x == 0);
+        mine += own.units<C::kStart>(a.Hkv);
+    }
     long long upto = mine;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -490,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
         int b = b0;
         Seq s;
         for (;; ++b) {
-            s = load_seq<D, NT>(a, b, false);
+            s = b == b1 - 1 ? own : load_seq<D, NT>(a, b, false);
             const long long n = s.units<C::kStart>(a.Hkv);
             if (u0 < at + n) break;
             at += n;
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
         sm.first.tile = (int)(local - seg * per) - C::kStart;
         sm.first.h = (int)(seg / s.rts);
         sm.first.rt = (int)(seg - (long long)sm.first.h * s.rts);
-        sm.first.left = u1 - u0;
+        sm.first.left = (int)(u1 - u0);
     }
     __syncthreads();
     Cursor<D, NT> cur = sm.first;
@@ -594,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                     gk[u] = m.ks;
                     gl[u] = (float)((int)(bits >> 23) - 127);
                     gi[u] = __uint_as_float((254u << 23) - bits);
-                    if (bits & 0x7fffffu) gl[u] = log2f(v), gi[u] = 1.f / v;
+                        if (__builtin_expect(bits & 0x7fffffu, 0)) gl[u] = log2f(v), gi[u] = 1.f / v;
                     ok[u] = m.ok;
                     whole_piece = whole_piece && m.ok;
                 }
@@ -656,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                             const float x = kAcc == 2 ? sc[u][nt][0][i] + sc[u][nt][kAcc - 1][i] : sc[u][nt][0][i];
                             sc[u][nt][0][i] = fmaf(x, qs[nt][i & 1] * gk[u], gl[u]);
                         }
-                        if (edge) {
+                        if (__builtin_expect(edge, 0)) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const int key = base + u * kGroup + kr + (i >> 1) * 8;
@@ -678,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                         moved |= x > m[nt][c] + kLazy;
                     }
                 }
-                if (__any_sync(0xffffffffu, moved)) {
+                if (__builtin_expect(__any_sync(0xffffffffu, moved), 0)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -731,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                                 w[box][q][0] = x.x, w[box][q][1] = x.y, w[box][q][2] = x.z, w[box][q][3] = x.w;
                             }
                         }
-                    if (edge) take_out_masked<D, NT>(a, s, w, o, r, base + u * kGroup, ok[u], row0 + g);
+                    if (__builtin_expect(edge, 0)) take_out_masked<D, NT>(a, s, w, o, r, base + u * kGroup, ok[u], row0 + g);
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) {
                         const int box = i / (kBox / 16), j = (i % (kBox / 16)) >> 1;
@@ -818,7 +819,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                         for (int u = 0; u < kPer; ++u) x[u] *= inv;
                         int i, hg;
                         row_place(row0 + n, a.group, i, hg);
-                        store_row<T, kPer>(a, (size_t)(s.t0 + i), cur.h * a.group + hg, D, d * kRow + jd, x);
+                        const size_t token = (size_t)(s.t0 + i);
+                        const int head = cur.h * a.group + hg;
+                        Channels<T, kPer> gate;
+                        if (a.g) gate.load_gate(a, token, head, d * kRow + jd);
+                        store_row<T, kPer>(a, token, head, D, d * kRow + jd, x, gate);
                     } else {
                         float* p = a.part + ((size_t)part * kRows + n) * D + d * kRow + jd;
 #pragma unroll
@@ -856,91 +861,96 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
     }
 }
 
-// Joins the segments that were cut.  Block (c, y): rows y * per_block .. of the segment whose first
-// part CTA c left; its other parts are the first ones of the CTAs c + 1 .. last.  8 / per_block warps
+// Joins the segments that were cut.  Block (c, y): rows y * kPerBlock .. of the segment whose first
+// part CTA c left; its other parts are the first ones of the CTAs c + 1 .. last.  8 / kPerBlock warps
 // share the parts of a row, each with a maximum of its own, so that all loads of a warp are under way
 // at once behind the one of the segment's description.
 constexpr int kJoinAhead = 4;  // parts a warp loads at a time
-template <int D, int NT, typename T>
-__global__ void __launch_bounds__(256) attn_kv8_join_kernel(const Args a, int grid, int per_block) {
+template <int D, int NT, typename T, int kPerBlock>
+__global__ void __launch_bounds__(256) attn_kv8_join_kernel(const Args a, int grid) {
     constexpr int kRows = 8 * NT, kVec = D / 32;  // channels of a lane
-    __shared__ float acc[8][D];
-    __shared__ float2 stat[8];
+    constexpr int kSharers = 8 / kPerBlock;
     grid_dependency_wait();
     allow_dependent_launch();
     const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int4 d = reinterpret_cast<const int4*>(a.meta)[c];
-    const int last = d.x, row0 = d.w & 0xffffff, rows = d.w >> 24;
+    const int4 desc = reinterpret_cast<const int4*>(a.meta)[c];
+    const int last = desc.x, row0 = desc.w & 0xffffff, rows = desc.w >> 24;
     if (last < 0) return;
-    const int sharers = 8 / per_block;
-    const int n = blockIdx.y * per_block + warp / sharers;
+    const int n = blockIdx.y * kPerBlock + warp / kSharers;
     const int parts = n < rows ? last - c + 1 : 0;
+    int i, hg;
+    row_place(row0 + n, a.group, i, hg);
+    const size_t token = (size_t)(desc.y + i);
+    const int head = desc.z + hg;
+    Channels<T, kVec> gate;
+    if (a.g && n < rows) gate.load_gate(a, token, head, lane * kVec);
     const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)grid * 2 * kRows * D);
     float M = -INFINITY, sum = 0.f, x[kVec];
 #pragma unroll
     for (int u = 0; u < kVec; ++u) x[u] = 0.f;
-    for (int p0 = warp % sharers; p0 < parts; p0 += sharers * kJoinAhead) {
+    for (int p0 = warp % kSharers; p0 < parts; p0 += kSharers * kJoinAhead) {
         float2 st[kJoinAhead];
         float y[kJoinAhead][kVec];
 #pragma unroll
-        for (int i = 0; i < kJoinAhead; ++i) {
-            const int p = p0 + i * sharers;
-            st[i] = make_float2(-INFINITY, 0.f);
+        for (int j = 0; j < kJoinAhead; ++j) {
+            const int p = min(p0 + j * kSharers, parts - 1);  // past the end: the last one, not counted
+            const size_t at = (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * kRows + n;
+            st[j] = ml[at];
+            if (p0 + j * kSharers >= parts) st[j] = make_float2(-INFINITY, 0.f);
+            const float* src = a.part + at * D + lane * kVec;
 #pragma unroll
-            for (int u = 0; u < kVec; ++u) y[i][u] = 0.f;
-            if (p < parts) {
-                const size_t at = (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * kRows + n;
-                st[i] = ml[at];
-                const float* src = a.part + at * D + lane * kVec;
-#pragma unroll
-                for (int u = 0; u < kVec; u += 2) {
-                    const float2 v = *reinterpret_cast<const float2*>(src + u);
-                    y[i][u] = v.x;
-                    y[i][u + 1] = v.y;
-                }
+            for (int u = 0; u < kVec; u += 2) {
+                const float2 v = *reinterpret_cast<const float2*>(src + u);
+                y[j][u] = v.x;
+                y[j][u + 1] = v.y;
             }
         }
         float to = M;
 #pragma unroll
-        for (int i = 0; i < kJoinAhead; ++i) to = fmaxf(to, st[i].x);
+        for (int j = 0; j < kJoinAhead; ++j) to = fmaxf(to, st[j].x);
         const float f = part_weight(M, sum, to);
         sum *= f;
 #pragma unroll
         for (int u = 0; u < kVec; ++u) x[u] *= f;
 #pragma unroll
-        for (int i = 0; i < kJoinAhead; ++i) {
-            const float w = part_weight(st[i].x, st[i].y, to);
-            sum = fmaf(w, st[i].y, sum);
+        for (int j = 0; j < kJoinAhead; ++j) {
+            if (p0 + j * kSharers >= parts) continue;
+            const float w = part_weight(st[j].x, st[j].y, to);
+            sum = fmaf(w, st[j].y, sum);
 #pragma unroll
-            for (int u = 0; u < kVec; ++u) x[u] = fmaf(w, y[i][u], x[u]);
+            for (int u = 0; u < kVec; ++u) x[u] = fmaf(w, y[j][u], x[u]);
         }
         M = to;
     }
-    if (lane == 0) stat[warp] = make_float2(M, sum);
+    if constexpr (kSharers > 1) {
+        __shared__ float acc[8][D];
+        __shared__ float2 stat[8];
+        if (lane == 0) stat[warp] = make_float2(M, sum);
 #pragma unroll
-    for (int u = 0; u < kVec; ++u) acc[warp][lane * kVec + u] = x[u];
-    __syncthreads();
-    // the warps' sums of each row, 4 channels a thread
-    for (int i = threadIdx.x; i < per_block * (D / 4); i += 256) {
-        const int r = i / (D / 4), ch = (i % (D / 4)) * 4;
-        const int m = blockIdx.y * per_block + r;
-        if (m >= rows) continue;
-        float all = -INFINITY;
-        for (int w = r * sharers; w < (r + 1) * sharers; ++w) all = fmaxf(all, stat[w].x);
-        float y[4] = {0.f, 0.f, 0.f, 0.f}, s = 0.f;
-        for (int w = r * sharers; w < (r + 1) * sharers; ++w) {
-            const float f = part_weight(stat[w].x, stat[w].y, all);
-            s = fmaf(f, stat[w].y, s);
+        for (int u = 0; u < kVec; ++u) acc[warp][lane * kVec + u] = x[u];
+        __syncthreads();
+        if (warp % kSharers != 0 || n >= rows) return;
+        float all = M;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) y[u] = fmaf(f, acc[w][ch + u], y[u]);
+        for (int w = 1; w < kSharers; ++w) all = fmaxf(all, stat[warp + w].x);
+        const float f = part_weight(M, sum, all);
+        sum *= f;
+#pragma unroll
+        for (int u = 0; u < kVec; ++u) x[u] *= f;
+#pragma unroll
+        for (int w = 1; w < kSharers; ++w) {
+            const float2 st = stat[warp + w];
+            const float g = part_weight(st.x, st.y, all);
+            sum = fmaf(g, st.y, sum);
+#pragma unroll
+            for (int u = 0; u < kVec; ++u) x[u] = fmaf(g, acc[warp + w][lane * kVec + u], x[u]);
         }
-        const float inv = s == 0.f ? 0.f : 1.f / s;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) y[u] *= inv;
-        int token, hg;
-        row_place(row0 + m, a.group, token, hg);
-        store_row<T, 4>(a, (size_t)(d.y + token), d.z + hg, D, ch, y);
     }
+    if (n >= rows) return;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int u = 0; u < kVec; ++u) x[u] *= inv;
+    store_row<T, kVec>(a, token, head, D, lane * kVec, x, gate);
 }
 
 // Column tiles of 8 query rows a CTA works on at once: as many as the rows of a kv group fill, up
@@ -986,12 +996,12 @@ int launch(Args a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int g
     if (rc != B200LAB_OK) return rc;
     const long long used = (long long)a.group * a.max_seqlen_q;
     const int rows_used = (int)(used < 8 * NT ? used : 8 * NT);
-    // Rows a block joins: eight, a warp each, where a segment is cut into two or three parts (many
-    // segments, or few tiles), down to one with eight warps on its parts where segments are few.
-    const int parts = grid / (a.B < grid / a.Hkv ? a.B * a.Hkv : grid) + 2;
-    const int per_block = parts <= 4 ? 8 : parts <= 8 ? 4 : parts <= 16 ? 2 : 1;
-    return kv8_launch(attn_kv8_join_kernel<D, NT, T>, dim3(grid, (rows_used + per_block - 1) / per_block), 256, 0, st, a,
-                      grid, per_block);
+    // Rows a block joins: eight, a warp each, where a segment is cut into few parts (segments are
+    // many); one, its parts shared by eight warps, where they are few.
+    const long long segments = (long long)a.B * a.Hkv;
+    if (segments * 4 >= grid)
+        return kv8_launch(attn_kv8_join_kernel<D, NT, T, 8>, dim3(grid, (rows_used + 7) / 8), 256, 0, st, a, grid);
+    return kv8_launch(attn_kv8_join_kernel<D, NT, T, 1>, dim3(grid, rows_used), 256, 0, st, a, grid);
 }
 
 template <int D, typename T>
