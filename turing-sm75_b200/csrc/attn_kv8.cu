@@ -42,14 +42,24 @@ constexpr int kMaxGrid = 2048;            // CTAs of a call at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;              // the running maximum is moved when x exceeds it by 2^8
 
-// What a variant's CTA works on and holds; kCtas of them fill an SM's registers and shared memory.
+// What a variant's CTA works on and holds; `ctas` of them fill an SM's registers and shared memory.
+struct Shape {
+    int groups;  // of a piece, the keys a warp takes at a time
+    int ctas;
+    int depth;   // pieces of a warp's ring
+};
+constexpr Shape shape_of(int D, int nt) {
+    return D == 64 ? (nt == 1 ? Shape{2, 4, 2} : nt == 2 ? Shape{1, 3, 6} : Shape{1, 2, 10})
+         : D == 128 ? (nt == 1 ? Shape{2, 3, 2} : nt == 2 ? Shape{2, 2, 2} : Shape{1, 2, 5})
+                    : (nt == 1 ? Shape{1, 2, 3} : Shape{1, 2, 2});
+}
 template <int D, int NT> struct Cfg {
-    static constexpr int kH = NT == 1 && D <= 128 ? 2 : 1;  // groups of a piece, the keys a warp takes at a time
+    static constexpr int kH = shape_of(D, NT).groups;
     static constexpr int kPiece = kGroup * kH;
     static constexpr int kTile = kPiece * kWarps;           // keys a CTA takes at a time
     static constexpr int kBytes = 2 * kPiece * D;           // a piece of K, then one of V
-    static constexpr int kCtas = NT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : NT == 2 && D <= 128 ? 3 : 2;
-    static constexpr int kDepth = (D == 64 ? (NT == 1 ? 5 : NT == 2 ? 6 : 10) : D == 128 ? (NT == 1 ? 4 : NT == 2 ? 3 : 5) : (NT == 1 ? 3 : 2)) / kH;
+    static constexpr int kCtas = shape_of(D, NT).ctas;
+    static constexpr int kDepth = shape_of(D, NT).depth;
     static constexpr int kRow = 64;                         // channels joined at a time
     static constexpr int kStart = 2;                        // what a segment's start and end cost, in tiles
 };
@@ -646,8 +656,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                 // ---- softmax over the piece: thread (g, t) has keys key(g), key(g) + 8 of each group and rows
                 // 2t, 2t + 1
                 const bool edge = base + kPiece > all_see || !whole_piece;  // some key is masked for some row
-                bool moved = false;
-                float mx[NT][2];
+                bool moved = false;  // some score of this thread is far above its row's maximum so far
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -672,19 +681,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                         float x = fmaxf(sc[0][nt][0][c], sc[0][nt][0][c + 2]);
 #pragma unroll
                         for (int u = 1; u < kH; ++u) x = fmaxf(x, fmaxf(sc[u][nt][0][c], sc[u][nt][0][c + 2]));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        mx[nt][c] = x;
                         moved |= x > m[nt][c] + kLazy;
                     }
                 }
+                // The maximum only has to keep 2^(x - m) in range, and fp16 has room for 2^kLazy: no lane asks
+                // the others for theirs until one lies beyond that.
                 if (__builtin_expect(__any_sync(0xffffffffu, moved), 0)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const float to = fmaxf(m[nt][c], mx[nt][c]);
+                            float x = fmaxf(sc[0][nt][0][c], sc[0][nt][0][c + 2]);
+#pragma unroll
+                            for (int u = 1; u < kH; ++u) x = fmaxf(x, fmaxf(sc[u][nt][0][c], sc[u][nt][0][c + 2]));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                            const float to = fmaxf(m[nt][c], x);
                             const float f = to == -INFINITY ? 1.f : ex2(m[nt][c] - to);
                             m[nt][c] = to;
                             l[nt][c] *= f;
@@ -960,16 +973,8 @@ int column_tiles(int rows, int D) {
     return rows <= 8 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
 }
 
-int piece_keys(int D, int nt) {
-    return nt > 1 || D == 256 ? kGroup : D == 64 ? Cfg<64, 1>::kPiece : Cfg<128, 1>::kPiece;
-}
-static_assert(Cfg<256, 1>::kH == 1 && Cfg<64, 2>::kH == 1 && Cfg<128, 2>::kH == 1 && Cfg<64, 4>::kH == 1, "piece_keys");
-
 int plan_grid(int D, int nt, int sms) {
-    const int ctas = nt == 1 ? (D == 64 ? Cfg<64, 1>::kCtas : D == 128 ? Cfg<128, 1>::kCtas : Cfg<256, 1>::kCtas)
-                   : nt == 2 ? (D == 64 ? Cfg<64, 2>::kCtas : D == 128 ? Cfg<128, 2>::kCtas : Cfg<256, 2>::kCtas)
-                             : (D == 64 ? Cfg<64, 4>::kCtas : Cfg<128, 4>::kCtas);
-    const int g = ctas * sms;
+    const int g = shape_of(D, nt).ctas * sms;
     return g < kMaxGrid ? g : kMaxGrid;
 }
 
@@ -1074,7 +1079,7 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     // the cache as [n_blocks * Hkv][block_size][D] bytes; a box is box_rows tokens of up to 128 channels
     CUtensorMap mk, mv;
     const uint32_t box = D > 128 ? 128 : (uint32_t)D;
-    const int piece = piece_keys(D, nt);
+    const int piece = kGroup * shape_of(D, nt).groups;
     a.box_rows = block_size < piece ? block_size : piece;
     const CUtensorMapSwizzle swizzle = D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
     for (int side = 0; side < 2; ++side) {
