@@ -16,14 +16,17 @@
 //     are (the tiles of all (sequence, kv-head, row tile) segments are numbered through on the
 //     device).  A segment that lies in one run is written out by its CTA; one that is cut leaves
 //     fp32 partial sums in the workspace, two at most a CTA, and a second kernel joins them.
-//   * A warp has a ring of its own of 16- or 32-key pieces of K and V, filled by TMA, whose next pieces
-//     are requested across segment borders, so that the loads never pause.
+//   * A warp has a ring of its own of 16- or 32-key pieces of K and V, which its lanes fill with
+//     16-byte asynchronous copies, whose next pieces are requested across segment borders, so that
+//     the loads never pause.  Nothing but the joins holds the warps of a CTA together.  (TMA boxes
+//     into the same rings measured the same on the largest batches and slower on short rings of
+//     small boxes: four drafted tokens x 16 sequences of 2-4k 35.0 against 33.7 us.)
 //   * Products are mma.sync m16n8k16 with the KEYS (S^T = K Q^T) and the CHANNELS (O^T = V^T P^T)
 //     on the 16-row side and 8 query rows on the 8-column side: a kv group of 1..8 rows fills one
 //     column tile, a code is converted to fp16 (exactly) once for all column tiles, and P^T
 //     turns from result into operand by a register transpose (movmatrix).
 //   * The channel and key order inside a product is free: each thread takes 32 consecutive channels
-//     of a K row (two 16-byte shared loads, conflict-free under the TMA swizzle) and 16 of four V
+//     of a K row (two 16-byte shared loads, conflict-free as the chunks are swizzled) and 16 of four V
 //     rows, whose bytes it pairs by key with one PRMT for two conversions.
 //   * Q is brought to fp16 with a power of two a row: exact, as bf16 and fp16 both have at most 11
 //     significant bits (below 2^-29 of the row's largest value, bits are lost).
@@ -74,6 +77,8 @@ struct Args {
     const void* g;  // gate or null
     void* o;
     long long q_st, q_sh, g_st, g_sh;  // strides of a token and of a head
+    const uint8_t* k;
+    const uint8_t* v;
     const int* table;
     const int* lens;
     const int* cu;  // null: one query token a sequence
@@ -82,7 +87,6 @@ struct Args {
     float* part;    // [grid][2][rows][D] sums, [grid][2][rows] (m, l)
     int* meta;      // [grid][4]
     int max_seqlen_q, total_q, B, max_blocks, n_blocks, log2P, Hq, Hkv, group, causal;
-    int box_rows;   // tokens a TMA box holds: the piece's, or the block's where that is less
     float scale;
 };
 
@@ -188,10 +192,8 @@ template <int D, int NT> struct Smem {
     GroupMeta meta[kWarps][Cfg<D, NT>::kDepth][Cfg<D, NT>::kH];
     float m[kWarps][8 * NT], l[kWarps][8 * NT];
     float qscale[8 * NT];
-    uint64_t full[kWarps][Cfg<D, NT>::kDepth];
     long long total[kWarps];
     Cursor<D, NT> first;
-    int abort;
 };
 
 // The factor that brings a part's sums from its own maximum m to the common one M.  A part without
@@ -235,8 +237,8 @@ __device__ __forceinline__ void store_row(const Args& a, size_t token, int head,
     }
 }
 
-// Where the words of a thread's K row lie: the 128-byte swizzle (64-byte at D = 64) of the TMA box,
-// 16-byte chunk index XOR row.
+// Where a 16-byte chunk of a row lies in a piece: chunk index XOR row (XOR half the row at D = 64,
+// where two rows share a line of banks).
 template <int D> __device__ __forceinline__ int chunk_at(int row, int chunk) {
     if constexpr (D == 64) {
         return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
@@ -299,13 +301,16 @@ __device__ __forceinline__ float load_q(const T* q, int t, uint32_t (&f)[D / 16]
     return finite ? __uint_as_float((254u - field) << 23) : __uint_as_float(0x7fc00000u);
 }
 
-// 4 bytes global -> shared without waiting, and this thread's arrival at `bar` once its copies are
-// complete (which the barrier's count includes).
-__device__ __forceinline__ void copy_word(void* smem, const void* src) {
+// 16 or 4 bytes global -> shared without waiting.
+__device__ __forceinline__ void copy16(uint32_t smem, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(void* smem, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(src) : "memory");
 }
-__device__ __forceinline__ void arrive_when_copied(uint64_t* bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending> __device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
 // The pieces of one warp in the order it takes them, requested ahead of their use.
@@ -313,75 +318,58 @@ template <int D, int NT> struct Producer {
     using C = Cfg<D, NT>;
     Cursor<D, NT> c;
     int k;        // next tile of the segment, from c.first()
-    int block;    // lane i: of group i of the next 32 / kH pieces
+    int block;    // lane i: block * Hkv + head of group i of the next 32 / kH pieces; -1: none
 
-    // Requests the next piece into a ring slot; false: none is left.
-    __device__ __forceinline__ bool issue(const Args& a, const CUtensorMap* mk, const CUtensorMap* mv, uint8_t* slot,
-                                          GroupMeta* meta, uint64_t* bar, int warp, int lane) {
-        for (;;) {
-            if (c.left <= 0) return false;
-            if (k < c.count() && (c.first() + k) * C::kTile + warp * C::kPiece < c.s.L) break;
+    // Requests the next piece, if one is left, into a ring slot, as one group of copies.
+    __device__ __forceinline__ void issue(const Args& a, uint8_t* slot, GroupMeta* meta, int warp, int lane) {
+        while (c.left > 0 && !(k < c.count() && (c.first() + k) * C::kTile + warp * C::kPiece < c.s.L)) {
             c.next(a);
             k = 0;
         }
-        constexpr int kAhead = 32 / C::kH;
-        if ((k & (kAhead - 1)) == 0) {  // the block ids of the next pieces, a group a lane
-            const int pos = (c.first() + k + lane / C::kH) * C::kTile + warp * C::kPiece + (lane % C::kH) * kGroup;
-            block = -1;
-            if (k + lane / C::kH < c.count() && pos < c.s.L) {
-                block = a.table[(size_t)c.b * a.max_blocks + (pos >> a.log2P)];
-                if (block < 0 || block >= a.n_blocks) {
-                    atomicExch(&g_err_attn_kv8, B200LAB_ERR_INVALID);
-                    block = -1;
+        if (c.left > 0) {
+            constexpr int kAhead = 32 / C::kH;
+            if ((k & (kAhead - 1)) == 0) {  // the blocks of the next pieces, a group a lane
+                const int pos = (c.first() + k + lane / C::kH) * C::kTile + warp * C::kPiece + (lane % C::kH) * kGroup;
+                block = -1;
+                if (k + lane / C::kH < c.count() && pos < c.s.L) {
+                    block = a.table[(size_t)c.b * a.max_blocks + (pos >> a.log2P)];
+                    if (block < 0 || block >= a.n_blocks) {
+                        atomicExch(&g_err_attn_kv8, B200LAB_ERR_INVALID);
+                        block = -1;
+                    } else {
+                        block = block * a.Hkv + c.h;
+                    }
                 }
             }
-        }
-        const int first = (k & (kAhead - 1)) * C::kH;  // lane of the piece's first group
-        int blk[C::kH];
-#pragma unroll
-        for (int u = 0; u < C::kH; ++u) blk[u] = __shfl_sync(0xffffffffu, block, first + u);
-        // the scales come as copies of their own, so that nothing here waits for them: each of the lanes
-        // that hold the piece's groups arrives at the barrier once its two words are there
-        if (lane >= first && lane < first + C::kH) {
-            GroupMeta* m = meta + (lane - first);
-            m->ok = block >= 0;
-            if (block >= 0) {
-                const size_t bh = (size_t)block * a.Hkv + c.h;
-                copy_word(&m->ks, a.k_scale + bh);
-                copy_word(&m->vs, a.v_scale + bh);
-            } else {
+            const int first = (k & (kAhead - 1)) * C::kH;  // lane of the piece's first group
+            if (lane >= first && lane < first + C::kH) {
+                GroupMeta* m = meta + (lane - first);
+                m->ok = block >= 0;
                 m->ks = m->vs = 1.f;
+                if (block >= 0) {
+                    copy4(&m->ks, a.k_scale + block);
+                    copy4(&m->vs, a.v_scale + block);
+                }
             }
-            arrive_when_copied(bar);
-        }
-        if (lane == 0) {
-            constexpr int kBox = D > 128 ? 128 : D;
-            const int step = a.box_rows / kGroup;  // groups of a box, all of one block
-            int boxes = 0;
-#pragma unroll
-            for (int u = 0; u < C::kH; ++u) boxes += u % step == 0 && blk[u] >= 0;
-            if (boxes) {
-                mbar_arrive_expect_tx(bar, boxes * a.box_rows * 2 * D);
-            } else {
-                mbar_arrive(bar);
-            }
-            const int pos = (c.first() + k) * C::kTile + warp * C::kPiece;
 #pragma unroll
             for (int u = 0; u < C::kH; ++u) {
-                if (u % step != 0 || blk[u] < 0) continue;
-                const int row = (pos + u * kGroup) & ((1 << a.log2P) - 1);
-                const int bh = blk[u] * a.Hkv + c.h;
+                const int bh = __shfl_sync(0xffffffffu, block, first + u);
+                if (bh < 0) continue;
+                const int row = ((c.first() + k) * C::kTile + warp * C::kPiece + u * kGroup) & ((1 << a.log2P) - 1);
+                const size_t at = (((size_t)(uint32_t)bh << a.log2P) + row) * D + lane * 16;
+                const uint32_t dst = smem_u32(slot);
 #pragma unroll
-                for (int box = 0; box < D / kBox; ++box) {
-                    uint8_t* dst = slot + (box * C::kPiece + u * kGroup) * kBox;
-                    tma_load_3d(dst, mk, bar, box * kBox, row, bh);
-                    tma_load_3d(dst + C::kPiece * D, mv, bar, box * kBox, row, bh);
+                for (int i = 0; i < kGroup * D / 512; ++i) {  // 512 contiguous bytes a copy of the warp
+                    constexpr int kBox = D > 128 ? 128 : D, kRowLanes = D / 16;
+                    const int r = i * (512 / D) + lane / kRowLanes, chunk = lane % kRowLanes;
+                    const int off = (chunk / (kBox / 16)) * (C::kPiece * kBox) + u * kGroup * kBox + chunk_at<D>(r, chunk % (kBox / 16));
+                    copy16(dst + off, a.k + at + i * 512);
+                    copy16(dst + C::kPiece * D + off, a.v + at + i * 512);
                 }
             }
+            ++k;
         }
-        __syncwarp();  // every lane sees m->ok
-        ++k;
-        return true;
+        copy_commit();
     }
 };
 
@@ -423,7 +411,10 @@ __device__ __forceinline__ void take_out_masked(const Args& a, const Seq& s, uin
             const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
             const uint32_t x = __byte_perm(f[0], f[1], sel), y = __byte_perm(f[2], f[3], sel);
             float hit[4] = {0.f, 0.f, 0.f, 0.f};
-            mma(hit, kv8_decode2(x), kv8_decode2_hi(x), kv8_decode2(y), kv8_decode2_hi(y), vis[0], vis[1]);
+            uint32_t a0, a1, a2, a3;
+            kv8_decode4(x, a0, a1);
+            kv8_decode4(y, a2, a3);
+            mma(hit, a0, a1, a2, a3, vis[0], vis[1]);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
                 if (hit[c] > 0.f) o[nt][i][c] = __uint_as_float(0x7fc00000u);
@@ -442,7 +433,7 @@ __device__ __forceinline__ void take_out_masked(const Args& a, const Seq& s, uin
 
 template <int D, int NT, typename T>
 __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
-    attn_kv8_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const Args a) {
+    attn_kv8_kernel(const Args a) {
     using C = Cfg<D, NT>;
     constexpr int kRows = 8 * NT, kDepth = C::kDepth, kH = C::kH, kPiece = C::kPiece, kTile = C::kTile;
     constexpr int kBox = D > 128 ? 128 : D, kBoxes = D / kBox;
@@ -451,15 +442,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
 
-    if (tid == 0) {
-        prefetch_tmap(&mapK);
-        prefetch_tmap(&mapV);
-        sm.abort = 0;
-    }
-    if (lane == 0) {
-        for (int i = 0; i < kDepth; ++i) mbar_init(&sm.full[warp][i], 1 + kH);  // the copies, a lane a group's scales
-        fence_barrier_init();
-    }
     // Launched early, but lets the join kernel start only as its CTAs end (the default): a join CTA that
     // waits on an SM keeps the next call's CTA from starting there (B64 16k, calls back to back: 580 us
     // with the trigger here, 350 without).
@@ -523,11 +505,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
     Producer<D, NT> pro;
     pro.c = cur;
     pro.k = 0;
-    int put = 0, got = 0, slot = 0;  // pieces requested and taken, the next one's slot
-    uint32_t phase = 0;
-    bool alive = true;
-    for (; put < kDepth; ++put)
-        if (!pro.issue(a, &mapK, &mapV, sm.ring[warp][put], sm.meta[warp][put], &sm.full[warp][put], warp, lane)) break;
+    int slot = 0;  // the next piece's
+    for (int i = 0; i < kDepth; ++i) pro.issue(a, sm.ring[warp][i], sm.meta[warp][i], warp, lane);
 
     bool has_tail = false;  // whether the run's last segment goes on in the next CTA's
     for (; cur.left > 0; cur.next(a)) {
@@ -588,9 +567,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
         for (int k = 0; k < run; ++k) {
             const int base = (first + k) * kTile + warp * kPiece;
             if (base >= s.L) break;
-            if (alive)  // agreed by the warp: every lane goes the same way on
-                alive = __all_sync(0xffffffffu, mbar_wait(&sm.full[warp][slot], phase, &sm.abort, &g_err_attn_kv8));
-            if (alive) {
+            copy_wait<kDepth - 1>();
+            __syncwarp();
+            {
                 const uint8_t* ks_ = sm.ring[warp][slot];
                 const uint8_t* vs_ = ks_ + kPiece * D;
                 // scale of K, log2 and inverse of the scale of V: powers of two, whose exponents are read off
@@ -638,8 +617,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const int ks = (box * kChunks + c) * 4 + j;
-                                const uint32_t a0 = kv8_decode2(w0[j]), a1 = kv8_decode2(w1[j]);
-                                const uint32_t a2 = kv8_decode2_hi(w0[j]), a3 = kv8_decode2_hi(w1[j]);
+                                uint32_t a0, a1, a2, a3;
+                                kv8_decode4(w0[j], a0, a2);
+                                kv8_decode4(w1[j], a1, a3);
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) {
                                     if constexpr (NT == 1) {
@@ -752,18 +732,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                         const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
                         const uint32_t x = __byte_perm(w[box][0][j], w[box][1][j], sel);
                         const uint32_t y = __byte_perm(w[box][2][j], w[box][3][j], sel);
-                        const uint32_t a0 = kv8_decode2(x), a1 = kv8_decode2_hi(x);
-                        const uint32_t a2 = kv8_decode2(y), a3 = kv8_decode2_hi(y);
+                        uint32_t a0, a1, a2, a3;
+                        kv8_decode4(x, a0, a1);
+                        kv8_decode4(y, a2, a3);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma(o[nt][i], a0, a1, a2, a3, pb[u][nt][0], pb[u][nt][1]);
                     }
                 }
-                ++got;
                 __syncwarp();  // every lane has read the slot
-                if (pro.issue(a, &mapK, &mapV, sm.ring[warp][slot], sm.meta[warp][slot], &sm.full[warp][slot], warp, lane))
-                    ++put;
+                pro.issue(a, sm.ring[warp][slot], sm.meta[warp][slot], warp, lane);
             }
-            if (++slot == kDepth) slot = 0, phase ^= 1;
+            if (++slot == kDepth) slot = 0;
         }
 
         // ---- join the warps' sums
@@ -862,16 +841,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
         }
     }
     if (!has_tail && tid == 0) a.meta[4 * blockIdx.x] = -1;
-    if (!alive) {
-        // a wait gave up: let the copies in flight land (again for a limited time) before the CTA's
-        // shared memory is given back
-        const unsigned long long began = globaltimer_ns();
-        for (; got < put; ++got) {
-            const int i = got % kDepth;
-            while (!mbar_test(&sm.full[warp][i], (got / kDepth) & 1))
-                if (globaltimer_ns() - began > kWaitLimitNs) return;
-        }
-    }
 }
 
 // Joins the segments that were cut.  Block (c, y): rows y * kPerBlock .. of the segment whose first
@@ -984,7 +953,7 @@ size_t workspace_bytes(int nt, int D, int sms) {
 }
 
 template <int D, int NT, typename T>
-int launch(Args a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid, int device,
+int launch(Args a, void* ws, int grid, int device,
            cudaStream_t st) {
     const size_t rows = (size_t)grid * 2 * 8 * NT;
     a.part = static_cast<float*>(ws);
@@ -997,7 +966,7 @@ int launch(Args a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int g
         B200_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    int rc = kv8_launch(kern, dim3(grid), kThreads, smem, st, mk, mv, a);
+    int rc = kv8_launch(kern, dim3(grid), kThreads, smem, st, a);
     if (rc != B200LAB_OK) return rc;
     const long long used = (long long)a.group * a.max_seqlen_q;
     const int rows_used = (int)(used < 8 * NT ? used : 8 * NT);
@@ -1010,21 +979,21 @@ int launch(Args a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int g
 }
 
 template <int D, typename T>
-int launch_rows(int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid, int device,
+int launch_rows(int nt, const Args& a, void* ws, int grid, int device,
            cudaStream_t st) {
-    if (nt == 1) return launch<D, 1, T>(a, mk, mv, ws, grid, device, st);
-    if (nt == 2) return launch<D, 2, T>(a, mk, mv, ws, grid, device, st);
-    if constexpr (D < 256) return launch<D, 4, T>(a, mk, mv, ws, grid, device, st);
+    if (nt == 1) return launch<D, 1, T>(a, ws, grid, device, st);
+    if (nt == 2) return launch<D, 2, T>(a, ws, grid, device, st);
+    if constexpr (D < 256) return launch<D, 4, T>(a, ws, grid, device, st);
     return B200LAB_ERR_UNSUPPORTED;
 }
 
 template <typename T>
-int launch_d(int D, int nt, const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws, int grid,
+int launch_d(int D, int nt, const Args& a, void* ws, int grid,
              int device, cudaStream_t st) {
     switch (D) {
-        case 64: return launch_rows<64, T>(nt, a, mk, mv, ws, grid, device, st);
-        case 128: return launch_rows<128, T>(nt, a, mk, mv, ws, grid, device, st);
-        default: return launch_rows<256, T>(nt, a, mk, mv, ws, grid, device, st);
+        case 64: return launch_rows<64, T>(nt, a, ws, grid, device, st);
+        case 128: return launch_rows<128, T>(nt, a, ws, grid, device, st);
+        default: return launch_rows<256, T>(nt, a, ws, grid, device, st);
     }
 }
 
@@ -1071,23 +1040,13 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     Args a;
     a.q = Q, a.g = G, a.o = O;
     a.q_st = q_stride_token, a.q_sh = q_stride_head, a.g_st = g_stride_token, a.g_sh = g_stride_head;
+    a.k = static_cast<const uint8_t*>(k_cache), a.v = static_cast<const uint8_t*>(v_cache);
     a.table = block_table, a.lens = seq_lens, a.cu = cu_seqlens_q;
     a.k_scale = k_scale, a.v_scale = v_scale;
     a.max_seqlen_q = most, a.total_q = total_q, a.B = B, a.max_blocks = max_blocks, a.n_blocks = n_blocks;
     a.log2P = kv8_log2_block(block_size), a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv, a.causal = causal;
     a.scale = scale;
-    // the cache as [n_blocks * Hkv][block_size][D] bytes; a box is box_rows tokens of up to 128 channels
-    CUtensorMap mk, mv;
-    const uint32_t box = D > 128 ? 128 : (uint32_t)D;
-    const int piece = kGroup * shape_of(D, nt).groups;
-    a.box_rows = block_size < piece ? block_size : piece;
-    const CUtensorMapSwizzle swizzle = D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
-    for (int side = 0; side < 2; ++side) {
-        rc = make_tmap_3d(side ? &mv : &mk, side ? v_cache : k_cache, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)D,
-                          (uint64_t)block_size, (uint64_t)n_blocks * Hkv, box, (uint32_t)a.box_rows, swizzle);
-        if (rc != B200LAB_OK) return rc;
-    }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, a, mk, mv, workspace, grid, dev.ordinal, st)
-                                : launch_d<__nv_bfloat16>(D, nt, a, mk, mv, workspace, grid, dev.ordinal, st);
+    return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, a, workspace, grid, dev.ordinal, st)
+                                : launch_d<__nv_bfloat16>(D, nt, a, workspace, grid, dev.ordinal, st);
 }

@@ -37,16 +37,14 @@ __device__ __forceinline__ uint32_t kv8_encode2(float a, float b) {
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 
-// Two codes (the low 16 bits) -> two fp16 values (exact: every e4m3 value is an fp16 value).
-__device__ __forceinline__ uint32_t kv8_decode2(uint32_t codes) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)(codes & 0xffffu)));
-    return r;
-}
-__device__ __forceinline__ uint32_t kv8_decode2_hi(uint32_t codes) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)(codes >> 16)));
-    return r;
+// Four codes -> four fp16 values, the lower two in `lo` (exact: every e4m3 value is an fp16 value).
+__device__ __forceinline__ void kv8_decode4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(codes));
 }
 
 // log2 of the block sizes that are built (16, 32, 64, 128 tokens), else -1.

@@ -51,7 +51,8 @@ constexpr int kAppendVecs = 8;  // vectors of 8 values a thread holds
 // Bound by memory for prompts and by latency (three dependent loads: offsets, block id, data)
 // for a step of one token a sequence, where a warp an item keeps the grid to one short wave.
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) kv8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads, kThreads <= 128 && sizeof(T) == 2 ? 8 : 1)
+    kv8_append_kernel(const AppendArgs a) {
     constexpr int kCta = kThreads < 128 ? 128 : kThreads;
     grid_dependency_wait();
     allow_dependent_launch();
@@ -130,7 +131,8 @@ __global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) kv8_append_ke
             uint32_t* e = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const uint32_t p0 = kv8_decode2(e[u]), p1 = kv8_decode2_hi(e[u]);
+                uint32_t p0, p1;
+                kv8_decode4(e[u], p0, p1);
                 const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&p0));
                 const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&p1));
                 e[u] = kv8_encode2(f0.x * ratio, f0.y * ratio) | (kv8_encode2(f1.x * ratio, f1.y * ratio) << 16);
@@ -162,70 +164,70 @@ struct ReadArgs {
     const int* cu;
     void* out[2];
     int max_seqlen, total, B, max_blocks, n_blocks, log2P, Hkv, log2D, blocks_per_seq;
-    long long vecs;
+    int chunks;  // CTAs for the codes of a block, K's or V's
 };
 
 constexpr int kReadThreads = 256;
-constexpr int kReadVecs = 4;  // vectors a thread has in flight
+constexpr int kReadVecs = 8;  // vectors a thread has in flight
 
-// Codes -> values, 16 bytes of output a thread and vector (a warp stores 512 contiguous bytes of
-// one or two token rows).  The vectors of all (sequence, block, head, K or V) items are numbered
-// through, each item's a power of two; a thread's vectors are loaded before the first is stored.
+// Codes -> values, 16 bytes of output a thread and vector.  A block's codes of all heads are one run
+// of memory, and so are its tokens' values; a CTA takes kReadThreads * kReadVecs vectors of such a
+// run, K's or V's, so that the chain of offsets, block id and codes is walked once for 16 KB of codes
+// and every thread has all its loads under way before the first store.
 template <typename T>
 __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const ReadArgs a) {
     constexpr int kVec = 16 / sizeof(T), kLog2Vec = sizeof(T) == 4 ? 2 : 3;
     grid_dependency_wait();
     allow_dependent_launch();
-    const int log2_item = a.log2P + a.log2D - kLog2Vec;
-    const int log2_row = a.log2D - kLog2Vec;
+    unsigned rest = blockIdx.x;
+    const int side = rest & 1;
+    rest >>= 1;
+    const int chunk = rest % (unsigned)a.chunks;
+    rest /= (unsigned)a.chunks;
+    const int bi = rest % (unsigned)a.blocks_per_seq, b = rest / (unsigned)a.blocks_per_seq;
+    const int t0 = a.cu[b];
+    const long long n = (long long)a.cu[b + 1] - t0;
+    if (t0 < 0 || n < 0 || t0 + n > a.total || n > a.max_seqlen || n > ((long long)a.max_blocks << a.log2P)) {
+        if (threadIdx.x == 0 && bi == 0) report_invalid();
+        return;
+    }
+    const long long left = n - ((long long)bi << a.log2P);  // tokens from the block's first on
+    if (left <= 0) return;
+    const int block = a.table[(size_t)b * a.max_blocks + bi];
+    if (block < 0 || block >= a.n_blocks) {
+        if (threadIdx.x == 0) report_invalid();
+        return;
+    }
+    const int log2_head = a.log2P + a.log2D;
+    const uint8_t* src = (side ? a.cache[1] : a.cache[0]) + (((size_t)block * a.Hkv) << log2_head);
+    const float* scales = (side ? a.scale[1] : a.scale[0]) + (size_t)block * a.Hkv;
+    T* dst = static_cast<T*>(side ? a.out[1] : a.out[0]) + ((((size_t)t0 + ((size_t)bi << a.log2P)) * a.Hkv) << a.log2D);
+    const int first = (chunk * (kReadVecs * kReadThreads) + threadIdx.x) << kLog2Vec;  // code in the run
+    const int end = a.Hkv << log2_head;
     uint2 codes[kReadVecs];
     float scale[kReadVecs];
-    T* dst[kReadVecs];
 #pragma unroll
     for (int v = 0; v < kReadVecs; ++v) {
-        dst[v] = nullptr;
-        const long long i = ((long long)blockIdx.x * kReadVecs + v) * kReadThreads + threadIdx.x;
-        if (i >= a.vecs) continue;
-        const long long item = i >> log2_item;
-        const int at = (int)(i & ((1 << log2_item) - 1));
-        const int side = (int)(item & 1);
-        long long rest = item >> 1;
-        const int h = (int)(rest % a.Hkv);
-        rest /= a.Hkv;
-        const int bi = (int)(rest % a.blocks_per_seq);
-        const int b = (int)(rest / a.blocks_per_seq);
-        const int t0 = a.cu[b];
-        const long long n = (long long)a.cu[b + 1] - t0;
-        if (t0 < 0 || n < 0 || t0 + n > a.total || n > a.max_seqlen || n > ((long long)a.max_blocks << a.log2P)) {
-            if (at == 0 && bi == 0) report_invalid();
-            continue;
+        const int i = first + ((v * kReadThreads) << kLog2Vec);
+        if (i < end && ((i & ((1 << log2_head) - 1)) >> a.log2D) < left) {
+            if constexpr (kVec == 8) {
+                codes[v] = *reinterpret_cast<const uint2*>(src + i);
+            } else {
+                codes[v].x = *reinterpret_cast<const uint32_t*>(src + i);
+            }
+            scale[v] = scales[i >> log2_head];
         }
-        const int pos = (bi << a.log2P) + (at >> log2_row);
-        if (pos >= n) continue;
-        const int block = a.table[(size_t)b * a.max_blocks + bi];
-        if (block < 0 || block >= a.n_blocks) {
-            if (at == 0) report_invalid();
-            continue;
-        }
-        const size_t bh = (size_t)block * a.Hkv + h;
-        const uint8_t* src = (side ? a.cache[1] : a.cache[0]) + ((bh << a.log2P) << a.log2D) + ((size_t)at << kLog2Vec);
-        if constexpr (kVec == 8) {
-            codes[v] = *reinterpret_cast<const uint2*>(src);
-        } else {
-            codes[v].x = *reinterpret_cast<const uint32_t*>(src);
-        }
-        scale[v] = (side ? a.scale[1] : a.scale[0])[bh];
-        dst[v] = static_cast<T*>(side ? a.out[1] : a.out[0]) + ((((size_t)(t0 + pos)) * a.Hkv + h) << a.log2D) +
-                 ((at & ((1 << log2_row) - 1)) << kLog2Vec);
     }
 #pragma unroll
     for (int v = 0; v < kReadVecs; ++v) {
-        if (!dst[v]) continue;
+        const int i = first + ((v * kReadThreads) << kLog2Vec);
+        const int row = (i & ((1 << log2_head) - 1)) >> a.log2D;
+        if (i >= end || row >= left) continue;
         float x[kVec];
 #pragma unroll
         for (int u = 0; u < kVec / 4; ++u) {
-            const uint32_t w = u == 0 ? codes[v].x : codes[v].y;
-            const uint32_t p0 = kv8_decode2(w), p1 = kv8_decode2_hi(w);
+            uint32_t p0, p1;
+            kv8_decode4(u == 0 ? codes[v].x : codes[v].y, p0, p1);
             const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&p0));
             const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&p1));
             x[4 * u] = f0.x * scale[v];
@@ -242,7 +244,8 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const ReadArgs a
         } else {
             o = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
         }
-        *reinterpret_cast<uint4*>(dst[v]) = o;
+        T* to = dst + ((((size_t)row * a.Hkv) + (i >> log2_head)) << a.log2D) + (i & ((1 << a.log2D) - 1));
+        *reinterpret_cast<uint4*>(to) = o;
     }
 }
 
@@ -333,9 +336,11 @@ extern "C" int kv8_read_sm100(const void* k_cache, const void* v_cache, const fl
     a.log2P = kv8_log2_block(block_size), a.Hkv = Hkv, a.log2D = ilog2(D);
     const long long blocks = ((long long)most + block_size - 1) / block_size;
     a.blocks_per_seq = (int)(blocks < max_blocks ? blocks : max_blocks);
-    a.vecs = (2LL * B * a.blocks_per_seq * Hkv) << (a.log2P + a.log2D - (out_dtype == B200LAB_F32 ? 2 : 3));
+    const long long run = ((long long)Hkv * block_size * D) >> (out_dtype == B200LAB_F32 ? 2 : 3);  // vectors
+    if (run > 0x10000000LL) return B200LAB_ERR_UNSUPPORTED;
     const long long per_cta = (long long)kReadThreads * kReadVecs;
-    const long long grid = (a.vecs + per_cta - 1) / per_cta;
+    a.chunks = (int)((run + per_cta - 1) / per_cta);
+    const long long grid = 2LL * B * a.blocks_per_seq * a.chunks;
     if (grid > 0x7fffffffLL) return B200LAB_ERR_UNSUPPORTED;
     rc = kv8_device().status;
     if (rc != B200LAB_OK) return rc;
