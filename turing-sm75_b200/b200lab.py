@@ -143,9 +143,15 @@ def _check(status: int, what: str) -> None:
 # ----------------------------------------------------------------------------
 # torch-facing wrappers
 # ----------------------------------------------------------------------------
+_TORCH = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = torch
+    return _TORCH
 
 
 def _dtype_code(t) -> int:
@@ -486,15 +492,15 @@ def _kv8_refuse(k_cache, v_cache, k_scale, v_scale, block_table):
 def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
     """Checks of the cache's tensors; returns ((n_blocks, Hkv, block_size, D), device index)."""
     torch = _torch()
-    shape, dev, e4m3 = k_cache.shape, k_cache.get_device(), torch.float8_e4m3fn
+    shape, dev, e4m3, f32 = k_cache.shape, k_cache.get_device(), torch.float8_e4m3fn, torch.float32
     if dev < 0:
         raise ValueError("k_cache must be a CUDA tensor (no CPU path)")
     if not (len(shape) == 4 and v_cache.shape == shape and k_cache.dtype is e4m3 and v_cache.dtype is e4m3
-            and k_scale.shape == shape[:2] and v_scale.shape == shape[:2] and k_scale.dtype is torch.float32
-            and v_scale.dtype is torch.float32 and block_table.dtype is torch.int32 and block_table.dim() == 2
-            and v_cache.get_device() == dev and k_scale.get_device() == dev and v_scale.get_device() == dev
-            and block_table.get_device() == dev and k_cache.is_contiguous() and v_cache.is_contiguous()
-            and k_scale.is_contiguous() and v_scale.is_contiguous() and block_table.is_contiguous()):
+            and k_scale.shape == v_scale.shape == shape[:2] and k_scale.dtype is f32 and v_scale.dtype is f32
+            and block_table.dtype is torch.int32 and block_table.dim() == 2
+            and v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == block_table.get_device() == dev
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous() and block_table.is_contiguous()):
         _kv8_refuse(k_cache, v_cache, k_scale, v_scale, block_table)
     return shape, dev
 
@@ -647,7 +653,7 @@ def attn_fwd_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *
         if n is None:  # at least a value, so that wrong sizes reach the library's own checks
             n = _kv8_workspace[key] = max(1, attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q, D) // 2)
         workspace = out.new_empty(n)
-        ws_bytes = n * out.element_size()
+        ws_bytes = 2 * n
     else:
         if not workspace.is_contiguous() or workspace.get_device() != dev:
             raise ValueError("workspace must be contiguous, on the cache's device")

@@ -11,8 +11,6 @@
 // bf16 and fp32, and the attention can carry the scale of V in the exponent of its weights.
 #pragma once
 
-#include <cuda_fp8.h>
-
 #include <atomic>
 
 #include "common.cuh"
@@ -32,9 +30,16 @@ __device__ __forceinline__ float kv8_scale_for(float amax) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// Two values -> two codes (a in the low byte): nearest even, |x| > 448 becomes 448, NaN stays NaN.
-__device__ __forceinline__ uint32_t kv8_encode2(float a, float b) {
-    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+// Four values -> four codes (a in the lowest byte): nearest even, |x| > 448 becomes 448, NaN stays NaN.
+__device__ __forceinline__ uint32_t kv8_encode4(float a, float b, float c, float d) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+        "mov.b32 %0, {l, h};\n\t}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
 }
 
 // Four codes -> four fp16 values, the lower two in `lo` (exact: every e4m3 value is an fp16 value).

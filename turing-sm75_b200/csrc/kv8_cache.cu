@@ -17,6 +17,34 @@ template <typename T> struct Raw8 {
     uint4 a;
     __device__ __forceinline__ void load(const T* p) { a = *reinterpret_cast<const uint4*>(p); }
     __device__ __forceinline__ float get(int i) const { return Elem<T>::to_f(reinterpret_cast<const T*>(&a)[i]); }
+    __device__ __forceinline__ void zero() { a = make_uint4(0, 0, 0, 0); }
+    // The largest magnitude of some vectors' finite values.  Magnitudes of one sign order as their
+    // bits do, so two values are compared at a time; only where an infinity or NaN turns up are the
+    // values looked at one by one.
+    template <int N> static __device__ __forceinline__ float amax(const Raw8 (&v)[N]) {
+        constexpr uint32_t kInf = sizeof(T) == 2 && Elem<T>::kFmt == 0 ? 0x7c00u : 0x7f80u;
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            m = __vimax3_u16x2(m, v[i].a.x & 0x7fff7fffu, v[i].a.y & 0x7fff7fffu);
+            m = __vimax3_u16x2(m, v[i].a.z & 0x7fff7fffu, v[i].a.w & 0x7fff7fffu);
+        }
+        uint32_t one = max(m & 0xffffu, m >> 16);
+        if (one >= kInf) {
+            one = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const uint16_t* e = reinterpret_cast<const uint16_t*>(&v[i].a);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const uint32_t x = e[u] & 0x7fffu;
+                    one = x < kInf ? max(one, x) : one;
+                }
+            }
+        }
+        const uint16_t bits = (uint16_t)one;
+        return Elem<T>::to_f(*reinterpret_cast<const T*>(&bits));
+    }
 };
 template <> struct Raw8<float> {
     float4 a, b;
@@ -27,7 +55,36 @@ template <> struct Raw8<float> {
     __device__ __forceinline__ float get(int i) const {
         return i < 4 ? reinterpret_cast<const float*>(&a)[i] : reinterpret_cast<const float*>(&b)[i - 4];
     }
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    template <int N> static __device__ __forceinline__ float amax(const Raw8 (&v)[N]) {
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float m = fabsf(v[i].get(u));
+                most = m <= 3.402823466e38f ? fmaxf(most, m) : most;  // infinities and NaN set no scale
+            }
+        return most;
+    }
 };
+
+// Division of n < 2^31 by a number the host knows: (n + umulhi(n, mul)) >> shift, with
+// 2^shift >= d and mul = floor(2^32 (2^shift - d) / d) + 1.
+struct Divisor {
+    uint32_t d, mul, shift;
+};
+Divisor make_divisor(uint32_t d) {
+    Divisor v = {d, 0, 0};
+    while ((1ull << v.shift) < d) ++v.shift;
+    v.mul = (uint32_t)((((1ull << v.shift) - d) << 32) / d + 1);
+    return v;
+}
+__device__ __forceinline__ uint32_t divide(uint32_t& n, const Divisor& v) {  // leaves the remainder
+    const uint32_t q = (n + __umulhi(n, v.mul)) >> v.shift, r = n - q * v.d;
+    n = r;
+    return q;
+}
 
 struct AppendArgs {
     const void* x[2];          // K, V
@@ -39,120 +96,134 @@ struct AppendArgs {
     const int* cu;
     int max_seqlen, total, B, max_blocks, n_blocks, log2P, Hkv, log2D, items_per_seq;  // blocks a sequence may touch
     long long items;
+    Divisor by_head, by_local;
 };
 
 constexpr int kAppendVecs = 8;  // vectors of 8 values a thread holds
 
-// One item = the new tokens of one sequence that fall into one block, of one head, of K or V.
-// kThreads threads hold them in registers (each value is read once from memory), reduce their
-// largest magnitude to the block's scale and write the codes.  A block begun by an earlier call
-// keeps a larger old scale; where the new tokens need a larger one, its codes are rounded to it
-// first.  Only slots below the sequence's length are written.
-// Bound by memory for prompts and by latency (three dependent loads: offsets, block id, data)
-// for a step of one token a sequence, where a warp an item keeps the grid to one short wave.
-template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads, kThreads <= 128 && sizeof(T) == 2 ? 8 : 1)
-    kv8_append_kernel(const AppendArgs a) {
-    constexpr int kCta = kThreads < 128 ? 128 : kThreads;
-    grid_dependency_wait();
-    allow_dependent_launch();
-    const int tid = threadIdx.x % kThreads;
-    const long long item = (long long)blockIdx.x * (kCta / kThreads) + threadIdx.x / kThreads;
-    if (item >= a.items) return;  // whole warps; whole CTAs where kThreads is the CTA
-    const int side = (int)(item & 1);
-    long long rest = item >> 1;
-    const int h = (int)(rest % a.Hkv);
-    rest /= a.Hkv;
-    const int local = (int)(rest % a.items_per_seq);
-    const int b = (int)(rest / a.items_per_seq);
-
+// What one item of the writer is: `count` new tokens from x on, into the slots from `before` on of one
+// head of a block, of K or V.
+struct AppendItem {
+    int side, h, token, count, before;
+    int bh;  // block * Hkv + head
+};
+__device__ __forceinline__ AppendItem append_item(const AppendArgs& a, long long item) {
+    AppendItem it = {0, 0, 0, 0, 0, 0};
+    if (item >= a.items) return it;
+    unsigned rest = (unsigned)item;
+    it.side = rest & 1;
+    rest >>= 1;
+    uint32_t local = divide(rest, a.by_head);
+    it.h = (int)rest;
+    const int b = (int)divide(local, a.by_local);
     const int L = a.lens[b];
     const int t0 = a.cu ? a.cu[b] : b;
     const long long n = a.cu ? (long long)a.cu[b + 1] - t0 : 1;
-    if (n == 0 || (!a.cu && L <= 0)) return;  // nothing new, or a padding entry of a step
+    if (n == 0 || (!a.cu && L <= 0)) return it;  // nothing new, or a padding entry of a step
     if (t0 < 0 || n < 0 || t0 + n > a.total || n > a.max_seqlen || L < n || L > ((long long)a.max_blocks << a.log2P)) {
-        if (tid == 0 && local == 0) report_invalid();
-        return;
+        if (local == 0) report_invalid();
+        return it;
     }
     const int start = L - (int)n;
-    const int bi = (start >> a.log2P) + local;
-    if (bi > (L - 1) >> a.log2P) return;
+    const int bi = (start >> a.log2P) + (int)local;
+    if (bi > (L - 1) >> a.log2P) return it;
     const int block = a.table[(size_t)b * a.max_blocks + bi];
     if (block < 0 || block >= a.n_blocks) {
-        if (tid == 0) report_invalid();
-        return;
+        report_invalid();
+        return it;
     }
     const int lo = max(start, bi << a.log2P);
-    const int count = min(L, (bi + 1) << a.log2P) - lo;
-    const int before = lo - (bi << a.log2P);  // tokens that the block holds already
-    const int D8 = a.log2D - 3;
-    const int vecs = count << D8;
+    it.token = t0 + (lo - start);
+    it.count = (int)(min((long long)L, ((long long)bi + 1) << a.log2P) - lo);
+    it.before = lo - (bi << a.log2P);
+    it.bh = block * a.Hkv + it.h;
+    return it;
+}
 
-    const T* x = static_cast<const T*>(a.x[side]) + (size_t)(t0 + (lo - start)) * a.stride_t[side] +
-                 (size_t)h * a.stride_h[side];
-    const size_t bh = (size_t)block * a.Hkv + h;
-    uint8_t* codes = a.cache[side] + ((bh << a.log2P) << a.log2D);
-    float* scale = a.scale[side] + bh;
-    const float old = before > 0 ? *scale : 0.f;
-
-    Raw8<T> raw[kAppendVecs];
-    float amax = 0.f;
+// kThreads threads hold an item's values in registers (each is read once from memory), reduce their
+// largest magnitude to the block's scale and write the codes.  A block begun by an earlier call keeps
+// a larger old scale; where the new tokens need a larger one, its codes are rounded to it first.  Only
+// slots below the sequence's length are written.
+// Bound by memory for prompts, by latency for a step of one token a sequence, where a warp has an item.
+// A grid of resident CTAs walks the items; each lane looks up one of the next 32 (a chain of two loads
+// and a hundred instructions, which with an item a CTA were half of all that ran: 25k tokens of
+// 8 sequences, D 128, 35 us so, 27 us now, 88 % of the bytes' time), and items with nothing to write
+// cost no more than that.
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads, kThreads <= 128 && sizeof(T) == 2 ? 8 : 1)
+    kv8_append_kernel(const AppendArgs a) {
+    constexpr int kItems = kThreads < 128 ? 128 / kThreads : 1;  // of a CTA at a time
+    __shared__ float part[2][kThreads / 32];
+    grid_dependency_wait();
+    allow_dependent_launch();
+    const int tid = threadIdx.x % kThreads, lane = threadIdx.x & 31;
+    const int log2_row = a.log2D - 3;  // vectors of a row
+    const long long stride = (long long)gridDim.x * kItems;
+    int turn = 0;
+    for (long long item = (long long)blockIdx.x * kItems + threadIdx.x / kThreads; item < a.items; item += 32 * stride) {
+        const AppendItem mine = append_item(a, item + lane * stride);
+        for (unsigned some = __ballot_sync(0xffffffffu, mine.count > 0); some; some &= some - 1, turn ^= 1) {
+            // the same item for all its threads: every warp of it has looked up the same ones
+            const int from = __ffs(some) - 1;
+            const int side = __shfl_sync(0xffffffffu, mine.side, from), h = __shfl_sync(0xffffffffu, mine.h, from);
+            const int count = __shfl_sync(0xffffffffu, mine.count, from);
+            const int before = __shfl_sync(0xffffffffu, mine.before, from);
+            const size_t token = __shfl_sync(0xffffffffu, mine.token, from), bh = __shfl_sync(0xffffffffu, mine.bh, from);
+            const long long stride_t = side ? a.stride_t[1] : a.stride_t[0];
+            // this thread's vectors: one every kThreads >> log2_row rows, in the same channels
+            const int row = tid >> log2_row, rows = kThreads >> log2_row;
+            const T* x = static_cast<const T*>(side ? a.x[1] : a.x[0]) + (token + row) * stride_t +
+                         (size_t)h * (side ? a.stride_h[1] : a.stride_h[0]) + ((tid & ((1 << log2_row) - 1)) << 3);
+            uint8_t* codes = (side ? a.cache[1] : a.cache[0]) + ((bh << a.log2P) << a.log2D);
+            float* scale = (side ? a.scale[1] : a.scale[0]) + bh;
+            Raw8<T> raw[kAppendVecs];
+            const float old = before > 0 ? *scale : 0.f;
 #pragma unroll
-    for (int v = 0; v < kAppendVecs; ++v) {
-        const int i = v * kThreads + tid;
-        if (i < vecs) raw[v].load(x + (size_t)(i >> D8) * a.stride_t[side] + ((i & ((1 << D8) - 1)) << 3));
-    }
-#pragma unroll
-    for (int v = 0; v < kAppendVecs; ++v) {
-        if (v * kThreads + tid < vecs) {
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float m = fabsf(raw[v].get(u));
-                amax = m <= 3.402823466e38f ? fmaxf(amax, m) : amax;  // infinities and NaN set no scale
+            for (int v = 0; v < kAppendVecs; ++v) {
+                raw[v].zero();
+                if (row + v * rows < count) raw[v].load(x + v * (rows * stride_t));
             }
-        }
-    }
+            float amax = Raw8<T>::amax(raw);
 #pragma unroll
-    for (int m = 16; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
-    if constexpr (kThreads > 32) {
-        __shared__ float part[kThreads / 32];
-        if ((tid & 31) == 0) part[tid >> 5] = amax;
-        __syncthreads();
+            for (int m = 16; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
+            if constexpr (kThreads > 32) {
+                // two sets in turn: what is read here is written again only after the next item's barrier
+                if ((tid & 31) == 0) part[turn][tid >> 5] = amax;
+                __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, part[w]);
-    }
-    const float fits = kv8_scale_for(amax);
-    const float s = fmaxf(old, fits);
-    if (before > 0 && s > old) {
-        const float ratio = old / s;
-        uint4* c = reinterpret_cast<uint4*>(codes);
-        for (int i = tid; i < before << (a.log2D - 4); i += kThreads) {
-            uint4 w = c[i];
-            uint32_t* e = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                uint32_t p0, p1;
-                kv8_decode4(e[u], p0, p1);
-                const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&p0));
-                const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&p1));
-                e[u] = kv8_encode2(f0.x * ratio, f0.y * ratio) | (kv8_encode2(f1.x * ratio, f1.y * ratio) << 16);
+                for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, part[turn][w]);
             }
-            c[i] = w;
-        }
-    }
-    if (tid == 0 && s != old) *scale = s;
-    const float inv = 1.f / s;  // exact: a power of two
-    uint8_t* dst = codes + ((size_t)before << a.log2D);
+            const float s = fmaxf(old, kv8_scale_for(amax));
+            if (before > 0 && s > old) {
+                const float ratio = old / s;
+                uint4* c = reinterpret_cast<uint4*>(codes);
+                for (int i = tid; i < before << (a.log2D - 4); i += kThreads) {
+                    uint4 w = c[i];
+                    uint32_t* e = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-    for (int v = 0; v < kAppendVecs; ++v) {
-        const int i = v * kThreads + tid;
-        if (i < vecs) {
-            uint2 w;
-            w.x = kv8_encode2(raw[v].get(0) * inv, raw[v].get(1) * inv) |
-                  (kv8_encode2(raw[v].get(2) * inv, raw[v].get(3) * inv) << 16);
-            w.y = kv8_encode2(raw[v].get(4) * inv, raw[v].get(5) * inv) |
-                  (kv8_encode2(raw[v].get(6) * inv, raw[v].get(7) * inv) << 16);
-            *reinterpret_cast<uint2*>(dst + ((size_t)i << 3)) = w;
+                    for (int u = 0; u < 4; ++u) {
+                        uint32_t p0, p1;
+                        kv8_decode4(e[u], p0, p1);
+                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&p0));
+                        const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&p1));
+                        e[u] = kv8_encode4(f0.x * ratio, f0.y * ratio, f1.x * ratio, f1.y * ratio);
+                    }
+                    c[i] = w;
+                }
+            }
+            if constexpr (kThreads == 32) __syncwarp();  // every lane has read the old scale
+            if (tid == 0 && s != old) *scale = s;
+            const float inv = 1.f / s;  // exact: a power of two
+            uint8_t* dst = codes + ((size_t)before << a.log2D) + tid * 8;
+#pragma unroll
+            for (int v = 0; v < kAppendVecs; ++v) {
+                if (row + v * rows < count) {
+                    uint2 w;
+                    w.x = kv8_encode4(raw[v].get(0) * inv, raw[v].get(1) * inv, raw[v].get(2) * inv, raw[v].get(3) * inv);
+                    w.y = kv8_encode4(raw[v].get(4) * inv, raw[v].get(5) * inv, raw[v].get(6) * inv, raw[v].get(7) * inv);
+                    *reinterpret_cast<uint2*>(dst + v * (kThreads * 8)) = w;
+                }
+            }
         }
     }
 }
@@ -249,17 +320,22 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const ReadArgs a
     }
 }
 
-template <typename T>
-int launch_append(const AppendArgs& a, long long values, cudaStream_t st) {
+template <typename T, int kThreads> int launch_append_as(const AppendArgs& a, int sms, cudaStream_t st) {
+    constexpr int kCta = kThreads < 128 ? 128 : kThreads, kItems = kCta / kThreads;
+    // as many CTAs as are resident, each with about the same number of items
+    constexpr int kResident = kThreads <= 128 && sizeof(T) == 2 ? 8 : 512 / kCta;
+    const long long ctas = (a.items + kItems - 1) / kItems, most = (long long)sms * kResident;
+    return kv8_launch(kv8_append_kernel<T, kThreads>, dim3((unsigned)(ctas < most ? ctas : most)), kCta, 0, st, a);
+}
+
+template <typename T> int launch_append(const AppendArgs& a, long long values, int sms, cudaStream_t st) {
     // values: the most one item can hold.  A warp an item up to 2048 of them, else the CTA that
     // holds them at 64 a thread.
-    const long long warp_grid = (a.items + 3) / 4;
-    if (values <= 32 * 8 * kAppendVecs) return kv8_launch(kv8_append_kernel<T, 32>, dim3((unsigned)warp_grid), 128, 0, st, a);
-    if (values <= 128 * 8 * kAppendVecs)
-        return kv8_launch(kv8_append_kernel<T, 128>, dim3((unsigned)a.items), 128, 0, st, a);
-    if (values <= 256 * 8 * kAppendVecs)
-        return kv8_launch(kv8_append_kernel<T, 256>, dim3((unsigned)a.items), 256, 0, st, a);
-    return kv8_launch(kv8_append_kernel<T, 512>, dim3((unsigned)a.items), 512, 0, st, a);
+    constexpr int kEach = 8 * kAppendVecs;
+    if (values <= 32 * kEach) return launch_append_as<T, 32>(a, sms, st);
+    if (values <= 128 * kEach) return launch_append_as<T, 128>(a, sms, st);
+    if (values <= 256 * kEach) return launch_append_as<T, 256>(a, sms, st);
+    return launch_append_as<T, 512>(a, sms, st);
 }
 
 int ilog2(int x) {
@@ -305,14 +381,17 @@ extern "C" int kv8_append_sm100(const void* k, long long k_stride_token, long lo
     a.items_per_seq = (int)(touched < max_blocks ? touched : max_blocks);
     a.items = 2LL * B * a.items_per_seq * Hkv;
     if (a.items > 0x7fffffffLL) return B200LAB_ERR_UNSUPPORTED;
-    rc = kv8_device().status;
+    a.by_head = make_divisor((uint32_t)Hkv);
+    a.by_local = make_divisor((uint32_t)a.items_per_seq);
+    const Kv8Device dev = kv8_device();
+    rc = dev.status;
     if (rc != B200LAB_OK) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const long long values = (long long)(most < block_size ? most : block_size) * D;
     switch (in_dtype) {
-        case B200LAB_F16: return launch_append<__half>(a, values, st);
-        case B200LAB_BF16: return launch_append<__nv_bfloat16>(a, values, st);
-        default: return launch_append<float>(a, values, st);
+        case B200LAB_F16: return launch_append<__half>(a, values, dev.sms, st);
+        case B200LAB_BF16: return launch_append<__nv_bfloat16>(a, values, dev.sms, st);
+        default: return launch_append<float>(a, values, dev.sms, st);
     }
 }
 
