@@ -52,9 +52,7 @@ struct Shape {
     int depth;   // pieces of a warp's ring
 };
 constexpr Shape shape_of(int D, int nt) {
-    return D == 64 ? (nt == 1 ? Shape{2, 4, 2} : nt == 2 ? Shape{1, 3, 6} : Shape{1, 2, 10})
-         : D == 128 ? (nt == 1 ? Shape{2, 3, 2} : nt == 2 ? Shape{2, 2, 2} : Shape{1, 2, 5})
-                    : (nt == 1 ? Shape{1, 2, 3} : Shape{1, 2, 2});
+    return D == 64 ? (nt == 1 ? Shape{2, 4, 2} : Shape{2, 3, 3}) : D == 128 ? (nt == 1 ? Shape{2, 3, 2} : Shape{2, 2, 2}) : Shape{1, 2, 3};
 }
 template <int D, int NT> struct Cfg {
     static constexpr int kH = shape_of(D, NT).groups;
@@ -935,12 +933,11 @@ __global__ void __launch_bounds__(256) attn_kv8_join_kernel(const Args a, int gr
     store_row<T, kVec>(a, token, head, D, lane * kVec, x, gate);
 }
 
-// Column tiles of 8 query rows a CTA works on at once: as many as the rows of a kv group fill, up
-// to what the sums leave registers for.  Rows beyond take further passes over the keys.
-int column_tiles(int rows, int D) {
-    const int most = D == 256 ? 2 : 4;
-    return rows <= 8 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
-}
+// Column tiles of 8 query rows a CTA works on at once; rows beyond take further passes over the keys,
+// which then come from L2.  Two tiles share the conversions but leave registers for fewer warps: they
+// pay from 17 rows on (B32, 2-4k keys, D 128, 32 rows: 74 us with two, 81 with one, 95 with four, 16
+// rows 34 with either), and never at D = 256 (16 rows: 51 us with one, 62 with two, which spill).
+int column_tiles(int rows, int D) { return D == 256 || rows <= 8 ? 1 : 2; }
 
 int plan_grid(int D, int nt, int sms) {
     const int g = shape_of(D, nt).ctas * sms;
@@ -982,9 +979,8 @@ template <int D, typename T>
 int launch_rows(int nt, const Args& a, void* ws, int grid, int device,
            cudaStream_t st) {
     if (nt == 1) return launch<D, 1, T>(a, ws, grid, device, st);
-    if (nt == 2) return launch<D, 2, T>(a, ws, grid, device, st);
-    if constexpr (D < 256) return launch<D, 4, T>(a, ws, grid, device, st);
-    return B200LAB_ERR_UNSUPPORTED;
+    if constexpr (D < 256) return launch<D, 2, T>(a, ws, grid, device, st);
+    return B200LAB_ERR_UNSUPPORTED;  // not reached: column_tiles
 }
 
 template <typename T>
