@@ -221,12 +221,13 @@ def test_attend_step(cuda, D, group, P, dtype):
 
 
 @pytest.mark.parametrize("causal", [True, False])
-@pytest.mark.parametrize("D,group", [(128, 4), (64, 1), (256, 6), (128, 8)])
-def test_attend_several_tokens(cuda, D, group, causal):
+@pytest.mark.parametrize("P", [16, 32, 64, 128])
+@pytest.mark.parametrize("D,group", [(128, 4), (64, 1), (256, 6), (128, 8), (64, 5)])
+def test_attend_several_tokens(cuda, D, group, P, causal):
     """Ragged query counts, some of them more than the sequence has keys (rows that see none), and more
     rows than one pass over the keys takes."""
     lens, new = [5, 64, 100, 17, 333, 2, 0], [5, 1, 9, 0, 7, 4, 2]
-    s = Setup(lens, 2, D, 32, seed=D + group, garbage=True)
+    s = Setup(lens, 2, D, P, seed=D + group, garbage=True)
     q = _normal((sum(new) + 2, 2 * group, D), 5, torch.bfloat16).cuda()
     out = torch.full_like(q, 55.0)
     _check_attend(s, q, new, causal=causal, out=out)
@@ -346,7 +347,11 @@ def test_bad_offsets_and_blocks_are_reported_not_followed(cuda):
         assert b200lab.device_status() == b200lab.ERR_INVALID, c
         if "lens" in c:
             assert bool((out[1] == 9.0).all()) and torch.equal(out[0], want[0]) and torch.equal(out[2], want[2])
-    # more new tokens than the sequence holds; a read longer than its table
+    # more new tokens than max_seqlen, than the sequence holds; a read longer than its table
+    before = s.k.view(torch.uint8).clone()
+    b200lab.kv8_append(x, x, *s.cache, s.l, cu_seqlens=_ints([0, 0, 3, 3]), max_seqlen=2)
+    assert b200lab.device_status() == b200lab.ERR_INVALID
+    assert torch.equal(before, s.k.view(torch.uint8))
     before = s.k.view(torch.uint8).clone()
     b200lab.kv8_append(x, x, *s.cache, _ints([2, 30, 20]), cu_seqlens=_ints([0, 3, 3, 3]), max_seqlen=3)
     assert b200lab.device_status() == b200lab.ERR_INVALID
@@ -452,6 +457,9 @@ def test_empty_batch_and_binding_refusals(cuda):
     assert b200lab.attn_fwd_kv8(q, *s.cache, s.l, cu_seqlens_q=zero).shape == (0, 8, 128)
     k, v = b200lab.kv8_read(*s.cache, zero, 1, 0)
     assert k.shape == v.shape == (0, 2, 128)
+    none = torch.empty((0, 3), dtype=torch.int32, device="cuda")  # no sequences at all
+    b200lab.kv8_append(x, x, *s.cache[:4], none, none[:, 0].contiguous())
+    assert b200lab.attn_fwd_kv8(q, *s.cache[:4], none, none[:, 0].contiguous()).shape == (0, 8, 128)
     s.same()
     q = torch.zeros((2, 8, 128), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(ValueError):
@@ -506,3 +514,35 @@ def test_prompt_then_steps(cuda):
         s.rv.append(v.double().numpy(), s.table, s.lens, [1] * 4)
         _check_attend(s, q.cuda(), [1] * 4)
     s.same()
+
+
+def test_first_call_inside_a_capture(cuda):
+    """A process whose first calls of all are recorded into a graph."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path[:0] = %r
+import b200lab
+b200lab.lib()
+c = [torch.zeros((4, 2, 16, 128), dtype=torch.float8_e4m3fn, device="cuda") for _ in range(2)]
+s = [torch.zeros((4, 2), device="cuda") for _ in range(2)]
+t = torch.tensor([[2, 1]], dtype=torch.int32, device="cuda")
+n = torch.tensor([3], dtype=torch.int32, device="cuda")
+x = torch.randn((3, 2, 128), device="cuda").to(torch.bfloat16)
+cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    b200lab.kv8_append(x, x, *c, *s, t, n, cu_seqlens=cu, max_seqlen=3)
+    k, v = b200lab.kv8_read(*c, *s, t, cu, 3, 3)
+    o = b200lab.attn_fwd_kv8(x, *c, *s, t, n, cu_seqlens_q=cu, max_seqlen_q=3)
+g.replay()
+torch.cuda.synchronize()
+assert b200lab.device_status() == 0
+assert torch.equal(o[0], v[0]) and float((k - x).abs().max()) < 0.5
+print("fine")
+""" % [p for p in sys.path if p]
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=dict(os.environ))
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]

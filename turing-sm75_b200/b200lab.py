@@ -156,13 +156,14 @@ def _torch():
 
 def _dtype_code(t) -> int:
     torch = _torch()
-    if t.dtype == torch.float16:
-        return F16
-    if t.dtype == torch.bfloat16:
+    dtype = t.dtype
+    if dtype is torch.bfloat16:
         return BF16
-    if t.dtype == torch.float32:
+    if dtype is torch.float16:
+        return F16
+    if dtype is torch.float32:
         return F32
-    raise TypeError(f"unsupported dtype {t.dtype}")
+    raise TypeError(f"unsupported dtype {dtype}")
 
 
 def _dev(t, name):
@@ -506,15 +507,16 @@ def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
 
 
 def _kv8_ints(t, n, name, dev):
-    if t.dtype is not _torch().int32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != dev:
+    if (t.dtype is not _torch().int32 or t.dim() != 1 or t.numel() != n or t.get_device() != dev
+            or not t.is_contiguous()):
         raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
     return t.data_ptr()
 
 
-def _rows(t, shape, name, dev):
+def _rows(t, total, H, D, name, dev):
     """Checks of a token-major [total, H, D] tensor with contiguous channels; (pointer, strides)."""
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.shape != (total, H, D):
+        raise ValueError(f"{name} must be {[total, H, D]}, got {list(t.shape)}")
     if t.get_device() != dev:
         raise ValueError(f"{name} must be on the cache's device")
     st, sh, sd = t.stride()
@@ -556,13 +558,12 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, 
     total = k.shape[0]
     if v.dtype is not k.dtype:
         raise TypeError("k and v must share a dtype")
-    shape = (total, Hkv, D)
-    kp, kt, kh = _rows(k, shape, "k", dev)
-    vp, vt, vh = _rows(v, shape, "v", dev)
+    kp, kt, kh = _rows(k, total, Hkv, D, "k", dev)
+    vp, vt, vh = _rows(v, total, Hkv, D, "v", dev)
     lens = _kv8_ints(seq_lens, B, "seq_lens", dev)
     cu = None if cu_seqlens is None else _kv8_ints(cu_seqlens, B + 1, "cu_seqlens", dev)
     code = _dtype_code(k)
-    if total == 0 and cu is not None:
+    if total == 0 and (cu is not None or B == 0):
         return
     ptr, ctx = _enter(dev, stream)
     args = (kp, kt, kh, vp, vt, vh, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
@@ -612,7 +613,7 @@ def attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q=1, D=128) -> int:
     return int(lib().attn_fwd_sm100_kv8_workspace(Hq, Hkv, int(max_seqlen_q), D))
 
 
-_kv8_workspace = {}  # (device, Hq, Hkv, max_seqlen_q, D) -> 16-bit values of a workspace
+_kv8_workspace = {}  # (device, dtype, Hq, Hkv, max_seqlen_q, D) -> one 16-bit value expanded to a workspace's size
 
 
 def attn_fwd_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *, cu_seqlens_q=None,
@@ -625,14 +626,13 @@ def attn_fwd_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *
     (n_blocks, Hkv, block_size, D), dev = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
     B, max_blocks = block_table.shape
     total, Hq = q.shape[0], q.shape[1]
-    shape = (total, Hq, D)
-    qp, qt, qh = _rows(q, shape, "q", dev)
+    qp, qt, qh = _rows(q, total, Hq, D, "q", dev)
     gp = None
     gt = gh = 0
     if gate is not None:
         if gate.dtype is not q.dtype:
             raise TypeError("gate must have q's dtype")
-        gp, gt, gh = _rows(gate, shape, "gate", dev)
+        gp, gt, gh = _rows(gate, total, Hq, D, "gate", dev)
     lens = _kv8_ints(seq_lens, B, "seq_lens", dev)
     cu = None if cu_seqlens_q is None else _kv8_ints(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
     code = _dtype_code(q)
@@ -642,18 +642,20 @@ def attn_fwd_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *
                         cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q, gate=gate, scale=scale, causal=causal,
                         out=out, workspace=workspace)
     if out is None:
-        out = q.new_empty(shape)
-    elif out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != dev:
+        out = _torch().empty_like(q) if q.is_contiguous() else q.new_empty((total, Hq, D))
+    elif out.shape != (total, Hq, D) or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError("out must be contiguous, like q, on the cache's device")
-    if total == 0 and cu is not None:
+    if total == 0 and (cu is not None or B == 0):
         return out
     if workspace is None:
-        key = (dev, Hq, Hkv, max_seqlen_q, D)
-        n = _kv8_workspace.get(key)
-        if n is None:  # at least a value, so that wrong sizes reach the library's own checks
-            n = _kv8_workspace[key] = max(1, attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q, D) // 2)
-        workspace = out.new_empty(n)
-        ws_bytes = 2 * n
+        # a tensor like a cached one of that many values that holds a single one: the quickest way to memory
+        key = (dev, code, Hq, Hkv, max_seqlen_q, D)
+        like = _kv8_workspace.get(key)
+        if like is None:  # at least a value, so that wrong sizes reach the library's own checks
+            n = max(1, attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q, D) // 2)
+            like = _kv8_workspace[key] = q.new_empty(1).expand(n)
+        workspace = _torch().empty_like(like)
+        ws_bytes = 2 * like.numel()
     else:
         if not workspace.is_contiguous() or workspace.get_device() != dev:
             raise ValueError("workspace must be contiguous, on the cache's device")
