@@ -38,10 +38,8 @@ namespace {
 
 __device__ int g_err_attn_kv8 = 0;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
+constexpr int kMostWarps = 4;             // of a CTA
 constexpr int kGroup = 16;                // keys of one product
-constexpr int kMaxGrid = 2048;            // CTAs of a call at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;              // the running maximum is moved when x exceeds it by 2^8
 
@@ -54,12 +52,12 @@ struct Shape {
 constexpr Shape shape_of(int D, int nt) {
     return D == 64 ? (nt == 1 ? Shape{2, 4, 2} : Shape{2, 3, 3}) : D == 128 ? (nt == 1 ? Shape{2, 3, 2} : Shape{2, 2, 2}) : Shape{1, 2, 3};
 }
-template <int D, int NT> struct Cfg {
+template <int D, int NT, int W> struct Cfg {  // W: warps of a CTA
     static constexpr int kH = shape_of(D, NT).groups;
     static constexpr int kPiece = kGroup * kH;
-    static constexpr int kTile = kPiece * kWarps;           // keys a CTA takes at a time
+    static constexpr int kTile = kPiece * W;                // keys a CTA takes at a time
     static constexpr int kBytes = 2 * kPiece * D;           // a piece of K, then one of V
-    static constexpr int kCtas = shape_of(D, NT).ctas;
+    static constexpr int kCtas = shape_of(D, NT).ctas * kMostWarps / W;
     static constexpr int kDepth = shape_of(D, NT).depth;
     static constexpr int kRow = 64;                         // channels joined at a time
     static constexpr int kStart = 2;                        // what a segment's start and end cost, in tiles
@@ -99,7 +97,7 @@ struct Seq {
 };
 
 // A sequence whose offsets or length are outside what the call was given has no tiles and is reported.
-template <int D, int NT> __device__ __forceinline__ Seq load_seq(const Args& a, int b, bool report) {
+template <int D, int NT, int W> __device__ __forceinline__ Seq load_seq(const Args& a, int b, bool report) {
     Seq s;
     s.L = a.lens[b];
     s.t0 = a.cu ? a.cu[b] : b;
@@ -112,7 +110,7 @@ template <int D, int NT> __device__ __forceinline__ Seq load_seq(const Args& a, 
         return s;
     }
     s.n = (int)n;
-    constexpr int kTile = Cfg<D, NT>::kTile;
+    constexpr int kTile = Cfg<D, NT, W>::kTile;
     s.tiles = max(1, (s.L + kTile - 1) / kTile);  // a sequence without keys has a tile, to write its zeros
     s.rts = (s.n * a.group + 8 * NT - 1) / (8 * NT);
     return s;
@@ -120,7 +118,7 @@ template <int D, int NT> __device__ __forceinline__ Seq load_seq(const Args& a, 
 
 // A place in the numbered tiles: sequence, kv-head, row tile, key tile (negative: in the kStart units
 // that stand for the segment's start); `left` units of the CTA's run from here on.
-template <int D, int NT> struct Cursor {
+template <int D, int NT, int W> struct Cursor {
     Seq s;
     int b, h, rt, tile, left;  // (a CTA's run fits 32 bits: 2^31 tiles would take it hours)
     // the CTA's tiles of this segment: [first, first + count), none where count <= 0
@@ -131,16 +129,27 @@ template <int D, int NT> struct Cursor {
     __device__ __forceinline__ void next(const Args& a) {
         left -= span();
         if (left <= 0) return;
-        tile = -Cfg<D, NT>::kStart;
+        tile = -Cfg<D, NT, W>::kStart;
         if (++rt < s.rts) return;
         rt = 0;
         if (++h < a.Hkv) return;
         h = 0;
         do {
-            s = load_seq<D, NT>(a, ++b, false);
+            s = load_seq<D, NT, W>(a, ++b, false);
         } while (s.tiles == 0);  // ends: tiles are left
     }
 };
+
+// The units of all sequences, summed by a warp.
+template <int D, int NT, int W> __device__ __forceinline__ long long sum_units(const Args& a, int lane) {
+    long long sum = 0;
+#pragma unroll 4
+    for (int b = lane; b < a.B; b += 32)
+        sum += load_seq<D, NT, W>(a, b, blockIdx.x == 0).template units<Cfg<D, NT, W>::kStart>(a.Hkv);
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    return sum;
+}
 
 // The units [0, total) dealt to G CTAs: total % G CTAs have one more than the others.
 struct Deal {
@@ -182,16 +191,14 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int D, int NT> struct Smem {
-    static constexpr int kRow = Cfg<D, NT>::kRow;
-    alignas(1024) uint8_t ring[kWarps][Cfg<D, NT>::kDepth][Cfg<D, NT>::kBytes];
-    alignas(16) float join[kWarps][8][kRow + 4];
+template <int D, int NT, int W> struct Smem {
+    using C = Cfg<D, NT, W>;
+    alignas(128) uint8_t ring[W][C::kDepth][C::kBytes];
+    alignas(16) float join[W > 1 ? W : 1][W > 1 ? 8 : 1][W > 1 ? C::kRow + 4 : 4];
     uint2 qfrag[NT > 1 ? NT : 1][NT > 1 ? D / 16 : 1][32];
-    GroupMeta meta[kWarps][Cfg<D, NT>::kDepth][Cfg<D, NT>::kH];
-    float m[kWarps][8 * NT], l[kWarps][8 * NT];
+    GroupMeta meta[W][C::kDepth][C::kH];
+    float m[W][8 * NT], l[W][8 * NT];
     float qscale[8 * NT];
-    long long total[kWarps];
-    Cursor<D, NT> first;
 };
 
 // The factor that brings a part's sums from its own maximum m to the common one M.  A part without
@@ -312,9 +319,9 @@ template <int kPending> __device__ __forceinline__ void copy_wait() {
 }
 
 // The pieces of one warp in the order it takes them, requested ahead of their use.
-template <int D, int NT> struct Producer {
-    using C = Cfg<D, NT>;
-    Cursor<D, NT> c;
+template <int D, int NT, int W> struct Producer {
+    using C = Cfg<D, NT, W>;
+    Cursor<D, NT, W> c;
     int k;        // next tile of the segment, from c.first()
     int block;    // lane i: block * Hkv + head of group i of the next 32 / kH pieces; -1: none
 
@@ -429,15 +436,15 @@ __device__ __forceinline__ void take_out_masked(const Args& a, const Seq& s, uin
             }
 }
 
-template <int D, int NT, typename T>
-__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
+template <int D, int NT, int W, typename T>
+__global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
     attn_kv8_kernel(const Args a) {
-    using C = Cfg<D, NT>;
+    using C = Cfg<D, NT, W>;
     constexpr int kRows = 8 * NT, kDepth = C::kDepth, kH = C::kH, kPiece = C::kPiece, kTile = C::kTile;
     constexpr int kBox = D > 128 ? 128 : D, kBoxes = D / kBox;
-    extern __shared__ uint8_t smem_raw[];
-    Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    Smem<D, NT, W>& sm = *reinterpret_cast<Smem<D, NT, W>*>(smem_raw);
+    const int tid = threadIdx.x, warp = W > 1 ? tid >> 5 : 0, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
 
     // Launched early, but lets the join kernel start only as its CTAs end (the default): a join CTA that
@@ -445,30 +452,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
     // with the trigger here, 350 without).
     grid_dependency_wait();
 
-    // ---- this CTA's run of tiles: thread i adds up the sequences of its share, the thread whose
-    // share holds the run's first tile finds its sequence
-    const int share = (a.B + kThreads - 1) / kThreads;
-    const int b0 = min(a.B, tid * share), b1 = min(a.B, b0 + share);
-    long long mine = 0;
-    Seq own;  // the last of the share: with up to 128 sequences, the only one
-    for (int b = b0; b < b1; ++b) {
-        own = load_seq<D, NT>(a, b, blockIdx.x == 0);
-        mine += own.units<C::kStart>(a.Hkv);
-    }
-    long long upto = mine;
-#pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, upto, m);
-        if (lane >= m) upto += other;
-    }
-    if (lane == 31) sm.total[warp] = upto;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) upto += sm.total[w];
-        total += sm.total[w];
-    }
+    // ---- this CTA's run of tiles.  Every warp finds it for itself, a sequence a lane, 32 at a time
+    Cursor<D, NT, W> cur;
+    const long long total = sum_units<D, NT, W>(a, lane);
     const int G = (int)min((long long)gridDim.x, total);
     if ((int)blockIdx.x >= G) {
         if (tid == 0) a.meta[4 * blockIdx.x] = -1;
@@ -476,31 +462,40 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
     }
     const Deal deal(total, G);
     const long long u0 = deal.start(blockIdx.x), u1 = deal.start(blockIdx.x + 1);
-    if (upto - mine <= u0 && u0 < upto) {
-        long long at = upto - mine;
-        int b = b0;
-        Seq s;
-        for (;; ++b) {
-            s = b == b1 - 1 ? own : load_seq<D, NT>(a, b, false);
-            const long long n = s.units<C::kStart>(a.Hkv);
-            if (u0 < at + n) break;
-            at += n;
+    long long before = 0;             // units of the sequences before this chunk of 32
+    for (int b = lane;; b += 32) {    // ends: u0 < total
+        Seq s = {0, 0, 0, 0, 0};
+        if (b < a.B) s = load_seq<D, NT, W>(a, b, false);
+        const long long mine = s.units<C::kStart>(a.Hkv);
+        long long upto = mine;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            const long long other = __shfl_up_sync(0xffffffffu, upto, m);
+            if (lane >= m) upto += other;
         }
-        // the segment and the tile in it; a sequence's units fit 32 bits nearly always
-        const long long local = u0 - at;
-        const int per = s.tiles + C::kStart;
-        const long long seg = local <= 0x7fffffffLL ? (long long)((uint32_t)local / (uint32_t)per) : local / per;
-        sm.first.s = s;
-        sm.first.b = b;
-        sm.first.tile = (int)(local - seg * per) - C::kStart;
-        sm.first.h = (int)(seg / s.rts);
-        sm.first.rt = (int)(seg - (long long)sm.first.h * s.rts);
-        sm.first.left = (int)(u1 - u0);
+        const unsigned past = __ballot_sync(0xffffffffu, u0 < before + upto);
+        if (past) {
+            const int from = __ffs(past) - 1;  // the lane whose sequence holds the run's first unit
+            cur.s.n = __shfl_sync(0xffffffffu, s.n, from);
+            cur.s.L = __shfl_sync(0xffffffffu, s.L, from);
+            cur.s.t0 = __shfl_sync(0xffffffffu, s.t0, from);
+            cur.s.tiles = __shfl_sync(0xffffffffu, s.tiles, from);
+            cur.s.rts = __shfl_sync(0xffffffffu, s.rts, from);
+            cur.b = __shfl_sync(0xffffffffu, b, from);
+            // the segment and the tile in it; a sequence's units fit 32 bits nearly always
+            const long long local = u0 - before - __shfl_sync(0xffffffffu, upto - mine, from);
+            const int per = cur.s.tiles + C::kStart;
+            const long long seg = local <= 0x7fffffffLL ? (long long)((uint32_t)local / (uint32_t)per) : local / per;
+            cur.tile = (int)(local - seg * per) - C::kStart;
+            cur.h = (int)(seg / cur.s.rts);
+            cur.rt = (int)(seg - (long long)cur.h * cur.s.rts);
+            cur.left = (int)(u1 - u0);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    __syncthreads();
-    Cursor<D, NT> cur = sm.first;
 
-    Producer<D, NT> pro;
+    Producer<D, NT, W> pro;
     pro.c = cur;
     pro.k = 0;
     int slot = 0;  // the next piece's
@@ -529,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                 qs[0][0] = __shfl_sync(0xffffffffu, f, 8 * t);
                 qs[0][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
             } else {
-                for (int nt = warp; nt < NT; nt += kWarps) {
+                for (int nt = warp; nt < NT; nt += W) {
                     const T* q = nullptr;
                     if (nt * 8 + g < rows) {
                         int i, hg;
@@ -543,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                     for (int ks = 0; ks < D / 16; ++ks) sm.qfrag[nt][ks][lane] = make_uint2(f[ks][0], f[ks][1]);
                     if (t == 0) sm.qscale[nt * 8 + g] = x;
                 }
-                __syncthreads();  // read again only after the joins below, which end with one too
+                __syncthreads();  // written again only after the join below, which ends with one too
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     qs[nt][0] = sm.qscale[nt * 8 + 2 * t];
@@ -743,23 +738,68 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
             if (++slot == kDepth) slot = 0;
         }
 
-        // ---- join the warps' sums
+        // ---- the sums of this run's part of the segment
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int x = 4; x <= 16; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+        const bool whole = first == 0 && run == s.tiles;
+        const int part = blockIdx.x * 2 + (first == 0 ? 1 : 0);
+        float2* part_ml = reinterpret_cast<float2*>(a.part + (size_t)gridDim.x * 2 * kRows * D) + (size_t)part * kRows;
+        constexpr int kOwn = kBox / 8;  // consecutive channels a thread has in a box, of rows 2t and 2t + 1
+        if constexpr (W == 1) {
+            // no other warp's to add: from the registers to where they belong
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int n = nt * 8 + 2 * t + c;
+                    if (n >= rows) continue;
+                    const float inv = l[nt][c] == 0.f ? 0.f : 1.f / l[nt][c];  // a row that sees no key: 0
+                    int i, hg;
+                    row_place(row0 + n, a.group, i, hg);
+                    const size_t token = (size_t)(s.t0 + i);
+                    const int head = cur.h * a.group + hg;
+                    if (!whole && g == 0) part_ml[n] = make_float2(m[nt][c], l[nt][c]);
+#pragma unroll
+                    for (int e = 0; e < D / 64; ++e) {  // 8 channels at a time
+                        const int box = e / (kOwn / 8), from = (e % (kOwn / 8)) * 8, ch = box * kBox + kOwn * g + from;
+                        float x[8];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            x[2 * u] = o[nt][box * (kBox / 16) + from / 2 + u][c];
+                            x[2 * u + 1] = o[nt][box * (kBox / 16) + from / 2 + u][c + 2];
+                        }
+                        if (whole) {
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) x[u] *= inv;
+                            Channels<T, 8> gate;
+                            if (a.g) gate.load_gate(a, token, head, ch);
+                            store_row<T, 8>(a, token, head, D, ch, x, gate);
+                        } else {
+                            float4* p = reinterpret_cast<float4*>(a.part + ((size_t)part * kRows + n) * D + ch);
+                            p[0] = make_float4(x[0], x[1], x[2], x[3]);
+                            p[1] = make_float4(x[4], x[5], x[6], x[7]);
+                        }
+                    }
+                }
+            __syncwarp();  // qfrag is read no more
+        } else {
+        // the other warps' are added by way of shared memory, kRow channels at a time
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
                 if (g == 0) {
                     sm.m[warp][nt * 8 + 2 * t + c] = m[nt][c];
                     sm.l[warp][nt * 8 + 2 * t + c] = l[nt][c];
                 }
-            }
         __syncthreads();
-        const bool whole = first == 0 && run == s.tiles;
-        const int part = blockIdx.x * 2 + (first == 0 ? 1 : 0);
-        constexpr int kRow = Smem<D, NT>::kRow, kPer = kRow / 16;
+        constexpr int kRow = C::kRow, kPer = kRow / 16;
         const int jr = tid >> 4, jd = (tid & 15) * kPer;  // this thread's row of a column tile, and channels
+        static_assert(W == 4, "8 rows x 16 threads");
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float f[2];
@@ -768,13 +808,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                 const int n = nt * 8 + 2 * t + c;
                 float M = sm.m[0][n];
 #pragma unroll
-                for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sm.m[w][n]);
+                for (int w = 1; w < W; ++w) M = fmaxf(M, sm.m[w][n]);
                 f[c] = part_weight(m[nt][c], l[nt][c], M);
             }
 #pragma unroll
             for (int d = 0; d < D / kRow; ++d) {
-                // rows 2t, 2t + 1; a thread has kOwn consecutive channels of a box, kRow / kOwn threads a join
-                constexpr int kOwn = kBox / 8, kSharers = kRow / kOwn, kJoins = kBox / kRow;
+                constexpr int kSharers = kRow / kOwn, kJoins = kBox / kRow;
                 if (g / kSharers == d % kJoins) {
 #pragma unroll
                     for (int i = 0; i < kOwn / 2; i += 2) {
@@ -791,16 +830,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
                 if (n < rows) {
                     float M = sm.m[0][n];
 #pragma unroll
-                    for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sm.m[w][n]);
+                    for (int w = 1; w < W; ++w) M = fmaxf(M, sm.m[w][n]);
                     float sum = 0.f;
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w)
+                    for (int w = 0; w < W; ++w)
                         sum += sm.l[w][n] * part_weight(sm.m[w][n], sm.l[w][n], M);
                     float x[kPer];
 #pragma unroll
                     for (int u = 0; u < kPer; ++u) x[u] = 0.f;
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w)
+                    for (int w = 0; w < W; ++w)
 #pragma unroll
                         for (int u = 0; u < kPer; ++u) x[u] += sm.join[w][jr][jd + u];
                     if (whole) {
@@ -819,13 +858,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas)
 #pragma unroll
                         for (int u = 0; u < kPer; u += 4)
                             *reinterpret_cast<float4*>(p + u) = make_float4(x[u], x[u + 1], x[u + 2], x[u + 3]);
-                        if (d == 0 && jd == 0)
-                            reinterpret_cast<float2*>(a.part + (size_t)gridDim.x * 2 * kRows * D)[(size_t)part * kRows + n] =
-                                make_float2(M, sum);
+                        if (d == 0 && jd == 0) part_ml[n] = make_float2(M, sum);
                     }
                 }
                 __syncthreads();
             }
+        }
         }
         if (first == 0 && run < s.tiles) {
             has_tail = true;
@@ -939,31 +977,34 @@ __global__ void __launch_bounds__(256) attn_kv8_join_kernel(const Args a, int gr
 // rows 34 with either), and never at D = 256 (16 rows: 51 us with one, 62 with two, which spill).
 int column_tiles(int rows, int D) { return D == 256 || rows <= 8 ? 1 : 2; }
 
-int plan_grid(int D, int nt, int sms) {
-    const int g = shape_of(D, nt).ctas * sms;
-    return g < kMaxGrid ? g : kMaxGrid;
+int plan_grid(int D, int nt, int warps, int sms) {
+    return shape_of(D, nt).ctas * kMostWarps / warps * sms;
 }
 
-size_t workspace_bytes(int nt, int D, int sms) {
-    const size_t grid = plan_grid(D, nt, sms), rows = grid * 2 * 8 * nt;
-    return rows * D * 4 + rows * 8 + grid * 16;
+// Warps of a CTA.
+int warps_of(long long segments, int D, int nt, int sms) {
+    return segments >= (long long)plan_grid(D, nt, 1, sms) ? 1 : 4;
 }
 
-template <int D, int NT, typename T>
-int launch(Args a, void* ws, int grid, int device,
-           cudaStream_t st) {
+size_t workspace_bytes(int D, int nt, int grid) {
+    const size_t rows = (size_t)grid * 2 * 8 * nt;
+    return rows * D * 4 + rows * 8 + (size_t)grid * 16;
+}
+
+template <int D, int NT, int W, typename T>
+int launch(Args a, void* ws, int grid, int device, cudaStream_t st) {
     const size_t rows = (size_t)grid * 2 * 8 * NT;
     a.part = static_cast<float*>(ws);
     a.meta = reinterpret_cast<int*>(a.part + rows * D + rows * 2);
-    constexpr size_t smem = sizeof(Smem<D, NT>) + 1024;
-    auto kern = attn_kv8_kernel<D, NT, T>;
+    constexpr size_t smem = sizeof(Smem<D, NT, W>);
+    auto kern = attn_kv8_kernel<D, NT, W, T>;
     static std::atomic<unsigned long long> ready{0};  // devices whose limit is raised
     const unsigned long long bit = device < 64 ? 1ull << device : 0;
     if (!bit || !(ready.load(std::memory_order_relaxed) & bit)) {
         B200_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    int rc = kv8_launch(kern, dim3(grid), kThreads, smem, st, a);
+    int rc = kv8_launch(kern, dim3(grid), 32 * W, smem, st, a);
     if (rc != B200LAB_OK) return rc;
     const long long used = (long long)a.group * a.max_seqlen_q;
     const int rows_used = (int)(used < 8 * NT ? used : 8 * NT);
@@ -975,22 +1016,19 @@ int launch(Args a, void* ws, int grid, int device,
     return kv8_launch(attn_kv8_join_kernel<D, NT, T, 1>, dim3(grid, rows_used), 256, 0, st, a, grid);
 }
 
-template <int D, typename T>
-int launch_rows(int nt, const Args& a, void* ws, int grid, int device,
-           cudaStream_t st) {
-    if (nt == 1) return launch<D, 1, T>(a, ws, grid, device, st);
-    if constexpr (D < 256) return launch<D, 2, T>(a, ws, grid, device, st);
-    return B200LAB_ERR_UNSUPPORTED;  // not reached: column_tiles
+template <int D, int NT, typename T>
+int launch_warps(int warps, const Args& a, void* ws, int grid, int device, cudaStream_t st) {
+    return warps == 1 ? launch<D, NT, 1, T>(a, ws, grid, device, st) : launch<D, NT, 4, T>(a, ws, grid, device, st);
 }
 
 template <typename T>
-int launch_d(int D, int nt, const Args& a, void* ws, int grid,
-             int device, cudaStream_t st) {
-    switch (D) {
-        case 64: return launch_rows<64, T>(nt, a, ws, grid, device, st);
-        case 128: return launch_rows<128, T>(nt, a, ws, grid, device, st);
-        default: return launch_rows<256, T>(nt, a, ws, grid, device, st);
-    }
+int launch_d(int D, int nt, int warps, const Args& a, void* ws, int grid, int device, cudaStream_t st) {
+    if (D == 256) return launch_warps<256, 1, T>(warps, a, ws, grid, device, st);
+    if (D == 128)
+        return nt == 1 ? launch_warps<128, 1, T>(warps, a, ws, grid, device, st)
+                       : launch_warps<128, 2, T>(warps, a, ws, grid, device, st);
+    return nt == 1 ? launch_warps<64, 1, T>(warps, a, ws, grid, device, st)
+                   : launch_warps<64, 2, T>(warps, a, ws, grid, device, st);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -1003,7 +1041,8 @@ B200_DEFINE_ERR_TAKER(attn_kv8, b200::g_err_attn_kv8)
 extern "C" size_t attn_fwd_sm100_kv8_workspace(int Hq, int Hkv, int max_seqlen_q, int D) {
     if (Hq < 1 || Hkv < 1 || Hq % Hkv || max_seqlen_q < 1 || (D != 64 && D != 128 && D != 256)) return 0;
     const long long rows = (long long)(Hq / Hkv) * max_seqlen_q;
-    return b200::workspace_bytes(b200::column_tiles(rows < 64 ? (int)rows : 64, D), D, b200::device_sm_count());
+    const int nt = b200::column_tiles(rows < 64 ? (int)rows : 64, D);
+    return b200::workspace_bytes(D, nt, b200::plan_grid(D, nt, 1, b200::device_sm_count()));
 }
 
 extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long long q_stride_head, const void* G,
@@ -1030,8 +1069,10 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     if (rows > 0xffffffLL) return B200LAB_ERR_UNSUPPORTED;  // 24 bits in a segment's description
     const int nt = column_tiles((int)rows, D);
     const Kv8Device dev = kv8_device();
-    const int sms = dev.sms > 0 ? dev.sms : device_sm_count(), grid = plan_grid(D, nt, sms);
-    if (!workspace || ws_bytes < workspace_bytes(nt, D, sms)) return B200LAB_ERR_WORKSPACE;
+    const int sms = dev.sms > 0 ? dev.sms : device_sm_count();
+    const int warps = warps_of((long long)B * Hkv * ((rows + 8 * nt - 1) / (8 * nt)), D, nt, sms);
+    const int grid = plan_grid(D, nt, warps, sms);
+    if (!workspace || ws_bytes < workspace_bytes(D, nt, plan_grid(D, nt, 1, sms))) return B200LAB_ERR_WORKSPACE;
     if (dev.status != B200LAB_OK) return dev.status;
     Args a;
     a.q = Q, a.g = G, a.o = O;
@@ -1043,6 +1084,6 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     a.log2P = kv8_log2_block(block_size), a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv, a.causal = causal;
     a.scale = scale;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, a, workspace, grid, dev.ordinal, st)
-                                : launch_d<__nv_bfloat16>(D, nt, a, workspace, grid, dev.ordinal, st);
+    return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, warps, a, workspace, grid, dev.ordinal, st)
+                                : launch_d<__nv_bfloat16>(D, nt, warps, a, workspace, grid, dev.ordinal, st);
 }
