@@ -140,15 +140,14 @@ template <int D, int NT, int W> struct Cursor {
     }
 };
 
-// The units of all sequences, summed by a warp.
-template <int D, int NT, int W> __device__ __forceinline__ long long sum_units(const Args& a, int lane) {
-    long long sum = 0;
-#pragma unroll 4
-    for (int b = lane; b < a.B; b += 32)
-        sum += load_seq<D, NT, W>(a, b, blockIdx.x == 0).template units<Cfg<D, NT, W>::kStart>(a.Hkv);
+// Sums of the lanes up to and including this one.
+__device__ __forceinline__ long long scan(long long x, int lane) {
 #pragma unroll
-    for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-    return sum;
+    for (int m = 1; m < 32; m <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffu, x, m);
+        if (lane >= m) x += other;
+    }
+    return x;
 }
 
 // The units [0, total) dealt to G CTAs: total % G CTAs have one more than the others.
@@ -452,9 +451,19 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
     // with the trigger here, 350 without).
     grid_dependency_wait();
 
-    // ---- this CTA's run of tiles.  Every warp finds it for itself, a sequence a lane, 32 at a time
+    // ---- this CTA's run of tiles.  Every warp finds it for itself: a lane adds up the sequences of its
+    // share, then the share that holds the run's first unit is looked at, a sequence a lane
     Cursor<D, NT, W> cur;
-    const long long total = sum_units<D, NT, W>(a, lane);
+    const int share = (a.B + 31) / 32;
+    Seq s = {0, 0, 0, 0, 0};
+    long long mine = 0;
+#pragma unroll 4
+    for (int b = min(a.B, lane * share), i = 0; i < share && b < a.B; ++i, ++b) {
+        s = load_seq<D, NT, W>(a, b, blockIdx.x == 0);
+        mine += s.template units<C::kStart>(a.Hkv);
+    }
+    long long upto = scan(mine, lane);
+    const long long total = __shfl_sync(0xffffffffu, upto, 31);
     const int G = (int)min((long long)gridDim.x, total);
     if ((int)blockIdx.x >= G) {
         if (tid == 0) a.meta[4 * blockIdx.x] = -1;
@@ -462,37 +471,40 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
     }
     const Deal deal(total, G);
     const long long u0 = deal.start(blockIdx.x), u1 = deal.start(blockIdx.x + 1);
-    long long before = 0;             // units of the sequences before this chunk of 32
-    for (int b = lane;; b += 32) {    // ends: u0 < total
-        Seq s = {0, 0, 0, 0, 0};
-        if (b < a.B) s = load_seq<D, NT, W>(a, b, false);
-        const long long mine = s.units<C::kStart>(a.Hkv);
-        long long upto = mine;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            const long long other = __shfl_up_sync(0xffffffffu, upto, m);
-            if (lane >= m) upto += other;
+    int from = __ffs(__ballot_sync(0xffffffffu, u0 < upto)) - 1;  // there is one: u0 < total
+    cur.b = from * share;
+    long long before = __shfl_sync(0xffffffffu, upto - mine, from);  // units before the sequence in hand
+    if (share > 1) {
+        const int end = min(a.B, cur.b + share);
+        for (int b = cur.b + lane;; b += 32) {
+            s.tiles = 0;
+            if (b < end) s = load_seq<D, NT, W>(a, b, false);
+            mine = s.template units<C::kStart>(a.Hkv);
+            upto = scan(mine, lane);
+            const unsigned past = __ballot_sync(0xffffffffu, u0 < before + upto);
+            if (past) {  // ends: the share holds u0
+                from = __ffs(past) - 1;
+                cur.b = __shfl_sync(0xffffffffu, b, from);
+                before += __shfl_sync(0xffffffffu, upto - mine, from);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        const unsigned past = __ballot_sync(0xffffffffu, u0 < before + upto);
-        if (past) {
-            const int from = __ffs(past) - 1;  // the lane whose sequence holds the run's first unit
-            cur.s.n = __shfl_sync(0xffffffffu, s.n, from);
-            cur.s.L = __shfl_sync(0xffffffffu, s.L, from);
-            cur.s.t0 = __shfl_sync(0xffffffffu, s.t0, from);
-            cur.s.tiles = __shfl_sync(0xffffffffu, s.tiles, from);
-            cur.s.rts = __shfl_sync(0xffffffffu, s.rts, from);
-            cur.b = __shfl_sync(0xffffffffu, b, from);
-            // the segment and the tile in it; a sequence's units fit 32 bits nearly always
-            const long long local = u0 - before - __shfl_sync(0xffffffffu, upto - mine, from);
-            const int per = cur.s.tiles + C::kStart;
-            const long long seg = local <= 0x7fffffffLL ? (long long)((uint32_t)local / (uint32_t)per) : local / per;
-            cur.tile = (int)(local - seg * per) - C::kStart;
-            cur.h = (int)(seg / cur.s.rts);
-            cur.rt = (int)(seg - (long long)cur.h * cur.s.rts);
-            cur.left = (int)(u1 - u0);
-            break;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    cur.s.n = __shfl_sync(0xffffffffu, s.n, from);
+    cur.s.L = __shfl_sync(0xffffffffu, s.L, from);
+    cur.s.t0 = __shfl_sync(0xffffffffu, s.t0, from);
+    cur.s.tiles = __shfl_sync(0xffffffffu, s.tiles, from);
+    cur.s.rts = __shfl_sync(0xffffffffu, s.rts, from);
+    {
+        // the segment and the tile in it; a sequence's units fit 32 bits nearly always
+        const long long local = u0 - before;
+        const int per = cur.s.tiles + C::kStart;
+        const long long seg = local <= 0x7fffffffLL ? (long long)((uint32_t)local / (uint32_t)per) : local / per;
+        cur.tile = (int)(local - seg * per) - C::kStart;
+        cur.h = (int)(seg / cur.s.rts);
+        cur.rt = (int)(seg - (long long)cur.h * cur.s.rts);
+        cur.left = (int)(u1 - u0);
     }
 
     Producer<D, NT, W> pro;
@@ -981,9 +993,16 @@ int plan_grid(int D, int nt, int warps, int sms) {
     return shape_of(D, nt).ctas * kMostWarps / warps * sms;
 }
 
-// Warps of a CTA.
-int warps_of(long long segments, int D, int nt, int sms) {
-    return segments >= (long long)plan_grid(D, nt, 1, sms) ? 1 : 4;
+// Warps of a CTA.  Four share the tiles of a segment and join their sums in shared memory, which
+// leaves few cut segments; a warp on its own joins nothing, and while it starts or ends a segment the
+// SM's other warps go on: better where segments are short and many.  The lengths are on the device, so
+// the rule goes by what the host has, the segments and the most that the block table can hold (measured
+// with four / with one, 32 q-heads on 8 kv-heads of 128 unless said: B64 x 200 tokens 15.0 / 14.0 us,
+// B128 x 200 25.3 / 21.5, B256 x 200 42.8 / 29.8, B512 x 64 58 / 35, B128 x 2k D 64 32 heads 149 / 137,
+// B256 x 1k 81 / 82, and the other way B256 x 200..4k 188 / 198, B32 x 200 11.3 / 16.8).
+int warps_of(long long segments, long long tokens, int D, int nt, int sms) {
+    const long long alone = plan_grid(D, nt, 1, sms);
+    return segments >= (tokens <= 512 ? alone / 2 : alone) ? 1 : 4;
 }
 
 size_t workspace_bytes(int D, int nt, int grid) {
@@ -1070,7 +1089,8 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     const int nt = column_tiles((int)rows, D);
     const Kv8Device dev = kv8_device();
     const int sms = dev.sms > 0 ? dev.sms : device_sm_count();
-    const int warps = warps_of((long long)B * Hkv * ((rows + 8 * nt - 1) / (8 * nt)), D, nt, sms);
+    const int warps = warps_of((long long)B * Hkv * ((rows + 8 * nt - 1) / (8 * nt)), (long long)max_blocks * block_size, D,
+                               nt, sms);
     const int grid = plan_grid(D, nt, warps, sms);
     if (!workspace || ws_bytes < workspace_bytes(D, nt, plan_grid(D, nt, 1, sms))) return B200LAB_ERR_WORKSPACE;
     if (dev.status != B200LAB_OK) return dev.status;
