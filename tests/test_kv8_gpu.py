@@ -441,6 +441,17 @@ def test_same_call_twice_gives_the_same_bits(cuda):
         assert torch.equal(first, b200lab.attn_fwd_kv8(q, *s.cache, s.l))
 
 
+def test_calls_share_the_library_of_the_other_entries(cuda):
+    """The extension module calls the library that ctypes has loaded: one launch count, one status."""
+    s = Setup([40], 2, 128, 16, seed=1)
+    n = b200lab.launch_count()
+    b200lab.attn_fwd_kv8(_normal((1, 8, 128), 1, torch.bfloat16).cuda(), *s.cache, s.l)
+    assert b200lab.launch_count() == n + 2
+    b200lab.kv8_append(_normal((1, 2, 128), 1, torch.bfloat16).cuda(), _normal((1, 2, 128), 2, torch.bfloat16).cuda(), *s.cache, s.l)
+    assert b200lab.launch_count() == n + 3
+    assert b200lab.device_status() == b200lab.OK
+
+
 def test_many_sequences(cuda):
     """More sequences than a CTA has threads, most of them short or padding."""
     lens = [(i * 37) % 90 if i % 3 else 0 for i in range(700)]

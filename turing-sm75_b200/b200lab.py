@@ -1,7 +1,9 @@
 """Python binding of the B200-native attention / Gated DeltaNet library.
 
 A thin ctypes layer over ``lib/libb200lab.so`` (C ABI in ``include/b200lab.h``)
-that takes torch CUDA tensors.  torch is used only for device memory and
+that takes torch CUDA tensors; the calls of the 8-bit key/value cache, made once
+a layer and token, go through an extension module (``lib/_b200torch.so``) for
+their host time.  torch is used only for device memory and
 streams; every computation runs in the library's sm_100a kernels.  There is
 no CPU fallback: if the shared library is missing or the device is not a
 B200, calls raise.
@@ -143,27 +145,20 @@ def _check(status: int, what: str) -> None:
 # ----------------------------------------------------------------------------
 # torch-facing wrappers
 # ----------------------------------------------------------------------------
-_TORCH = None
-
-
 def _torch():
-    global _TORCH
-    if _TORCH is None:
-        import torch
-        _TORCH = torch
-    return _TORCH
+    import torch
+    return torch
 
 
 def _dtype_code(t) -> int:
     torch = _torch()
-    dtype = t.dtype
-    if dtype is torch.bfloat16:
-        return BF16
-    if dtype is torch.float16:
+    if t.dtype == torch.float16:
         return F16
-    if dtype is torch.float32:
+    if t.dtype == torch.bfloat16:
+        return BF16
+    if t.dtype == torch.float32:
         return F32
-    raise TypeError(f"unsupported dtype {dtype}")
+    raise TypeError(f"unsupported dtype {t.dtype}")
 
 
 def _dev(t, name):
@@ -473,76 +468,33 @@ def gdn_decode_slots(q, k, v, g_log, beta, state_pool, slots, *, scale: float | 
 
 
 # ---- 8-bit key/value cache -------------------------------------------------
-# These calls are made once a layer and token, so the checks are kept cheap: one condition over all
-# tensors, and the search for what it was only once it fails.
-def _kv8_refuse(k_cache, v_cache, k_scale, v_scale, block_table):
-    torch = _torch()
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
-        raise ValueError("k_cache and v_cache must be [n_blocks, Hkv, block_size, D], alike")
-    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
-        raise TypeError("k_cache and v_cache must be float8_e4m3fn")
-    if k_scale.shape != k_cache.shape[:2] or v_scale.shape != k_cache.shape[:2]:
-        raise ValueError("k_scale and v_scale must be [n_blocks, Hkv]")
-    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
-        raise TypeError("k_scale and v_scale must be float32")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32:
-        raise ValueError("block_table must be int32 [B, max_blocks]")
-    raise ValueError("the cache, its scales and the block table must be contiguous CUDA tensors on one device")
+_NATIVE = None
 
 
-def _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table):
-    """Checks of the cache's tensors; returns ((n_blocks, Hkv, block_size, D), device index)."""
-    torch = _torch()
-    shape, dev, e4m3, f32 = k_cache.shape, k_cache.get_device(), torch.float8_e4m3fn, torch.float32
-    if dev < 0:
-        raise ValueError("k_cache must be a CUDA tensor (no CPU path)")
-    if not (len(shape) == 4 and v_cache.shape == shape and k_cache.dtype is e4m3 and v_cache.dtype is e4m3
-            and k_scale.shape == v_scale.shape == shape[:2] and k_scale.dtype is f32 and v_scale.dtype is f32
-            and block_table.dtype is torch.int32 and block_table.dim() == 2
-            and v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == block_table.get_device() == dev
-            and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
-            and v_scale.is_contiguous() and block_table.is_contiguous()):
-        _kv8_refuse(k_cache, v_cache, k_scale, v_scale, block_table)
-    return shape, dev
+def _native():
+    """The extension module lib/_b200torch.so (raises if it has not been built)."""
+    global _NATIVE
+    if _NATIVE is None:
+        import importlib.machinery
+        import importlib.util
+        _torch()  # its libraries first
+        lib()
+        path = os.path.join(_HERE, "lib", "_b200torch.so")
+        if not os.path.exists(path):
+            raise FileNotFoundError(f"{path} is missing: build it with `make -C {_HERE}`")
+        loader = importlib.machinery.ExtensionFileLoader("_b200torch", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_b200torch", loader))
+        loader.exec_module(module)
+        _NATIVE = module
+    return _NATIVE
 
 
-def _kv8_ints(t, n, name, dev):
-    if (t.dtype is not _torch().int32 or t.dim() != 1 or t.numel() != n or t.get_device() != dev
-            or not t.is_contiguous()):
-        raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
-    return t.data_ptr()
-
-
-def _rows(t, total, H, D, name, dev):
-    """Checks of a token-major [total, H, D] tensor with contiguous channels; (pointer, strides)."""
-    if t.shape != (total, H, D):
-        raise ValueError(f"{name} must be {[total, H, D]}, got {list(t.shape)}")
-    if t.get_device() != dev:
-        raise ValueError(f"{name} must be on the cache's device")
-    st, sh, sd = t.stride()
-    if sd != 1:
-        raise ValueError(f"{name} must have contiguous channels")
-    return t.data_ptr(), st, sh
-
-
-def _enter(dev, stream):
-    """(handle of the stream to launch on, context that makes device `dev` and that stream the
-    current ones, so that new tensors belong to them, or None where they are already)."""
-    torch = _torch()
-    if torch.cuda.current_device() == dev:
-        cur = torch._C._cuda_getCurrentRawStream(dev)  # torch.cuda.current_stream takes 2 us for it
-        if stream is None or stream.cuda_stream == cur:
-            return cur, None
-    elif stream is None:
-        stream = torch.cuda.current_stream(dev)
-    if stream.device_index != dev:
-        raise ValueError("stream belongs to another device than the tensors")
-    return stream.cuda_stream, torch.cuda.stream(stream)  # sets the device too
-
-
-def _entered(ctx, f, *args, **kw):
-    with ctx:
-        return f(*args, **kw)
+def _on_stream(stream, k_cache, f, *args):
+    """f on `stream`, to which the tensors that it allocates then belong."""
+    if stream.device != k_cache.device:
+        raise ValueError("stream belongs to another device than the cache")
+    with _torch().cuda.stream(stream):
+        return f(*args)
 
 
 def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *, cu_seqlens=None,
@@ -553,24 +505,9 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, 
     block_table int32 [B,max_blocks]; seq_lens int32 [B], the new tokens counted; cu_seqlens int32
     [B+1] of the new tokens (None: one a sequence, seq_lens <= 0 marking padding) with max_seqlen
     the most of one sequence."""
-    (n_blocks, Hkv, block_size, D), dev = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
-    B, max_blocks = block_table.shape
-    total = k.shape[0]
-    if v.dtype is not k.dtype:
-        raise TypeError("k and v must share a dtype")
-    kp, kt, kh = _rows(k, total, Hkv, D, "k", dev)
-    vp, vt, vh = _rows(v, total, Hkv, D, "v", dev)
-    lens = _kv8_ints(seq_lens, B, "seq_lens", dev)
-    cu = None if cu_seqlens is None else _kv8_ints(cu_seqlens, B + 1, "cu_seqlens", dev)
-    code = _dtype_code(k)
-    if total == 0 and (cu is not None or B == 0):
-        return
-    ptr, ctx = _enter(dev, stream)
-    args = (kp, kt, kh, vp, vt, vh, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            block_table.data_ptr(), lens, cu, int(max_seqlen), total, B, max_blocks, n_blocks, block_size, Hkv, D,
-            code, ptr)
-    f = lib().kv8_append_sm100
-    st = f(*args) if ctx is None else _entered(ctx, f, *args)
+    args = (k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, max_seqlen)
+    f = _native().append
+    st = f(*args) if stream is None else _on_stream(stream, k_cache, f, *args)
     if st != OK:
         raise B200LabError(st, "kv8_append_sm100")
 
@@ -579,41 +516,17 @@ def kv8_read(k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, max_se
              out_dtype=None, k_out=None, v_out=None, stream=None):
     """Read the first cu_seqlens[b+1] - cu_seqlens[b] tokens of each sequence back from the 8-bit
     cache, packed [total_tokens,Hkv,D] in out_dtype (fp16/bf16/fp32, default bf16).  Returns (k, v)."""
-    torch = _torch()
-    (n_blocks, Hkv, block_size, D), dev = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
-    B, max_blocks = block_table.shape
-    cu = _kv8_ints(cu_seqlens, B + 1, "cu_seqlens", dev)
-    shape = (int(total_tokens), Hkv, D)
-    ptr, ctx = _enter(dev, stream)
-    if ctx is not None:
-        return _entered(ctx, kv8_read, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, max_seqlen,
-                        total_tokens, out_dtype=out_dtype, k_out=k_out, v_out=v_out)
-    if k_out is None and v_out is None:
-        k_out = k_scale.new_empty(shape, dtype=out_dtype or torch.bfloat16)
-        v_out = torch.empty_like(k_out)
-    else:
-        if k_out is None or v_out is None:
-            raise ValueError("k_out and v_out go together")
-        for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-            if (t.shape != shape or t.get_device() != dev or not t.is_contiguous() or t.dtype is not k_out.dtype
-                    or t.dtype is not (out_dtype or t.dtype)):
-                raise ValueError(f"{name} must be contiguous {list(shape)} of out_dtype on the cache's device")
-    if shape[0] > 0:
-        st = lib().kv8_read_sm100(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                  block_table.data_ptr(), cu, int(max_seqlen), shape[0], k_out.data_ptr(),
-                                  v_out.data_ptr(), B, max_blocks, n_blocks, block_size, Hkv, D, _dtype_code(k_out),
-                                  ptr)
-        if st != OK:
-            raise B200LabError(st, "kv8_read_sm100")
-    return k_out, v_out
+    args = (k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, max_seqlen, total_tokens, out_dtype, k_out, v_out)
+    f = _native().read
+    r = f(*args) if stream is None else _on_stream(stream, k_cache, f, *args)
+    if type(r) is int:
+        raise B200LabError(r, "kv8_read_sm100")
+    return r
 
 
 def attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q=1, D=128) -> int:
     """Workspace bytes of attn_fwd_kv8 (independent of batch and lengths) on the current device."""
     return int(lib().attn_fwd_sm100_kv8_workspace(Hq, Hkv, int(max_seqlen_q), D))
-
-
-_kv8_workspace = {}  # (device, dtype, Hq, Hkv, max_seqlen_q, D) -> one 16-bit value expanded to a workspace's size
 
 
 def attn_fwd_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *, cu_seqlens_q=None,
@@ -623,51 +536,13 @@ def attn_fwd_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, *
     appended).  q [total_q,Hq,D] fp16/bf16, gate like q or None (out * sigmoid(gate)), both possibly
     strided views; cu_seqlens_q int32 [B+1] (None: one token a sequence) with max_seqlen_q the most of
     one sequence; the cache as in :func:`kv8_append`.  Returns [total_q,Hq,D]; rows that see no key are 0."""
-    (n_blocks, Hkv, block_size, D), dev = _kv8_check(k_cache, v_cache, k_scale, v_scale, block_table)
-    B, max_blocks = block_table.shape
-    total, Hq = q.shape[0], q.shape[1]
-    qp, qt, qh = _rows(q, total, Hq, D, "q", dev)
-    gp = None
-    gt = gh = 0
-    if gate is not None:
-        if gate.dtype is not q.dtype:
-            raise TypeError("gate must have q's dtype")
-        gp, gt, gh = _rows(gate, total, Hq, D, "gate", dev)
-    lens = _kv8_ints(seq_lens, B, "seq_lens", dev)
-    cu = None if cu_seqlens_q is None else _kv8_ints(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
-    code = _dtype_code(q)
-    ptr, ctx = _enter(dev, stream)
-    if ctx is not None:
-        return _entered(ctx, attn_fwd_kv8, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
-                        cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q, gate=gate, scale=scale, causal=causal,
-                        out=out, workspace=workspace)
-    if out is None:
-        out = _torch().empty_like(q) if q.is_contiguous() else q.new_empty((total, Hq, D))
-    elif out.shape != (total, Hq, D) or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != dev:
-        raise ValueError("out must be contiguous, like q, on the cache's device")
-    if total == 0 and (cu is not None or B == 0):
-        return out
-    if workspace is None:
-        # a tensor like a cached one of that many values that holds a single one: the quickest way to memory
-        key = (dev, code, Hq, Hkv, max_seqlen_q, D)
-        like = _kv8_workspace.get(key)
-        if like is None:  # at least a value, so that wrong sizes reach the library's own checks
-            n = max(1, attn_fwd_kv8_workspace_bytes(Hq, Hkv, max_seqlen_q, D) // 2)
-            like = _kv8_workspace[key] = q.new_empty(1).expand(n)
-        workspace = _torch().empty_like(like)
-        ws_bytes = 2 * like.numel()
-    else:
-        if not workspace.is_contiguous() or workspace.get_device() != dev:
-            raise ValueError("workspace must be contiguous, on the cache's device")
-        ws_bytes = workspace.numel() * workspace.element_size()
-    st = lib().attn_fwd_sm100_kv8(qp, qt, qh, gp, gt, gh, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                                  v_scale.data_ptr(), block_table.data_ptr(), lens, cu, int(max_seqlen_q), total,
-                                  out.data_ptr(), B, max_blocks, n_blocks, block_size, Hq, Hkv, D,
-                                  D ** -0.5 if scale is None else float(scale), 1 if causal else 0, code,
-                                  workspace.data_ptr(), ws_bytes, ptr)
-    if st != OK:
-        raise B200LabError(st, "attn_fwd_sm100_kv8")
-    return out
+    args = (q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, gate, scale,
+            causal, out, workspace)
+    f = _native().attend
+    r = f(*args) if stream is None else _on_stream(stream, k_cache, f, *args)
+    if type(r) is int:
+        raise B200LabError(r, "attn_fwd_sm100_kv8")
+    return r
 
 
 def launch_count() -> int:
