@@ -249,6 +249,8 @@ def test_attend_gate_and_strides(cuda, D):
     s = Setup(lens, 2, D, 64, seed=D)
     qg = _normal((3, 12, 2, D), 6, torch.bfloat16, 2.0).cuda()
     _check_attend(s, qg[:, :, 0], [1, 1, 1], gate=qg[:, :, 1])
+    odd = _normal((3, 12, D + 3), 7, torch.bfloat16, 2.0).cuda()[:, :, 3:]  # a gate on no boundary
+    _check_attend(s, qg[:, :, 0], [1, 1, 1], gate=odd)
 
 
 def test_attend_one_sequence_cut_over_all_ctas(cuda):

@@ -73,6 +73,7 @@ struct Args {
     const void* g;  // gate or null
     void* o;
     long long q_st, q_sh, g_st, g_sh;  // strides of a token and of a head
+    int g_aligned;  // the gate's rows lie on 16 bytes
     const uint8_t* k;
     const uint8_t* v;
     const int* table;
@@ -214,11 +215,21 @@ __device__ __forceinline__ void row_place(int row, int group, int& i, int& hg) {
 
 // kPer consecutive channels of a row: the gate's, and the gated outputs' store.
 template <typename T, int kPer> struct Channels {
-    T v[kPer];
+    alignas(sizeof(T) * kPer) T v[kPer];
     __device__ __forceinline__ void load_gate(const Args& a, size_t token, int head, int d0) {
         const T* g = static_cast<const T*>(a.g) + token * a.g_st + (size_t)head * a.g_sh + d0;
+        if (a.g_aligned) {  // d0 is a multiple of kPer
+            if constexpr (kPer == 8) {
+                *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(g);
+            } else if constexpr (kPer == 4) {
+                *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(g);
+            } else {
+                *reinterpret_cast<uint32_t*>(v) = *reinterpret_cast<const uint32_t*>(g);
+            }
+        } else {
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) v[u] = g[u];
+            for (int u = 0; u < kPer; ++u) v[u] = g[u];
+        }
     }
 };
 template <typename T, int kPer>
@@ -891,22 +902,49 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
     if (!has_tail && tid == 0) a.meta[4 * blockIdx.x] = -1;
 }
 
-// Joins the segments that were cut.  Block (c, y): rows y * kPerBlock .. of the segment whose first
-// part CTA c left; its other parts are the first ones of the CTAs c + 1 .. last.  8 / kPerBlock warps
-// share the parts of a row, each with a maximum of its own, so that all loads of a warp are under way
-// at once behind the one of the segment's description.
+// Joins the segments that were cut: part 0 of each is its owner's second one, the others are the first
+// ones of the CTAs that follow, up to `last`.  Two forms, by how many segments there are:
+//   many (kFew false): block (c, y), rows 8 y .. of the segment that CTA c owns, if it owns one; a warp a
+//     row, as there are few parts (B4 x 8k, 4 tokens, eleven parts: 24.5 us so, 27.3 the other way).
+//   few: block (i, n), row n of the i-th segment that was cut, which the block looks up among the owners;
+//     sixteen warps share the parts, of which there can be as many as CTAs.  (A block for every CTA and row
+//     is a thousand blocks more to start: B1 x 64k, 16 heads on 1, 21.8 us with them, 17 without.)
+// Either way a warp has all its loads under way at once behind the one of the segment's description.
 constexpr int kJoinAhead = 4;  // parts a warp loads at a time
-template <int D, int NT, typename T, int kPerBlock>
-__global__ void __launch_bounds__(256) attn_kv8_join_kernel(const Args a, int grid) {
+template <int D, int NT, typename T, bool kFew>
+__global__ void __launch_bounds__(kFew ? 512 : 256) attn_kv8_join_kernel(const Args a, int grid) {
     constexpr int kRows = 8 * NT, kVec = D / 32;  // channels of a lane
-    constexpr int kSharers = 8 / kPerBlock;
+    constexpr int kSharers = kFew ? 16 : 1, kPerBlock = kFew ? 1 : 8;
     grid_dependency_wait();
     allow_dependent_launch();
-    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int c = blockIdx.x;
+    if constexpr (kFew) {
+        __shared__ int owners[16], found;
+        int before = 0, wanted = blockIdx.x;
+        if (threadIdx.x == 0) found = -1;
+        for (int i0 = 0; i0 < grid; i0 += 512) {
+            const int i = i0 + threadIdx.x;
+            const unsigned own = __ballot_sync(0xffffffffu, i < grid && a.meta[4 * i] >= 0);
+            __syncthreads();  // the last chunk's owners are read
+            if (lane == 0) owners[warp] = __popc(own);
+            __syncthreads();
+            int mine = before;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+                if (w < warp) mine += owners[w];
+                before += owners[w];
+            }
+            if ((own >> lane & 1) && mine + __popc(own & ((1u << lane) - 1)) == wanted) found = i;
+        }
+        __syncthreads();
+        c = found;
+        if (c < 0) return;
+    }
     const int4 desc = reinterpret_cast<const int4*>(a.meta)[c];
     const int last = desc.x, row0 = desc.w & 0xffffff, rows = desc.w >> 24;
     if (last < 0) return;
-    const int n = blockIdx.y * kPerBlock + warp / kSharers;
+    const int n = blockIdx.y * kPerBlock + (kFew ? 0 : warp);
     const int parts = n < rows ? last - c + 1 : 0;
     int i, hg;
     row_place(row0 + n, a.group, i, hg);
@@ -953,8 +991,8 @@ __global__ void __launch_bounds__(256) attn_kv8_join_kernel(const Args a, int gr
         M = to;
     }
     if constexpr (kSharers > 1) {
-        __shared__ float acc[8][D];
-        __shared__ float2 stat[8];
+        __shared__ float acc[kSharers][D];
+        __shared__ float2 stat[kSharers];
         if (lane == 0) stat[warp] = make_float2(M, sum);
 #pragma unroll
         for (int u = 0; u < kVec; ++u) acc[warp][lane * kVec + u] = x[u];
@@ -1027,12 +1065,10 @@ int launch(Args a, void* ws, int grid, int device, cudaStream_t st) {
     if (rc != B200LAB_OK) return rc;
     const long long used = (long long)a.group * a.max_seqlen_q;
     const int rows_used = (int)(used < 8 * NT ? used : 8 * NT);
-    // Rows a block joins: eight, a warp each, where a segment is cut into few parts (segments are
-    // many); one, its parts shared by eight warps, where they are few.
-    const long long segments = (long long)a.B * a.Hkv;
-    if (segments * 4 >= grid)
-        return kv8_launch(attn_kv8_join_kernel<D, NT, T, 8>, dim3(grid, (rows_used + 7) / 8), 256, 0, st, a, grid);
-    return kv8_launch(attn_kv8_join_kernel<D, NT, T, 1>, dim3(grid, rows_used), 256, 0, st, a, grid);
+    const long long segments = (long long)a.B * a.Hkv * ((used + 8 * NT - 1) / (8 * NT));
+    if (segments * 16 >= grid)
+        return kv8_launch(attn_kv8_join_kernel<D, NT, T, false>, dim3(grid, (rows_used + 7) / 8), 256, 0, st, a, grid);
+    return kv8_launch(attn_kv8_join_kernel<D, NT, T, true>, dim3((unsigned)segments, rows_used), 512, 0, st, a, grid);
 }
 
 template <int D, int NT, typename T>
@@ -1097,6 +1133,7 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     Args a;
     a.q = Q, a.g = G, a.o = O;
     a.q_st = q_stride_token, a.q_sh = q_stride_head, a.g_st = g_stride_token, a.g_sh = g_stride_head;
+    a.g_aligned = aligned16(G) && g_stride_token % 8 == 0 && g_stride_head % 8 == 0;
     a.k = static_cast<const uint8_t*>(k_cache), a.v = static_cast<const uint8_t*>(v_cache);
     a.table = block_table, a.lens = seq_lens, a.cu = cu_seqlens_q;
     a.k_scale = k_scale, a.v_scale = v_scale;
