@@ -12,10 +12,11 @@
 //
 // What bounds it: the bytes of the cache; a code is used by the few rows of its kv group only
 // (2 x rows flop a byte).  Everything follows from streaming them:
-//   * The batch's work is cut into equal runs of 64-key tiles, one run a CTA, whatever the lengths
-//     are (the tiles of all (sequence, kv-head, row tile) segments are numbered through on the
-//     device).  A segment that lies in one run is written out by its CTA; one that is cut leaves
-//     fp32 partial sums in the workspace, two at most a CTA, and a second kernel joins them.
+//   * The batch's work is cut into equal runs of key tiles, one run a CTA, whatever the lengths are
+//     (the tiles of all (sequence, kv-head, row tile) segments are numbered through on the device, and
+//     a segment counts two tiles more than it has, for its start and end: ragged B64 108 us without,
+//     99 with).  A segment that lies in one run is written out by its CTA; one that is cut leaves fp32
+//     partial sums in the workspace, two at most a CTA, and a second kernel joins them.
 //   * A warp has a ring of its own of 16- or 32-key pieces of K and V, which its lanes fill with
 //     16-byte asynchronous copies, whose next pieces are requested across segment borders, so that
 //     the loads never pause.  Nothing but the joins holds the warps of a CTA together.  (TMA boxes
@@ -28,8 +29,15 @@
 //   * The channel and key order inside a product is free: each thread takes 32 consecutive channels
 //     of a K row (two 16-byte shared loads, conflict-free as the chunks are swizzled) and 16 of four V
 //     rows, whose bytes it pairs by key with one PRMT for two conversions.
+//   * No lane asks the others for a row's maximum until a score lies 2^8 above the one in use.
 //   * Q is brought to fp16 with a power of two a row: exact, as bf16 and fp16 both have at most 11
 //     significant bits (below 2^-29 of the row's largest value, bits are lost).
+// Measured, 32 q-heads on 8 kv-heads of 128 unless said, calls back to back in a graph: B64 x 16k 345 us
+// (6.2 TB/s, 97 % of the measured copy rate), B64 x 400..8k 100 us (88 %), B1 x 16k 14.7 us, B1 x 1000
+// 9.1 us, 4 tokens x B16 x 2-4k 32 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 45 us, 8 heads of 64
+// B48 x 250..2500 23 us.  The longest streams are bound by memory; what the shorter ones add to that is
+// a call's own chain (lengths, block ids, codes; the part's join; the second kernel: 7 us in all) and,
+// with more rows or 64 channels, the instructions of converting (0.5 issued a cycle and scheduler).
 #include "errwords.h"
 #include "kv8.cuh"
 
@@ -43,7 +51,10 @@ constexpr int kGroup = 16;                // keys of one product
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;              // the running maximum is moved when x exceeds it by 2^8
 
-// What a variant's CTA works on and holds; `ctas` of them fill an SM's registers and shared memory.
+// What a variant's CTA works on and holds; `ctas` (of four warps) fill an SM's registers and shared
+// memory.  Two groups a piece halve what a piece costs beside its products where registers allow it
+// (one column tile of D 128: B64 x 16k 424 us with one group and two CTAs, 348 with two and three; two
+// column tiles: 41 us with one and three CTAs, 35 with two and two; D 256: 46 us with one, 59 with two).
 struct Shape {
     int groups;  // of a piece, the keys a warp takes at a time
     int ctas;
@@ -87,7 +98,7 @@ struct Args {
     float scale;
 };
 
-// ---- the plan: sequences -> segments -> 64-key tiles ------------------------------------------
+// ---- the plan: sequences -> segments -> key tiles ----------------------------------------------
 struct Seq {
     int n, L, t0;      // query tokens, keys, first packed token
     int tiles, rts;    // key tiles and row tiles
@@ -1035,9 +1046,9 @@ int plan_grid(int D, int nt, int warps, int sms) {
 // leaves few cut segments; a warp on its own joins nothing, and while it starts or ends a segment the
 // SM's other warps go on: better where segments are short and many.  The lengths are on the device, so
 // the rule goes by what the host has, the segments and the most that the block table can hold (measured
-// with four / with one, 32 q-heads on 8 kv-heads of 128 unless said: B64 x 200 tokens 15.0 / 14.0 us,
-// B128 x 200 25.3 / 21.5, B256 x 200 42.8 / 29.8, B512 x 64 58 / 35, B128 x 2k D 64 32 heads 149 / 137,
-// B256 x 1k 81 / 82, and the other way B256 x 200..4k 188 / 198, B32 x 200 11.3 / 16.8).
+// with four / with one, 32 q-heads on 8 kv-heads of 128 unless said: B64 x 200 tokens 14.8 / 14.0 us,
+// B128 x 200 24.9 / 21.6, B256 x 200 40.9 / 29.1, B512 x 64 52 / 31, B128 x 2k D 64 32 heads 148 / 136,
+// B256 x 1k 79 / 81, and the other way B256 x 200..4k 188 / 197, B32 x 200 11.0 / 16.6).
 int warps_of(long long segments, long long tokens, int D, int nt, int sms) {
     const long long alone = plan_grid(D, nt, 1, sms);
     return segments >= (tokens <= 512 ? alone / 2 : alone) ? 1 : 4;
