@@ -435,6 +435,34 @@ def test_captured_graphs_and_streams(cuda):
     assert torch.equal(a.k.view(torch.uint8), b.k.view(torch.uint8)) and torch.equal(a.vs, b.vs)
 
 
+def test_capture_with_joined_streams(cuda):
+    """The calls behind an event of another captured stream, as the last of two branches."""
+    s, u = Setup([50, 7], 2, 64, 16, seed=5), Setup([50, 7], 2, 64, 16, seed=5)
+    x, y, q = (_normal((2, h, 64), i, torch.bfloat16).cuda() for i, h in enumerate((2, 2, 4)))
+    b200lab.kv8_append(x, y + 1, *u.cache, u.l)
+    want = b200lab.attn_fwd_kv8(q, *u.cache, u.l)
+    z, other = torch.empty_like(y), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        other.wait_stream(main)
+        with torch.cuda.stream(other):
+            torch.add(y, 1, out=z)
+        w = x * 1
+        main.wait_stream(other)
+        b200lab.kv8_append(w, z, *s.cache, s.l)
+        other.wait_stream(main)
+        with torch.cuda.stream(other):
+            o = b200lab.attn_fwd_kv8(q, *s.cache, s.l)
+        main.wait_stream(other)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert b200lab.device_status() == b200lab.OK
+    assert torch.equal(o, want) and torch.equal(s.v.view(torch.uint8), u.v.view(torch.uint8))
+
+
 def test_same_call_twice_gives_the_same_bits(cuda):
     s = Setup([3000, 17, 911, 64], 4, 128, 64, seed=2)
     q = _normal((4, 16, 128), 4, torch.bfloat16).cuda()
@@ -459,6 +487,18 @@ def test_many_sequences(cuda):
     lens = [(i * 37) % 90 if i % 3 else 0 for i in range(700)]
     s = Setup(lens, 1, 64, 16, seed=7, garbage=True)
     _check_attend(s, _normal((700, 2, 64), 4, torch.bfloat16).cuda(), [1] * 700)
+
+
+@pytest.mark.parametrize("D,Hkv,group,B,new", [(128, 8, 2, 230, 1), (64, 8, 1, 300, 1), (256, 8, 1, 150, 1),
+                                               (128, 4, 4, 300, 3), (64, 8, 5, 225, 2)])
+def test_many_segments(cuda, D, Hkv, group, B, new):
+    """So many (sequence, kv-head) pairs that each warp takes segments of its own; a long sequence
+    among them, which many warps share, and padding."""
+    lens = [3000] + [(i * 29) % 71 if i % 5 else 0 for i in range(1, B)]
+    counts = [new] + [(i * 7) % (new + 1) if new > 1 else 1 for i in range(1, B)]
+    s = Setup(lens, Hkv, D, 16, seed=D + B, garbage=True)
+    q = _normal((sum(counts), Hkv * group, D), 5, torch.bfloat16).cuda()
+    _check_attend(s, q, counts)
 
 
 def test_empty_batch_and_binding_refusals(cuda):

@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                     gk[u] = m.ks;
                     gl[u] = (float)((int)(bits >> 23) - 127);
                     gi[u] = __uint_as_float((254u << 23) - bits);
-                        if (__builtin_expect(bits & 0x7fffffu, 0)) gl[u] = log2f(v), gi[u] = 1.f / v;
+                    if (__builtin_expect(bits & 0x7fffffu, 0)) gl[u] = log2f(v), gi[u] = 1.f / v;
                     ok[u] = m.ok;
                     whole_piece = whole_piece && m.ok;
                 }

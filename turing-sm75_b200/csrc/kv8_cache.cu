@@ -418,7 +418,7 @@ extern "C" int kv8_read_sm100(const void* k_cache, const void* v_cache, const fl
     const long long blocks = ((long long)most + block_size - 1) / block_size;
     a.blocks_per_seq = (int)(blocks < max_blocks ? blocks : max_blocks);
     const long long run = ((long long)Hkv * block_size * D) >> (out_dtype == B200LAB_F32 ? 2 : 3);  // vectors
-    if (run > 0x10000000LL) return B200LAB_ERR_UNSUPPORTED;
+    if (run > 0x8000000LL) return B200LAB_ERR_UNSUPPORTED;  // a code's place in the run fits 31 bits
     const long long per_cta = (long long)kReadThreads * kReadVecs;
     a.chunks = (int)((run + per_cta - 1) / per_cta);
     const long long grid = 2LL * B * a.blocks_per_seq * a.chunks;
