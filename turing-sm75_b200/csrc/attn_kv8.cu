@@ -74,9 +74,10 @@ template <int D, int NT, int W> struct Cfg {  // W: warps of a CTA
     static constexpr int kStart = 2;                        // what a segment's start and end cost, in tiles
 };
 
-struct GroupMeta {  // of 16 keys
+struct alignas(16) GroupMeta {  // of 16 keys
     float ks, vs;   // scales of K and V
     int ok;         // 0: no key of the group is in the sequence, or its block id lies outside the pool
+    int unused;
 };
 
 struct Args {
@@ -95,6 +96,7 @@ struct Args {
     float* part;    // [grid][2][rows][D] sums, [grid][2][rows] (m, l)
     int* meta;      // [grid][4]
     int max_seqlen_q, total_q, B, max_blocks, n_blocks, log2P, Hq, Hkv, group, causal;
+    uint32_t head_bytes;  // of a block's codes of one head: block_size * D
     float scale;
 };
 
@@ -345,6 +347,7 @@ template <int D, int NT, int W> struct Producer {
     Cursor<D, NT, W> c;
     int k;        // next tile of the segment, from c.first()
     int block;    // lane i: block * Hkv + head of group i of the next 32 / kH pieces; -1: none
+    uint32_t to;  // where this lane's first 16 bytes of a group go in a piece
 
     // Requests the next piece, if one is left, into a ring slot, as one group of copies.
     __device__ __forceinline__ void issue(const Args& a, uint8_t* slot, GroupMeta* meta, int warp, int lane) {
@@ -377,20 +380,22 @@ template <int D, int NT, int W> struct Producer {
                     copy4(&m->vs, a.v_scale + block);
                 }
             }
+            const uint32_t dst = smem_u32(slot);
 #pragma unroll
             for (int u = 0; u < C::kH; ++u) {
                 const int bh = __shfl_sync(0xffffffffu, block, first + u);
                 if (bh < 0) continue;
                 const int row = ((c.first() + k) * C::kTile + warp * C::kPiece + u * kGroup) & ((1 << a.log2P) - 1);
-                const size_t at = (((size_t)(uint32_t)bh << a.log2P) + row) * D + lane * 16;
-                const uint32_t dst = smem_u32(slot);
+                const size_t at = (size_t)(uint32_t)bh * a.head_bytes + (uint32_t)(row * D + lane * 16);
+                const uint8_t *from_k = a.k + at, *from_v = a.v + at;
 #pragma unroll
-                for (int i = 0; i < kGroup * D / 512; ++i) {  // 512 contiguous bytes a copy of the warp
-                    constexpr int kBox = D > 128 ? 128 : D, kRowLanes = D / 16;
-                    const int r = i * (512 / D) + lane / kRowLanes, chunk = lane % kRowLanes;
-                    const int off = (chunk / (kBox / 16)) * (C::kPiece * kBox) + u * kGroup * kBox + chunk_at<D>(r, chunk % (kBox / 16));
-                    copy16(dst + off, a.k + at + i * 512);
-                    copy16(dst + C::kPiece * D + off, a.v + at + i * 512);
+                for (int i = 0; i < kGroup * D / 512; ++i) {  // 512 contiguous bytes a copy of the warp: 512 / D rows
+                    constexpr int kBox = D > 128 ? 128 : D, kStep = 512 / D;
+                    // rows i * kStep further: the same place in a row, chunk index XOR what the row adds to it
+                    constexpr uint32_t kTurn = D == 64 ? 0u : (uint32_t)(kStep & 7) << 4;
+                    const uint32_t off = (to ^ ((i * kTurn) & 0x70u)) + (uint32_t)((u * kGroup + i * kStep) * kBox);
+                    copy16(dst + off, from_k + i * 512);
+                    copy16(dst + C::kPiece * D + off, from_v + i * 512);
                 }
             }
             ++k;
@@ -532,6 +537,17 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
     Producer<D, NT, W> pro;
     pro.c = cur;
     pro.k = 0;
+    {
+        constexpr int kRowLanes = D / 16, kBoxLanes = kBox / 16;
+        const int chunk = lane % kRowLanes;
+        pro.to = (chunk / kBoxLanes) * (kPiece * kBox) + chunk_at<D>(lane / kRowLanes, chunk % kBoxLanes);
+    }
+    // where this thread's codes lie in a group: chunks of K's rows key(g) (key(g) + 8: 8 rows further), of
+    // V's rows key(2t) and key(2t + 1)
+    const int kr = key_of<D>(g);
+    const int k_at = chunk_at<D>(kr, D == 64 ? t : 2 * t);
+    const int v_at[2] = {D == 64 ? chunk_at<D>(key_of<D>(2 * t), g >> 1) + (g & 1) * 8 : chunk_at<D>(2 * t, g),
+                         D == 64 ? chunk_at<D>(key_of<D>(2 * t + 1), g >> 1) + (g & 1) * 8 : chunk_at<D>(2 * t + 1, g)};
     int slot = 0;  // the next piece's
     for (int i = 0; i < kDepth; ++i) pro.issue(a, sm.ring[warp][i], sm.meta[warp][i], warp, lane);
 
@@ -628,18 +644,17 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                             sc[u][nt][0][i] = 0.f;
                             sc[u][nt][kAcc - 1][i] = 0.f;
                         }
-                const int kr = key_of<D>(g);
 #pragma unroll
                 for (int box = 0; box < kBoxes; ++box) {
                     constexpr int kChunks = D == 64 ? 1 : 2;
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c) {
-                        const int chunk = kChunks * t + c;
 #pragma unroll
                         for (int u = 0; u < kH; ++u) {
                             const uint8_t* kb = ks_ + (box * kPiece + u * kGroup) * kBox;
-                            const uint4 lo = *reinterpret_cast<const uint4*>(kb + chunk_at<D>(kr, chunk));
-                            const uint4 hi = *reinterpret_cast<const uint4*>(kb + chunk_at<D>(kr + 8, chunk));
+                            // the other chunk of the pair is the swizzled index with its last bit turned
+                            const uint4 lo = *reinterpret_cast<const uint4*>(kb + (k_at ^ (c * 16)));
+                            const uint4 hi = *reinterpret_cast<const uint4*>(kb + (k_at ^ (c * 16)) + 8 * kBox);
                             const uint32_t w0[4] = {lo.x, lo.y, lo.z, lo.w}, w1[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
@@ -743,12 +758,13 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                     for (int box = 0; box < kBoxes; ++box)
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            const uint8_t* vb = vs_ + (box * kPiece + u * kGroup) * kBox;
+                            // rows key(2t), key(2t + 1), and those 8 further, which are swizzled alike
+                            const uint8_t* vb = vs_ + (box * kPiece + u * kGroup + (q >> 1) * 8) * kBox + v_at[q & 1];
                             if constexpr (D == 64) {
-                                const uint2 x = *reinterpret_cast<const uint2*>(vb + chunk_at<D>(r[q], g >> 1) + (g & 1) * 8);
+                                const uint2 x = *reinterpret_cast<const uint2*>(vb);
                                 w[box][q][0] = x.x, w[box][q][1] = x.y;
                             } else {
-                                const uint4 x = *reinterpret_cast<const uint4*>(vb + chunk_at<D>(r[q], g));
+                                const uint4 x = *reinterpret_cast<const uint4*>(vb);
                                 w[box][q][0] = x.x, w[box][q][1] = x.y, w[box][q][2] = x.z, w[box][q][3] = x.w;
                             }
                         }
@@ -1151,6 +1167,7 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     a.max_seqlen_q = most, a.total_q = total_q, a.B = B, a.max_blocks = max_blocks, a.n_blocks = n_blocks;
     a.log2P = kv8_log2_block(block_size), a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv, a.causal = causal;
     a.scale = scale;
+    a.head_bytes = (uint32_t)(block_size * D);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, warps, a, workspace, grid, dev.ordinal, st)
                                 : launch_d<__nv_bfloat16>(D, nt, warps, a, workspace, grid, dev.ordinal, st);
