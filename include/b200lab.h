@@ -355,8 +355,9 @@ int kv8_read_sm100(const void* k_cache, const void* v_cache, const float* k_scal
  *       behind the last sequence are left as they were.
  * GQA as attn_fwd_sm100.  Any number of query tokens is right, but the kernel is
  * made for few: it reads the cache once for every 8 or 16 rows of a kv group,
- * so the queries of a long prompt are faster through kv8_read_sm100 and
- * attn_fwd_sm100_varlen.  Calls that may overlap need
+ * so from about 64 new tokens a sequence on they are faster through
+ * kv8_read_sm100 and attn_fwd_sm100_varlen (8 sequences of 4096 keys, 32 q-heads on
+ * 8 of 128: 64 tokens 139 us against 147, 256 tokens 478 against 167).  Calls that may overlap need
  * workspaces of their own. */
 int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long long q_stride_head,
                        const void* G, long long g_stride_token, long long g_stride_head,

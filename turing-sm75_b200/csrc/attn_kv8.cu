@@ -33,9 +33,9 @@
 //   * Q is brought to fp16 with a power of two a row: exact, as bf16 and fp16 both have at most 11
 //     significant bits (below 2^-29 of the row's largest value, bits are lost).
 // Measured, 32 q-heads on 8 kv-heads of 128 unless said, calls back to back in a graph: B64 x 16k 345 us
-// (6.2 TB/s, 97 % of the measured copy rate), B64 x 400..8k 100 us (88 %), B1 x 16k 14.7 us, B1 x 1000
-// 9.1 us, 4 tokens x B16 x 2-4k 32 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 45 us, 8 heads of 64
-// B48 x 250..2500 23 us.  The longest streams are bound by memory; what the shorter ones add to that is
+// (6.2 TB/s, 97 % of the measured copy rate), B64 x 400..8k 99 us (89 %), B1 x 16k 14.5 us, B1 x 1000
+// 9.0 us, 4 tokens x B16 x 2-4k 31 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 45 us, 8 heads of 64
+// B48 x 250..2500 22 us.  The longest streams are bound by memory; what the shorter ones add to that is
 // a call's own chain (lengths, block ids, codes; the part's join; the second kernel: 7 us in all) and,
 // with more rows or 64 channels, the instructions of converting (0.5 issued a cycle and scheduler).
 #include "errwords.h"
@@ -742,8 +742,8 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                         const float p2 = ex2(sc[u][nt][0][2] - m0), p3 = ex2(sc[u][nt][0][3] - m1);
                         l[nt][0] = fmaf(p0 + p2, gi[u], l[nt][0]);
                         l[nt][1] = fmaf(p1 + p3, gi[u], l[nt][1]);
-                        // the weights are rounded to fp16 (2^-11 relative; the sum l is not, its rounding
-                        // errors would not cancel theirs)
+                        // the weights are rounded to fp16 (2^-11 relative); the sum l takes them before: a
+                        // weight that is small because its block's scale is counts in l all the same
                         pb[u][nt][0] = transpose8x8(pack_h2(p0, p1));
                         pb[u][nt][1] = transpose8x8(pack_h2(p2, p3));
                     }
