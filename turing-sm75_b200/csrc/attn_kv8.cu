@@ -14,7 +14,7 @@
 // (2 x rows flop a byte).  Everything follows from streaming them:
 //   * The batch's work is cut into equal runs of key tiles, one run a CTA, whatever the lengths are
 //     (the tiles of all (sequence, kv-head, row tile) segments are numbered through on the device, and
-//     a segment counts two tiles more than it has, for its start and end: ragged B64 108 us without,
+//     a segment counts two or three tiles more than it has, for its start and end: ragged B64 108 us without,
 //     99 with).  A segment that lies in one run is written out by its CTA; one that is cut leaves fp32
 //     partial sums in the workspace, two at most a CTA, and a second kernel joins them.
 //   * A warp has a ring of its own of 16- or 32-key pieces of K and V, which its lanes fill with
@@ -34,7 +34,7 @@
 //     significant bits (below 2^-29 of the row's largest value, bits are lost).
 // Measured, 32 q-heads on 8 kv-heads of 128 unless said, calls back to back in a graph: B64 x 16k 345 us
 // (6.2 TB/s, 97 % of the measured copy rate), B64 x 400..8k 99 us (89 %), B1 x 16k 14.5 us, B1 x 1000
-// 9.0 us, 4 tokens x B16 x 2-4k 31 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 45 us, 8 heads of 64
+// 9.0 us, 4 tokens x B16 x 2-4k 31 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 43 us, 8 heads of 64
 // B48 x 250..2500 22 us.  The longest streams are bound by memory; what the shorter ones add to that is
 // a call's own chain (lengths, block ids, codes; the part's join; the second kernel: 7 us in all) and,
 // with more rows or 64 channels, the instructions of converting (0.5 issued a cycle and scheduler).
@@ -61,7 +61,7 @@ struct Shape {
     int depth;   // pieces of a warp's ring
 };
 constexpr Shape shape_of(int D, int nt) {
-    return D == 64 ? (nt == 1 ? Shape{2, 4, 2} : Shape{2, 3, 3}) : D == 128 ? (nt == 1 ? Shape{2, 3, 2} : Shape{2, 2, 2}) : Shape{1, 2, 3};
+    return D == 64 ? (nt == 1 ? Shape{2, 4, 2} : Shape{2, 3, 3}) : D == 128 ? (nt == 1 ? Shape{2, 3, 2} : Shape{2, 2, 2}) : Shape{1, 2, 2};
 }
 template <int D, int NT, int W> struct Cfg {  // W: warps of a CTA
     static constexpr int kH = shape_of(D, NT).groups;
@@ -70,8 +70,11 @@ template <int D, int NT, int W> struct Cfg {  // W: warps of a CTA
     static constexpr int kBytes = 2 * kPiece * D;           // a piece of K, then one of V
     static constexpr int kCtas = shape_of(D, NT).ctas * kMostWarps / W;
     static constexpr int kDepth = shape_of(D, NT).depth;
-    static constexpr int kRow = 64;                         // channels joined at a time
-    static constexpr int kStart = 2;                        // what a segment's start and end cost, in tiles
+    // channels joined at a time: as many as leave room for the CTAs (D 256: 42.8 us with 128, 43.0 with 64)
+    static constexpr int kRow = D == 256 || (D == 128 && NT == 2) ? 128 : 64;
+    // what a segment's start and end cost, in tiles (a tile of D 256 has a group a warp, and its sums are
+    // the longest to join: 45.4 us with 2 and a ring of three, 43.0 with 3 and a ring of two)
+    static constexpr int kStart = D == 256 ? 3 : 2;
 };
 
 struct alignas(16) GroupMeta {  // of 16 keys
