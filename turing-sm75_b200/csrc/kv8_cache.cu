@@ -99,7 +99,10 @@ struct AppendArgs {
     Divisor by_head, by_local;
 };
 
-constexpr int kAppendVecs = 8;  // vectors of 8 values a thread holds
+constexpr int kAppendVecs = 8;  // vectors of 8 values a thread holds: 32 registers of 16-bit values, 64 of fp32
+constexpr int append_cta(int threads) { return threads < 128 ? 128 : threads; }
+// CTAs an SM: 1024 threads of 64 registers, or 512 of 128
+template <typename T> constexpr int append_resident(int threads) { return (sizeof(T) == 2 ? 1024 : 512) / append_cta(threads); }
 
 // What one item of the writer is: `count` new tokens from x on, into the slots from `before` on of one
 // head of a block, of K or V.
@@ -150,7 +153,7 @@ __device__ __forceinline__ AppendItem append_item(const AppendArgs& a, long long
 // 8 sequences, D 128, 35 us so, 27 us now, 88 % of the bytes' time), and items with nothing to write
 // cost no more than that.
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads, kThreads <= 128 && sizeof(T) == 2 ? 8 : 1)
+__global__ void __launch_bounds__(append_cta(kThreads), append_resident<T>(kThreads))
     kv8_append_kernel(const AppendArgs a) {
     constexpr int kItems = kThreads < 128 ? 128 / kThreads : 1;  // of a CTA at a time
     __shared__ float part[2][kThreads / 32];
@@ -323,10 +326,9 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const ReadArgs a
 }
 
 template <typename T, int kThreads> int launch_append_as(const AppendArgs& a, int sms, cudaStream_t st) {
-    constexpr int kCta = kThreads < 128 ? 128 : kThreads, kItems = kCta / kThreads;
+    constexpr int kCta = append_cta(kThreads), kItems = kCta / kThreads;
     // as many CTAs as are resident, each with about the same number of items
-    constexpr int kResident = kThreads <= 128 && sizeof(T) == 2 ? 8 : 512 / kCta;
-    const long long ctas = (a.items + kItems - 1) / kItems, most = (long long)sms * kResident;
+    const long long ctas = (a.items + kItems - 1) / kItems, most = (long long)sms * append_resident<T>(kThreads);
     return kv8_launch(kv8_append_kernel<T, kThreads>, dim3((unsigned)(ctas < most ? ctas : most)), kCta, 0, st, a);
 }
 
