@@ -600,3 +600,54 @@ print("fine")
 """ % [p for p in sys.path if p]
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=dict(os.environ))
     assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+# ---- both ways of the attention --------------------------------------------------------------------------------------
+class Wide(Setup):
+    """The same with a block table for 9000 tokens: the attention then goes by its plan, where a table that is
+    no wider than the lengths mostly gives a cluster of CTAs a segment."""
+
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        spare = torch.full((len(self.lens), 9000 // self.P), self.n_blocks + 7, dtype=torch.int32, device="cuda")
+        self.t = torch.cat([self.t, spare], 1).contiguous()
+
+
+@pytest.mark.parametrize("test,kw", [
+    *((test_attend_step, dict(D=D, group=g, P=16, dtype=torch.bfloat16)) for D in (64, 128, 256) for g in (1, 8, 20)),
+    *((test_attend_several_tokens, dict(D=D, group=g, P=P, causal=c))
+      for D, g in ((128, 4), (64, 1), (256, 6), (64, 5)) for P in (16, 128) for c in (True, False)),
+    *((test_attend_gate_and_strides, dict(D=D)) for D in (64, 128, 256)),
+    *((test_attend_long_queries, dict(D=D)) for D in (64, 128, 256)),
+    (test_attend_scales_far_apart, {}), (test_attend_sharp_scores, {}), (test_attend_nan, {}),
+], ids=lambda x: x.__name__[5:] if callable(x) else "-".join(str(v) for v in x.values()))
+def test_by_the_plan(cuda, monkeypatch, test, kw):
+    monkeypatch.setitem(globals(), "Setup", Wide)
+    test(cuda, **kw)
+
+
+@pytest.mark.parametrize("D,group", [(64, 4), (64, 12), (128, 8), (128, 9), (256, 6), (256, 11)])
+@pytest.mark.parametrize("B,longest", [(2, 900), (7, 500), (20, 260), (48, 130), (70, 40)])
+def test_clusters_of_every_size(cuda, D, group, B, longest):
+    """From one CTA a segment to eight, of which some have no keys; padding, several tokens, a gate, NaN wherever
+    no token lies."""
+    lens = [longest] + [(i * 53) % longest if i % 4 else 0 for i in range(1, B)]
+    new = [(i * 5) % 4 for i in range(B)]
+    s = Setup(lens, 2, D, 32, seed=D + B, garbage=True)
+    q = _normal((sum(new) + 1, 2 * group, D), 6, torch.bfloat16).cuda()
+    gate = _normal(tuple(q.shape), 7, torch.bfloat16, 2.0).cuda()
+    out = torch.full_like(q, 55.0)
+    _check_attend(s, q, new, gate=gate, out=out)
+    assert bool((out[sum(new):] == 55.0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_both_ways_agree(cuda, dtype):
+    """A call by clusters and one by the plan on the same cache: each within its bound, so both together
+    within twice that; and a call by clusters gives the same bits every time."""
+    narrow, wide = (C([1000, 333, 64, 1], 4, 128, 32, seed=5) for C in (Setup, Wide))
+    q = _normal((4, 16, 128), 8, dtype).cuda()
+    a = _check_attend(narrow, q, [1] * 4)
+    _check_attend(wide, q, [1] * 4)
+    for _ in range(3):
+        assert torch.equal(a, b200lab.attn_fwd_kv8(q, *narrow.cache, narrow.l))

@@ -17,6 +17,8 @@
 //     a segment counts two or three tiles more than it has, for its start and end: ragged B64 108 us without,
 //     99 with).  A segment that lies in one run is written out by its CTA; one that is cut leaves fp32
 //     partial sums in the workspace, two at most a CTA, and a second kernel joins them.
+//   * Where there are few short segments, the chain of plan, parts and second kernel is most of a call: there
+//     a cluster of CTAs has a segment, and joins its sums through distributed shared memory.
 //   * A warp has a ring of its own of 16- or 32-key pieces of K and V, which its lanes fill with
 //     16-byte asynchronous copies, whose next pieces are requested across segment borders, so that
 //     the loads never pause.  Nothing but the joins holds the warps of a CTA together.  (TMA boxes
@@ -34,9 +36,9 @@
 //     significant bits (below 2^-29 of the row's largest value, bits are lost).
 // Measured, 32 q-heads on 8 kv-heads of 128 unless said, calls back to back in a graph: B64 x 16k 345 us
 // (6.2 TB/s, 97 % of the measured copy rate), B64 x 400..8k 99 us (89 %), B1 x 16k 14.5 us, B1 x 1000
-// 9.0 us, 4 tokens x B16 x 2-4k 31 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 43 us, 8 heads of 64
+// 6.4 us, 4 tokens x B16 x 2-4k 31 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 43 us, 8 heads of 64
 // B48 x 250..2500 22 us.  The longest streams are bound by memory; what the shorter ones add to that is
-// a call's own chain (lengths, block ids, codes; the part's join; the second kernel: 7 us in all) and,
+// a call's own chain (lengths, block ids, codes; the part's join; the second kernel: 7 us in all, 4 with clusters) and,
 // with more rows or 64 channels, the instructions of converting (0.5 issued a cycle and scheduler).
 #include "errwords.h"
 #include "kv8.cuh"
@@ -47,6 +49,7 @@ namespace {
 __device__ int g_err_attn_kv8 = 0;
 
 constexpr int kMostWarps = 4;             // of a CTA
+constexpr int kMostCluster = 8;           // CTAs of a cluster
 constexpr int kGroup = 16;                // keys of one product
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;              // the running maximum is moved when x exceeds it by 2^8
@@ -98,6 +101,8 @@ struct Args {
     const float* v_scale;
     float* part;    // [grid][2][rows][D] sums, [grid][2][rows] (m, l)
     int* meta;      // [grid][4]
+    int rts;        // row tiles that a sequence can have
+    int log2C;      // CTAs of a cluster that has a segment; negative: the segments are cut by a plan
     int max_seqlen_q, total_q, B, max_blocks, n_blocks, log2P, Hq, Hkv, group, causal;
     uint32_t head_bytes;  // of a block's codes of one head: block_size * D
     float scale;
@@ -170,6 +175,7 @@ __device__ __forceinline__ long long scan(long long x, int lane) {
 // The units [0, total) dealt to G CTAs: total % G CTAs have one more than the others.
 struct Deal {
     long long each, more;
+    Deal() = default;
     __device__ __forceinline__ Deal(long long total, int G) {
         // 32-bit division, a fraction of the 64-bit one's time, wherever it does
         each = total <= 0x7fffffffLL ? (long long)((uint32_t)total / (uint32_t)G) : total / G;
@@ -344,6 +350,27 @@ template <int kPending> __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
+// Barrier of a cluster's threads: what they wrote to shared memory before is read by all after it.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address in CTA `rank` of the cluster of what lies at `smem` in this one, and loads from there.
+__device__ __forceinline__ uint32_t cluster_at(uint32_t smem, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t at) {
+    float2 x;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at) : "memory");
+    return x;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t at) {
+    float4 x;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+    return x;
+}
+
 // The pieces of one warp in the order it takes them, requested ahead of their use.
 template <int D, int NT, int W> struct Producer {
     using C = Cfg<D, NT, W>;
@@ -465,7 +492,9 @@ __device__ __forceinline__ void take_out_masked(const Args& a, const Seq& s, uin
             }
 }
 
-template <int D, int NT, int W, typename T>
+// kCluster: a cluster has a segment, its CTAs equal runs of the segment's tiles; they read one another's
+// sums and write the outputs, so that there is no plan and no second kernel.
+template <int D, int NT, int W, bool kCluster, typename T>
 __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
     attn_kv8_kernel(const Args a) {
     using C = Cfg<D, NT, W>;
@@ -484,57 +513,72 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
     // ---- this CTA's run of tiles.  Every warp finds it for itself: a lane adds up the sequences of its
     // share, then the share that holds the run's first unit is looked at, a sequence a lane
     Cursor<D, NT, W> cur;
-    const int share = (a.B + 31) / 32;
-    Seq s = {0, 0, 0, 0, 0};
-    long long mine = 0;
-#pragma unroll 4
-    for (int b = min(a.B, lane * share), i = 0; i < share && b < a.B; ++i, ++b) {
-        s = load_seq<D, NT, W>(a, b, blockIdx.x == 0);
-        mine += s.template units<C::kStart>(a.Hkv);
-    }
-    long long upto = scan(mine, lane);
-    const long long total = __shfl_sync(0xffffffffu, upto, 31);
-    const int G = (int)min((long long)gridDim.x, total);
-    if ((int)blockIdx.x >= G) {
-        if (tid == 0) a.meta[4 * blockIdx.x] = -1;
-        return;
-    }
-    const Deal deal(total, G);
-    const long long u0 = deal.start(blockIdx.x), u1 = deal.start(blockIdx.x + 1);
-    int from = __ffs(__ballot_sync(0xffffffffu, u0 < upto)) - 1;  // there is one: u0 < total
-    cur.b = from * share;
-    long long before = __shfl_sync(0xffffffffu, upto - mine, from);  // units before the sequence in hand
-    if (share > 1) {
-        const int end = min(a.B, cur.b + share);
-        for (int b = cur.b + lane;; b += 32) {
-            s.tiles = 0;
-            if (b < end) s = load_seq<D, NT, W>(a, b, false);
-            mine = s.template units<C::kStart>(a.Hkv);
-            upto = scan(mine, lane);
-            const unsigned past = __ballot_sync(0xffffffffu, u0 < before + upto);
-            if (past) {  // ends: the share holds u0
-                from = __ffs(past) - 1;
-                cur.b = __shfl_sync(0xffffffffu, b, from);
-                before += __shfl_sync(0xffffffffu, upto - mine, from);
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, upto, 31);
+    Deal deal;
+    long long u1 = 0;
+    const int rank = kCluster ? blockIdx.x & ((1 << a.log2C) - 1) : 0;
+    if constexpr (kCluster) {
+        const int segment = blockIdx.x >> a.log2C, bh = segment / a.rts;
+        cur.rt = segment - bh * a.rts;
+        cur.b = bh / a.Hkv;
+        cur.h = bh - cur.b * a.Hkv;
+        cur.s = load_seq<D, NT, W>(a, cur.b, cur.h == 0 && cur.rt == 0);
+        if (cur.rt >= cur.s.rts) return;  // the whole cluster
+        cur.tile = (int)((long long)cur.s.tiles * rank >> a.log2C);
+        cur.left = (int)((long long)cur.s.tiles * (rank + 1) >> a.log2C) - cur.tile;
+    } else {
+        const int share = (a.B + 31) / 32;
+        Seq s = {0, 0, 0, 0, 0};
+        long long mine = 0;
+    #pragma unroll 4
+        for (int b = min(a.B, lane * share), i = 0; i < share && b < a.B; ++i, ++b) {
+            s = load_seq<D, NT, W>(a, b, blockIdx.x == 0);
+            mine += s.template units<C::kStart>(a.Hkv);
         }
-    }
-    cur.s.n = __shfl_sync(0xffffffffu, s.n, from);
-    cur.s.L = __shfl_sync(0xffffffffu, s.L, from);
-    cur.s.t0 = __shfl_sync(0xffffffffu, s.t0, from);
-    cur.s.tiles = __shfl_sync(0xffffffffu, s.tiles, from);
-    cur.s.rts = __shfl_sync(0xffffffffu, s.rts, from);
-    {
-        // the segment and the tile in it; a sequence's units fit 32 bits nearly always
-        const long long local = u0 - before;
-        const int per = cur.s.tiles + C::kStart;
-        const long long seg = local <= 0x7fffffffLL ? (long long)((uint32_t)local / (uint32_t)per) : local / per;
-        cur.tile = (int)(local - seg * per) - C::kStart;
-        cur.h = (int)(seg / cur.s.rts);
-        cur.rt = (int)(seg - (long long)cur.h * cur.s.rts);
-        cur.left = (int)(u1 - u0);
+        long long upto = scan(mine, lane);
+        const long long total = __shfl_sync(0xffffffffu, upto, 31);
+        const int G = (int)min((long long)gridDim.x, total);
+        if ((int)blockIdx.x >= G) {
+            if (tid == 0) a.meta[4 * blockIdx.x] = -1;
+            return;
+        }
+        deal = Deal(total, G);
+        const long long u0 = deal.start(blockIdx.x);
+        u1 = deal.start(blockIdx.x + 1);
+        int from = __ffs(__ballot_sync(0xffffffffu, u0 < upto)) - 1;  // there is one: u0 < total
+        cur.b = from * share;
+        long long before = __shfl_sync(0xffffffffu, upto - mine, from);  // units before the sequence in hand
+        if (share > 1) {
+            const int end = min(a.B, cur.b + share);
+            for (int b = cur.b + lane;; b += 32) {
+                s.tiles = 0;
+                if (b < end) s = load_seq<D, NT, W>(a, b, false);
+                mine = s.template units<C::kStart>(a.Hkv);
+                upto = scan(mine, lane);
+                const unsigned past = __ballot_sync(0xffffffffu, u0 < before + upto);
+                if (past) {  // ends: the share holds u0
+                    from = __ffs(past) - 1;
+                    cur.b = __shfl_sync(0xffffffffu, b, from);
+                    before += __shfl_sync(0xffffffffu, upto - mine, from);
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+        cur.s.n = __shfl_sync(0xffffffffu, s.n, from);
+        cur.s.L = __shfl_sync(0xffffffffu, s.L, from);
+        cur.s.t0 = __shfl_sync(0xffffffffu, s.t0, from);
+        cur.s.tiles = __shfl_sync(0xffffffffu, s.tiles, from);
+        cur.s.rts = __shfl_sync(0xffffffffu, s.rts, from);
+        {
+            // the segment and the tile in it; a sequence's units fit 32 bits nearly always
+            const long long local = u0 - before;
+            const int per = cur.s.tiles + C::kStart;
+            const long long seg = local <= 0x7fffffffLL ? (long long)((uint32_t)local / (uint32_t)per) : local / per;
+            cur.tile = (int)(local - seg * per) - C::kStart;
+            cur.h = (int)(seg / cur.s.rts);
+            cur.rt = (int)(seg - (long long)cur.h * cur.s.rts);
+            cur.left = (int)(u1 - u0);
+        }
     }
 
     Producer<D, NT, W> pro;
@@ -555,9 +599,9 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
     for (int i = 0; i < kDepth; ++i) pro.issue(a, sm.ring[warp][i], sm.meta[warp][i], warp, lane);
 
     bool has_tail = false;  // whether the run's last segment goes on in the next CTA's
-    for (; cur.left > 0; cur.next(a)) {
+    for (bool once = kCluster; once || cur.left > 0; once = false, cur.next(a)) {
         const int first = cur.first(), run = cur.count();
-        if (run <= 0) continue;  // the cut lies in the segment's start: the next CTA has it
+        if (!kCluster && run <= 0) continue;  // the cut lies in the segment's start: the next CTA has it
         const Seq& s = cur.s;
         const int row0 = cur.rt * kRows, rows = min(kRows, s.n * a.group - row0);
 
@@ -798,10 +842,95 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int x = 4; x <= 16; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+        constexpr int kOwn = kBox / 8;  // consecutive channels a thread has in a box, of rows 2t and 2t + 1
+        if constexpr (kCluster) {
+            // every warp leaves its sums in its own ring, from which nothing is read any more: a row's
+            // channels, then its maximum and sum
+            constexpr int kStride = D + 4;
+            static_assert(kRows * kStride * 4 <= kDepth * C::kBytes, "");
+            __syncwarp();
+            float* own = reinterpret_cast<float*>(sm.ring[warp]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float* to = own + (nt * 8 + 2 * t + c) * kStride;
+                    if (g == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m[nt][c], l[nt][c]);
+#pragma unroll
+                    for (int e = 0; e < D / 32; ++e) {  // 4 channels at a time
+                        const int box = e / (kOwn / 4), i = box * (kBox / 16) + (e % (kOwn / 4)) * 2;
+                        *reinterpret_cast<float4*>(to + box * kBox + kOwn * g + (e % (kOwn / 4)) * 4) =
+                            make_float4(o[nt][i][c], o[nt][i][c + 2], o[nt][i + 1][c], o[nt][i + 1][c + 2]);
+                    }
+                }
+            cluster_sync();
+            // as many threads as CTAs share four channels of a row, each with the sums of one CTA's warps;
+            // kAhead such shares of a thread are under way at a time
+            constexpr int kVecs = D / 4, kThreads = 32 * W, kAhead = 1;
+            const int from = tid & ((1 << a.log2C) - 1);
+            const uint32_t theirs = cluster_at(smem_u32(sm.ring), from);
+            for (int i0 = (rank * kThreads + tid) >> a.log2C; i0 < rows * kVecs; i0 += kAhead * kThreads) {
+                float4 v[kAhead][W];
+                float2 ml[kAhead][W];
+                Channels<T, 4> gate[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    const int i = i0 + j * kThreads, n = i / kVecs, d = (i % kVecs) * 4;
+                    if (i >= rows * kVecs) continue;
+                    if (a.g && from == 0) {
+                        int token, hg;
+                        row_place(row0 + n, a.group, token, hg);
+                        gate[j].load_gate(a, (size_t)(s.t0 + token), cur.h * a.group + hg, d);
+                    }
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        const uint32_t row = theirs + w * (kDepth * C::kBytes) + n * (kStride * 4);
+                        v[j][w] = cluster_load4(row + d * 4);
+                        ml[j][w] = cluster_load2(row + D * 4);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    const int i = i0 + j * kThreads, n = i / kVecs, d = (i % kVecs) * 4;
+                    if (i >= rows * kVecs) continue;  // of a whole warp: a row's shares are a multiple of a warp's
+                    float M = ml[j][0].x, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int w = 1; w < W; ++w) M = fmaxf(M, ml[j][w].x);
+#pragma unroll
+                    for (int k = 1; k < kMostCluster; k <<= 1)
+                        if (k < 1 << a.log2C) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        const float f = part_weight(ml[j][w].x, ml[j][w].y, M);
+                        sum = fmaf(f, ml[j][w].y, sum);
+                        x[0] = fmaf(f, v[j][w].x, x[0]);
+                        x[1] = fmaf(f, v[j][w].y, x[1]);
+                        x[2] = fmaf(f, v[j][w].z, x[2]);
+                        x[3] = fmaf(f, v[j][w].w, x[3]);
+                    }
+#pragma unroll
+                    for (int k = 1; k < kMostCluster; k <<= 1) {
+                        if (k >= 1 << a.log2C) break;
+                        sum += __shfl_xor_sync(0xffffffffu, sum, k);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) x[u] += __shfl_xor_sync(0xffffffffu, x[u], k);
+                    }
+                    if (from == 0) {
+                        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key: 0
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) x[u] *= inv;
+                        int token, hg;
+                        row_place(row0 + n, a.group, token, hg);
+                        store_row<T, 4>(a, (size_t)(s.t0 + token), cur.h * a.group + hg, D, d, x, gate[j]);
+                    }
+                }
+            }
+            cluster_sync();  // the others have read this CTA's sums
+            continue;
+        }
         const bool whole = first == 0 && run == s.tiles;
         const int part = blockIdx.x * 2 + (first == 0 ? 1 : 0);
         float2* part_ml = reinterpret_cast<float2*>(a.part + (size_t)gridDim.x * 2 * kRows * D) + (size_t)part * kRows;
-        constexpr int kOwn = kBox / 8;  // consecutive channels a thread has in a box, of rows 2t and 2t + 1
         if constexpr (W == 1) {
             // no other warp's to add: from the registers to where they belong
 #pragma unroll
@@ -929,7 +1058,7 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
             }
         }
     }
-    if (!has_tail && tid == 0) a.meta[4 * blockIdx.x] = -1;
+    if (!kCluster && !has_tail && tid == 0) a.meta[4 * blockIdx.x] = -1;
 }
 
 // Joins the segments that were cut: part 0 of each is its owner's second one, the others are the first
@@ -1073,9 +1202,51 @@ int warps_of(long long segments, long long tokens, int D, int nt, int sms) {
     return segments >= (tokens <= 512 ? alone / 2 : alone) ? 1 : 4;
 }
 
+// log2 of the CTAs of a cluster that works on a segment for itself, or -1 where the segments go by the plan.
+// A cluster saves the plan and the second kernel, 2.5 to 4 us of a call's chain; the plan has all SMs on few
+// segments and equal runs where lengths differ.  Which it is goes by the segments and by the most key tiles
+// that one can have (by the block table: the lengths are on the device): clusters as wide as gives an SM one
+// CTA, or two where a CTA had more than four tiles else, which take longer to start; none where a CTA
+// would have more than four (two, for two column tiles, which also join 16 rows: clusters of four at most).
+// Measured, 32 q-heads on 8 kv-heads of 128, planned / by clusters: B1 x 64 7.2 / 4.2 us, B1 x 1000 9.1 / 6.5,
+// B1 x 4096 10.3 / 9.5, B1 x 8192 11.2 / 13.5 (so planned), B4 x 2000 12.1 / 9.0, B8 x 4096 19 / 17, B16 x 250
+// 10.2 / 6.1, B32 x 250 11.5 / 6.8, B64 x 250 15.7 / 13.1, B128 x 200 21.3 / 21.9 (so planned); 4 tokens x B16 x
+// 250 11.8 / 8.2, x B1 x 2000 11.1 / 11.5 (so planned).
+int cluster_of(long long segments, long long tokens, int D, int nt, int sms) {
+    const int tile = kGroup * shape_of(D, nt).groups * kMostWarps, most = nt == 1 ? 4 : 2;  // tiles of a CTA
+    const long long tiles = (tokens + tile - 1) / tile;
+    if (segments > 4LL * sms || tiles > kMostCluster * most) return -1;
+    const int widest = nt == 1 ? 3 : 2;
+    int log2C = 0;
+    while (log2C < widest && 1 << log2C < tiles && segments << (log2C + 1) <= sms) ++log2C;
+    if (log2C < widest && tiles > (long long)most << log2C && segments << (log2C + 1) <= 2LL * sms) ++log2C;
+    return tiles <= (long long)most << log2C ? log2C : -1;
+}
+
+// Lets a kernel have its shared memory, once a device.
+template <typename Kern> int raise_smem(Kern kern, size_t smem, int device, std::atomic<unsigned long long>& ready) {
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (!bit || !(ready.load(std::memory_order_relaxed) & bit)) {
+        B200_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return B200LAB_OK;
+}
+
 size_t workspace_bytes(int D, int nt, int grid) {
     const size_t rows = (size_t)grid * 2 * 8 * nt;
     return rows * D * 4 + rows * 8 + (size_t)grid * 16;
+}
+
+template <int D, int NT, typename T> int launch_clusters(const Args& a, int device, cudaStream_t st) {
+    constexpr int W = kMostWarps;
+    const unsigned segments = (unsigned)(a.B * a.Hkv * a.rts);  // cluster_of bounds them
+    constexpr size_t smem = sizeof(Smem<D, NT, W>);
+    auto kern = attn_kv8_kernel<D, NT, W, true, T>;
+    static std::atomic<unsigned long long> ready{0};  // devices whose limit is raised
+    const int rc = raise_smem(kern, smem, device, ready);
+    if (rc != B200LAB_OK) return rc;
+    return kv8_launch_clusters(1 << a.log2C, kern, dim3(segments << a.log2C), 32 * W, smem, st, a);
 }
 
 template <int D, int NT, int W, typename T>
@@ -1084,14 +1255,11 @@ int launch(Args a, void* ws, int grid, int device, cudaStream_t st) {
     a.part = static_cast<float*>(ws);
     a.meta = reinterpret_cast<int*>(a.part + rows * D + rows * 2);
     constexpr size_t smem = sizeof(Smem<D, NT, W>);
-    auto kern = attn_kv8_kernel<D, NT, W, T>;
+    auto kern = attn_kv8_kernel<D, NT, W, false, T>;
     static std::atomic<unsigned long long> ready{0};  // devices whose limit is raised
-    const unsigned long long bit = device < 64 ? 1ull << device : 0;
-    if (!bit || !(ready.load(std::memory_order_relaxed) & bit)) {
-        B200_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        ready.fetch_or(bit, std::memory_order_relaxed);
-    }
-    int rc = kv8_launch(kern, dim3(grid), 32 * W, smem, st, a);
+    int rc = raise_smem(kern, smem, device, ready);
+    if (rc != B200LAB_OK) return rc;
+    rc = kv8_launch(kern, dim3(grid), 32 * W, smem, st, a);
     if (rc != B200LAB_OK) return rc;
     const long long used = (long long)a.group * a.max_seqlen_q;
     const int rows_used = (int)(used < 8 * NT ? used : 8 * NT);
@@ -1103,6 +1271,7 @@ int launch(Args a, void* ws, int grid, int device, cudaStream_t st) {
 
 template <int D, int NT, typename T>
 int launch_warps(int warps, const Args& a, void* ws, int grid, int device, cudaStream_t st) {
+    if (a.log2C >= 0) return launch_clusters<D, NT, T>(a, device, st);
     return warps == 1 ? launch<D, NT, 1, T>(a, ws, grid, device, st) : launch<D, NT, 4, T>(a, ws, grid, device, st);
 }
 
@@ -1155,8 +1324,9 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     const int nt = column_tiles((int)rows, D);
     const Kv8Device dev = kv8_device();
     const int sms = dev.sms > 0 ? dev.sms : device_sm_count();
-    const int warps = warps_of((long long)B * Hkv * ((rows + 8 * nt - 1) / (8 * nt)), (long long)max_blocks * block_size, D,
-                               nt, sms);
+    const int rts = (int)((rows + 8 * nt - 1) / (8 * nt));
+    const long long segments = (long long)B * Hkv * rts, tokens = (long long)max_blocks * block_size;
+    const int warps = warps_of(segments, tokens, D, nt, sms);
     const int grid = plan_grid(D, nt, warps, sms);
     if (!workspace || ws_bytes < workspace_bytes(D, nt, plan_grid(D, nt, 1, sms))) return B200LAB_ERR_WORKSPACE;
     if (dev.status != B200LAB_OK) return dev.status;
@@ -1170,6 +1340,8 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     a.max_seqlen_q = most, a.total_q = total_q, a.B = B, a.max_blocks = max_blocks, a.n_blocks = n_blocks;
     a.log2P = kv8_log2_block(block_size), a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv, a.causal = causal;
     a.scale = scale;
+    a.rts = rts;
+    a.log2C = cluster_of(segments, tokens, D, nt, sms);
     a.head_bytes = (uint32_t)(block_size * D);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, warps, a, workspace, grid, dev.ordinal, st)

@@ -99,21 +99,29 @@ inline Kv8Device kv8_device() {
 // Launches `kern` with programmatic stream serialisation: every kernel of this cache waits
 // (grid_dependency_wait) before it touches memory and then lets the next one be scheduled, so
 // the steps append -> attend -> ... of a decode loop follow one another without the launch gap.
+// `cluster`: CTAs of a cluster.
 template <typename Kern, typename... Args>
-int kv8_launch(Kern kern, dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
+int kv8_launch_clusters(int cluster, Kern kern, dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return B200LAB_ERR_CUDA;
     count_launch(1);
     return cudaGetLastError() == cudaSuccess ? B200LAB_OK : B200LAB_ERR_CUDA;
+}
+template <typename Kern, typename... Args>
+int kv8_launch(Kern kern, dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
+    return kv8_launch_clusters(1, kern, grid, threads, smem, st, args...);
 }
 
 }  // namespace b200
