@@ -358,7 +358,7 @@ int kv8_read_sm100(const void* k_cache, const void* v_cache, const float* k_scal
  * so from about 64 new tokens a sequence on they are faster through
  * kv8_read_sm100 and attn_fwd_sm100_varlen (8 sequences of 4096 keys, 32 q-heads on
  * 8 of 128: 64 tokens 139 us against 147, 256 tokens 478 against 167).  Few short
- * sequences take one kernel instead of two (B1 x 1000 6.4 us against 9.1); the call knows
+ * sequences take one kernel instead of two (B1 x 1000 6.2 us against 9.1); the call knows
  * them by the width of the block table (max_blocks * block_size tokens), so one that
  * is no wider than the batch needs is faster.  Calls that may overlap need
  * workspaces of their own. */

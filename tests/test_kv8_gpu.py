@@ -627,9 +627,9 @@ def test_by_the_plan(cuda, monkeypatch, test, kw):
 
 
 @pytest.mark.parametrize("D,group", [(64, 4), (64, 12), (128, 8), (128, 9), (256, 6), (256, 11)])
-@pytest.mark.parametrize("B,longest", [(2, 900), (7, 500), (20, 260), (48, 130), (70, 40)])
+@pytest.mark.parametrize("B,longest", [(2, 900), (7, 500), (12, 950), (20, 260), (26, 990), (40, 500), (48, 130), (70, 40)])
 def test_clusters_of_every_size(cuda, D, group, B, longest):
-    """From one CTA a segment to eight, of which some have no keys; padding, several tokens, a gate, NaN wherever
+    """From one CTA a segment to eight, of four warps or eight, of which some have no keys; padding, several tokens, a gate, NaN wherever
     no token lies."""
     lens = [longest] + [(i * 53) % longest if i % 4 else 0 for i in range(1, B)]
     new = [(i * 5) % 4 for i in range(B)]

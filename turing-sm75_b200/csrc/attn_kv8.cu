@@ -36,7 +36,7 @@
 //     significant bits (below 2^-29 of the row's largest value, bits are lost).
 // Measured, 32 q-heads on 8 kv-heads of 128 unless said, calls back to back in a graph: B64 x 16k 345 us
 // (6.2 TB/s, 97 % of the measured copy rate), B64 x 400..8k 99 us (89 %), B1 x 16k 14.5 us, B1 x 1000
-// 6.4 us, 4 tokens x B16 x 2-4k 31 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 43 us, 8 heads of 64
+// 6.2 us, 4 tokens x B16 x 2-4k 31 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 43 us, 8 heads of 64
 // B48 x 250..2500 22 us.  The longest streams are bound by memory; what the shorter ones add to that is
 // a call's own chain (lengths, block ids, codes; the part's join; the second kernel: 7 us in all, 4 with clusters) and,
 // with more rows or 64 channels, the instructions of converting (0.5 issued a cycle and scheduler).
@@ -48,7 +48,8 @@ namespace {
 
 __device__ int g_err_attn_kv8 = 0;
 
-constexpr int kMostWarps = 4;             // of a CTA
+constexpr int kMostWarps = 4;             // of a CTA that goes by the plan
+constexpr int kWideWarps = 8;             // of a wide CTA of a cluster
 constexpr int kMostCluster = 8;           // CTAs of a cluster
 constexpr int kGroup = 16;                // keys of one product
 constexpr float kLog2e = 1.4426950408889634f;
@@ -864,65 +865,55 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                     }
                 }
             cluster_sync();
-            // as many threads as CTAs share four channels of a row, each with the sums of one CTA's warps;
-            // kAhead such shares of a thread are under way at a time
-            constexpr int kVecs = D / 4, kThreads = 32 * W, kAhead = 1;
+            // as many threads as CTAs share four channels of a row, each with the sums of one CTA's warps (with two
+            // shares under way a thread the tiles before them spill, 8 % slower).  A row is a multiple of 16 shares, so in
+            // clusters of two and more, whose threads exchange values, a warp is in the loop as a whole
+            constexpr int kVecs = D / 4, kThreads = 32 * W;
             const int from = tid & ((1 << a.log2C) - 1);
             const uint32_t theirs = cluster_at(smem_u32(sm.ring), from);
-            for (int i0 = (rank * kThreads + tid) >> a.log2C; i0 < rows * kVecs; i0 += kAhead * kThreads) {
-                float4 v[kAhead][W];
-                float2 ml[kAhead][W];
-                Channels<T, 4> gate[kAhead];
+            for (int at = (rank * kThreads + tid) >> a.log2C; at < rows * kVecs; at += kThreads) {
+                const int n = at / kVecs, d = (at % kVecs) * 4;
+                int i, hg;
+                row_place(row0 + n, a.group, i, hg);
+                const size_t token = (size_t)(s.t0 + i);
+                const int head = cur.h * a.group + hg;
+                Channels<T, 4> gate;
+                if (a.g && from == 0) gate.load_gate(a, token, head, d);
+                float4 v[W];
+                float2 ml[W];
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    const int i = i0 + j * kThreads, n = i / kVecs, d = (i % kVecs) * 4;
-                    if (i >= rows * kVecs) continue;
-                    if (a.g && from == 0) {
-                        int token, hg;
-                        row_place(row0 + n, a.group, token, hg);
-                        gate[j].load_gate(a, (size_t)(s.t0 + token), cur.h * a.group + hg, d);
-                    }
+                for (int w = 0; w < W; ++w) {
+                    const uint32_t row = theirs + w * (kDepth * C::kBytes) + n * (kStride * 4);
+                    v[w] = cluster_load4(row + d * 4);
+                    ml[w] = cluster_load2(row + D * 4);
+                }
+                float M = ml[0].x, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int w = 0; w < W; ++w) {
-                        const uint32_t row = theirs + w * (kDepth * C::kBytes) + n * (kStride * 4);
-                        v[j][w] = cluster_load4(row + d * 4);
-                        ml[j][w] = cluster_load2(row + D * 4);
-                    }
+                for (int w = 1; w < W; ++w) M = fmaxf(M, ml[w].x);
+#pragma unroll
+                for (int k = 1; k < kMostCluster; k <<= 1)
+                    if (k < 1 << a.log2C) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const float f = part_weight(ml[w].x, ml[w].y, M);
+                    sum = fmaf(f, ml[w].y, sum);
+                    x[0] = fmaf(f, v[w].x, x[0]);
+                    x[1] = fmaf(f, v[w].y, x[1]);
+                    x[2] = fmaf(f, v[w].z, x[2]);
+                    x[3] = fmaf(f, v[w].w, x[3]);
                 }
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    const int i = i0 + j * kThreads, n = i / kVecs, d = (i % kVecs) * 4;
-                    if (i >= rows * kVecs) continue;  // of a whole warp: a row's shares are a multiple of a warp's
-                    float M = ml[j][0].x, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int k = 1; k < kMostCluster; k <<= 1) {
+                    if (k >= 1 << a.log2C) break;
+                    sum += __shfl_xor_sync(0xffffffffu, sum, k);
 #pragma unroll
-                    for (int w = 1; w < W; ++w) M = fmaxf(M, ml[j][w].x);
+                    for (int u = 0; u < 4; ++u) x[u] += __shfl_xor_sync(0xffffffffu, x[u], k);
+                }
+                if (from == 0) {
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key: 0
 #pragma unroll
-                    for (int k = 1; k < kMostCluster; k <<= 1)
-                        if (k < 1 << a.log2C) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-#pragma unroll
-                    for (int w = 0; w < W; ++w) {
-                        const float f = part_weight(ml[j][w].x, ml[j][w].y, M);
-                        sum = fmaf(f, ml[j][w].y, sum);
-                        x[0] = fmaf(f, v[j][w].x, x[0]);
-                        x[1] = fmaf(f, v[j][w].y, x[1]);
-                        x[2] = fmaf(f, v[j][w].z, x[2]);
-                        x[3] = fmaf(f, v[j][w].w, x[3]);
-                    }
-#pragma unroll
-                    for (int k = 1; k < kMostCluster; k <<= 1) {
-                        if (k >= 1 << a.log2C) break;
-                        sum += __shfl_xor_sync(0xffffffffu, sum, k);
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) x[u] += __shfl_xor_sync(0xffffffffu, x[u], k);
-                    }
-                    if (from == 0) {
-                        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key: 0
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) x[u] *= inv;
-                        int token, hg;
-                        row_place(row0 + n, a.group, token, hg);
-                        store_row<T, 4>(a, (size_t)(s.t0 + token), cur.h * a.group + hg, D, d, x, gate[j]);
-                    }
+                    for (int u = 0; u < 4; ++u) x[u] *= inv;
+                    store_row<T, 4>(a, token, head, D, d, x, gate);
                 }
             }
             cluster_sync();  // the others have read this CTA's sums
@@ -981,7 +972,7 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
         __syncthreads();
         constexpr int kRow = C::kRow, kPer = kRow / 16;
         const int jr = tid >> 4, jd = (tid & 15) * kPer;  // this thread's row of a column tile, and channels
-        static_assert(W == 4, "8 rows x 16 threads");
+        static_assert(W == 4 || kCluster, "8 rows x 16 threads");  // (clusters have gone on above)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float f[2];
@@ -1202,25 +1193,34 @@ int warps_of(long long segments, long long tokens, int D, int nt, int sms) {
     return segments >= (tokens <= 512 ? alone / 2 : alone) ? 1 : 4;
 }
 
-// log2 of the CTAs of a cluster that works on a segment for itself, or -1 where the segments go by the plan.
-// A cluster saves the plan and the second kernel, 2.5 to 4 us of a call's chain; the plan has all SMs on few
-// segments and equal runs where lengths differ.  Which it is goes by the segments and by the most key tiles
-// that one can have (by the block table: the lengths are on the device): clusters as wide as gives an SM one
-// CTA, or two where a CTA had more than four tiles else, which take longer to start; none where a CTA
-// would have more than four (two, for two column tiles, which also join 16 rows: clusters of four at most).
-// Measured, 32 q-heads on 8 kv-heads of 128, planned / by clusters: B1 x 64 7.2 / 4.2 us, B1 x 1000 9.1 / 6.5,
-// B1 x 4096 10.3 / 9.5, B1 x 8192 11.2 / 13.5 (so planned), B4 x 2000 12.1 / 9.0, B8 x 4096 19 / 17, B16 x 250
-// 10.2 / 6.1, B32 x 250 11.5 / 6.8, B64 x 250 15.7 / 13.1, B128 x 200 21.3 / 21.9 (so planned); 4 tokens x B16 x
-// 250 11.8 / 8.2, x B1 x 2000 11.1 / 11.5 (so planned).
-int cluster_of(long long segments, long long tokens, int D, int nt, int sms) {
-    const int tile = kGroup * shape_of(D, nt).groups * kMostWarps, most = nt == 1 ? 4 : 2;  // tiles of a CTA
+// The clusters that work on a segment each: log2 of their CTAs, or -1 where the segments go by the plan, and a
+// CTA's warps.  A cluster saves the plan and the second kernel, 2.5 to 4 us of a call's chain; the plan has all
+// SMs on few segments and equal runs where lengths differ.  Which it is goes by the segments and by the most
+// key tiles that one can have (by the block table: the lengths are on the device).  A cluster is as wide as gives
+// an SM one CTA.  Where a CTA then has more than two tiles, eight warps share them, if the segments are so
+// many that the clusters are pairs at most (wider ones of such CTAs do not all find room at once: B2 x 4096
+// 16.4 us with eight CTAs of eight warps, 9.8 of four); else two CTAs an SM do, from four tiles on.
+// Measured, 32 q-heads on 8 kv-heads of 128, planned / by clusters: B1 x 64 7.2 / 4.2 us, B1 x 1000 9.1 / 6.4,
+// B1 x 4096 10.3 / 9.4, B1 x 8192 11.2 / 13.5 (so planned), B4 x 2000 12.1 / 9.0, B16 x 250 10.2 / 6.2, B32 x 250
+// 11.5 / 6.8, B64 x 250 15.7 / 12.8, B128 x 200 21.3 / 21.9 (so planned); with four warps / eight: B8 x 1000 8.9 /
+// 7.8, B16 x 500 8.4 / 7.0, B1 x 2000 7.1 / 7.8 (so four).  Two column tiles: 4 tokens x B16 x 250 planned 11.8, by
+// clusters 8.2, x B16 x 1000 15.8 / 12.2, x B1 x 2000 11.1 / 11.5 (so planned).
+struct Clusters {
+    int log2C, warps;
+};
+Clusters clusters_of(long long segments, long long tokens, int D, int nt, int sms) {
+    const Shape shape = shape_of(D, nt);
+    const int tile = kGroup * shape.groups * kMostWarps, widest = nt == 1 ? 3 : 2, most = nt == 1 ? 4 : 2;
     const long long tiles = (tokens + tile - 1) / tile;
-    if (segments > 4LL * sms || tiles > kMostCluster * most) return -1;
-    const int widest = nt == 1 ? 3 : 2;
+    if (segments > 4LL * sms || tiles > 8 * kMostCluster) return {-1, 0};
     int log2C = 0;
     while (log2C < widest && 1 << log2C < tiles && segments << (log2C + 1) <= sms) ++log2C;
+    const long long wide = (long long)sms * (shape.ctas * kMostWarps / kWideWarps);  // places of eight warps
+    if (log2C <= 1 && segments << log2C <= wide && tiles > 2LL << log2C && tiles <= 8LL << log2C)
+        return {log2C, kWideWarps};
     if (log2C < widest && tiles > (long long)most << log2C && segments << (log2C + 1) <= 2LL * sms) ++log2C;
-    return tiles <= (long long)most << log2C ? log2C : -1;
+    if (tiles > (long long)most << log2C) return {-1, 0};
+    return {log2C, kMostWarps};
 }
 
 // Lets a kernel have its shared memory, once a device.
@@ -1238,9 +1238,8 @@ size_t workspace_bytes(int D, int nt, int grid) {
     return rows * D * 4 + rows * 8 + (size_t)grid * 16;
 }
 
-template <int D, int NT, typename T> int launch_clusters(const Args& a, int device, cudaStream_t st) {
-    constexpr int W = kMostWarps;
-    const unsigned segments = (unsigned)(a.B * a.Hkv * a.rts);  // cluster_of bounds them
+template <int D, int NT, int W, typename T> int launch_clusters(const Args& a, int device, cudaStream_t st) {
+    const unsigned segments = (unsigned)(a.B * a.Hkv * a.rts);  // clusters_of bounds them
     constexpr size_t smem = sizeof(Smem<D, NT, W>);
     auto kern = attn_kv8_kernel<D, NT, W, true, T>;
     static std::atomic<unsigned long long> ready{0};  // devices whose limit is raised
@@ -1271,7 +1270,9 @@ int launch(Args a, void* ws, int grid, int device, cudaStream_t st) {
 
 template <int D, int NT, typename T>
 int launch_warps(int warps, const Args& a, void* ws, int grid, int device, cudaStream_t st) {
-    if (a.log2C >= 0) return launch_clusters<D, NT, T>(a, device, st);
+    if (a.log2C >= 0)
+        return warps == kWideWarps ? launch_clusters<D, NT, kWideWarps, T>(a, device, st)
+                                   : launch_clusters<D, NT, kMostWarps, T>(a, device, st);
     return warps == 1 ? launch<D, NT, 1, T>(a, ws, grid, device, st) : launch<D, NT, 4, T>(a, ws, grid, device, st);
 }
 
@@ -1326,7 +1327,8 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     const int sms = dev.sms > 0 ? dev.sms : device_sm_count();
     const int rts = (int)((rows + 8 * nt - 1) / (8 * nt));
     const long long segments = (long long)B * Hkv * rts, tokens = (long long)max_blocks * block_size;
-    const int warps = warps_of(segments, tokens, D, nt, sms);
+    const Clusters clusters = clusters_of(segments, tokens, D, nt, sms);
+    const int warps = clusters.log2C >= 0 ? clusters.warps : warps_of(segments, tokens, D, nt, sms);
     const int grid = plan_grid(D, nt, warps, sms);
     if (!workspace || ws_bytes < workspace_bytes(D, nt, plan_grid(D, nt, 1, sms))) return B200LAB_ERR_WORKSPACE;
     if (dev.status != B200LAB_OK) return dev.status;
@@ -1341,7 +1343,7 @@ extern "C" int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long 
     a.log2P = kv8_log2_block(block_size), a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv, a.causal = causal;
     a.scale = scale;
     a.rts = rts;
-    a.log2C = cluster_of(segments, tokens, D, nt, sms);
+    a.log2C = clusters.log2C;
     a.head_bytes = (uint32_t)(block_size * D);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return dtype == B200LAB_F16 ? launch_d<__half>(D, nt, warps, a, workspace, grid, dev.ordinal, st)
