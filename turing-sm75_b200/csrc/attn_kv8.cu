@@ -1185,7 +1185,7 @@ int plan_grid(int D, int nt, int warps, int sms) {
 // leaves few cut segments; a warp on its own joins nothing, and while it starts or ends a segment the
 // SM's other warps go on: better where segments are short and many.  The lengths are on the device, so
 // the rule goes by what the host has, the segments and the most that the block table can hold (measured
-// with four / with one, 32 q-heads on 8 kv-heads of 128 unless said: B64 x 200 tokens 14.8 / 14.0 us,
+// by the plan, with four / with one, 32 q-heads on 8 kv-heads of 128 unless said: B64 x 200 tokens 14.8 / 14.0 us,
 // B128 x 200 24.9 / 21.6, B256 x 200 40.9 / 29.1, B512 x 64 52 / 31, B128 x 2k D 64 32 heads 148 / 136,
 // B256 x 1k 79 / 81, and the other way B256 x 200..4k 188 / 197, B32 x 200 11.0 / 16.6).
 int warps_of(long long segments, long long tokens, int D, int nt, int sms) {
