@@ -405,10 +405,13 @@ template <int D, int NT, int W> struct Producer {
             if (lane >= first && lane < first + C::kH) {
                 GroupMeta* m = meta + (lane - first);
                 m->ok = block >= 0;
-                m->ks = m->vs = 1.f;
+                // a scale is stored or copied, never both: nothing orders a store before an asynchronous
+                // copy of the same thread to the same address
                 if (block >= 0) {
                     copy4(&m->ks, a.k_scale + block);
                     copy4(&m->vs, a.v_scale + block);
+                } else {
+                    m->ks = m->vs = 1.f;
                 }
             }
             const uint32_t dst = smem_u32(slot);
