@@ -1,4 +1,5 @@
-"""GPU tests of calls at the edge of what the 8-bit key/value cache documents."""
+"""GPU tests of calls at the edge of what the 8-bit key/value cache documents: blocks outside the pool between
+good ones, weights far below a row's largest."""
 import numpy as np
 import pytest
 import torch
@@ -41,3 +42,129 @@ def test_attend_bad_blocks_between_good_ones(cuda, kind, D, Hkv, B):
     ref, bound = kv8_ref.attend(q.double().cpu().numpy(), s.rk, s.rv, good, left, [1] * B, 1 / np.sqrt(D), True,
                                 unit=UNIT[q.dtype])
     _within(o, ref, bound)
+
+
+# ---- weights far below a row's largest -------------------------------------------------------------------------------
+def _attend_tight(s, q, scale):
+    """(o, bound) of one query token a sequence, where the weights' fp16 range may cost little.
+
+    A warp takes the keys in pieces of at most 32, from multiples of 32 on.  Its weights 2^(x - m), x with the log of
+    V's scale, are held to at most 2^15 (below fp16's end, 2^16), and a piece's largest to at least 2^-8, unless the
+    row's sums, moved to such an m, pass 2^60.  Rounded to fp16 they are off by 2^-11 of themselves, or by 2^-25 where
+    they are subnormal: 2^-17 of the piece's largest.  So beside the relative roundings (kv8_ref.attend), each
+    piece adds 2^-17 (its largest w sV) sum |codes|, and a weight beyond the sums' range is under 2^-25 / 2^58 of a
+    unit of l: 448 2^-83 a key.  Nothing here grows with the distance between a weight and the row's largest.
+    The output's own rounding is off by half a step: of the value, or, for an fp16 value below 2^-14, of the steps of
+    2^-24 that its subnormal numbers have: 2^-25."""
+    B, Hq, D = q.shape
+    unit, least = UNIT[q.dtype], 2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -32
+    qd = q.double().cpu().numpy()
+    o, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for b, n in enumerate(s.lens):
+        k, v = s.rk.tokens(s.table[b], n), s.rv.tokens(s.table[b], n)
+        sv = s.rv.token_scales(s.table[b], n)
+        for hq in range(Hq):
+            h = hq // (Hq // s.Hkv)
+            x = scale * (k[:, h] @ qd[b, hq])
+            p = np.exp(x - x.max())
+            w = p / p.sum()
+            o[b, hq] = w @ v[:, h]
+            size = w @ np.abs(v[:, h])
+            dx = (D + 4) * 2.0 ** -22 * scale * (np.abs(k[:, h]) @ np.abs(qd[b, hq])).max()
+            at = np.arange(0, n, 32)
+            largest = np.maximum.reduceat(w * sv[:, h], at)
+            codes = np.add.reduceat(np.abs(v[:, h]) / sv[:, h][:, None], at)
+            bound[b, hq] = ((2 * (dx + 2.0 ** -20 + n * 2.0 ** -24) + 2.0 ** -11) * size + 2.0 ** -17 * (largest @ codes)
+                            + n * 448 * 2.0 ** -83 + unit * np.abs(o[b, hq]) * (1 + 2.0 ** -6) + least)
+    return o, bound
+
+
+def _check_tight(s, q, scale, copies=1):
+    """A call with the cache as the reference has it.  copies: that many sequences of the same blocks and queries,
+    so that a warp has a whole sequence, or a quarter of one, not the few keys that it has of a lone one."""
+    for t, ts, r in ((s.k, s.ks, s.rk), (s.v, s.vs, s.rv)):
+        t.copy_(torch.from_numpy(r.values).float().to(t.dtype))
+        ts.copy_(torch.from_numpy(r.scales).float())
+    table, lens = s.t.repeat(copies, 1), s.l.repeat(copies)
+    o = b200lab.attn_fwd_kv8(q.repeat(copies, 1, 1), s.k, s.v, s.ks, s.vs, table, lens, scale=scale)
+    assert b200lab.device_status() == b200lab.OK
+    ref, bound = _attend_tight(s, q, scale)
+    for x in o.view(copies, *q.shape):
+        _within(x, ref, bound)
+
+
+def _sink(s, b, pos, h, D):
+    """Makes every score of sequence b's head h zero but that of the key at `pos`: q's channel 0 times 448 sK."""
+    for i in range(-(-s.lens[b] // s.P)):
+        s.rk.values[s.table[b][i], h] = 0
+    s.rk.values[s.table[b][pos // s.P], h, pos % s.P, 0] = 448
+
+
+def _q_of_bits(bits, D, sk, dtype):
+    """Rows whose score with the sink (scale 1) lies that many powers of two above the others'."""
+    q = torch.zeros((1, len(bits), D), dtype=torch.float32)
+    q[0, :, 0] = torch.tensor(bits) * float(np.log(2)) / (448 * sk)
+    return q.to(dtype).cuda()
+
+
+BITS = [0.0, 13.0, 16.5, 20.3, 24.5, 25.5, 29.0, 36.0]
+
+
+# one segment cut over all CTAs, one in a cluster, CTAs of four warps with a segment each, warps with one each
+FORMS = [(Setup, 128, 131072, 1), (Setup, 128, 900, 1), (Wide, 128, 2000, 450), (Wide, 128, 3000, 1800), (Setup, 128, 500, 450),
+         (Setup, 64, 700, 1), (Wide, 64, 2000, 600), (Wide, 64, 2000, 2400), (Setup, 64, 250, 580),
+         (Setup, 256, 500, 1), (Wide, 256, 2000, 300), (Wide, 256, 2000, 1200), (Setup, 256, 250, 300)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind,D,n,copies", FORMS)
+def test_attend_one_sharp_key_and_a_long_even_tail(cuda, kind, D, n, copies, dtype):
+    """One key takes most of the weight, of values 0; all the others share the rest evenly, and make the output.
+    The rows differ by how far below the sharp key's the others' weights are."""
+    s = kind([n], 1, D, 64, seed=n + D, exps=(-6, -6))
+    s.rk.scales[:] = 2.0 ** -7
+    pos = n // 20
+    _sink(s, 0, pos, 0, D)
+    s.rv.values[:] = np.abs(s.rv.values)  # of one sign: what is lost of the tail is not noise
+    # nothing but the tail in the output: the sharp key's 31 neighbours would be a term of the bound
+    s.rv.values[s.table[0][pos // 64], 0, pos % 64 // 32 * 32:][:32] = 0
+    _check_tight(s, _q_of_bits(BITS, D, 2.0 ** -7, dtype), 1.0, copies)
+
+
+@pytest.mark.parametrize("kind,D,n,copies", FORMS)
+@pytest.mark.parametrize("far", [9, 11, 20, 44])
+def test_attend_sharp_key_in_a_block_of_large_values(cuda, kind, D, n, copies, far):
+    """The sharp key's block has a V scale 2^far times the others', and codes of 0 in all channels but one: the
+    other channels are made by the small weights alone."""
+    s = kind([n], 1, D, 16, seed=far, exps=(-12, -12))
+    s.rk.scales[:] = 2.0 ** -7
+    pos = n // 20
+    _sink(s, 0, pos, 0, D)
+    s.rv.values[:] = np.abs(s.rv.values)
+    block = s.table[0][pos // 16]
+    s.rv.scales[block] = 2.0 ** (far - 12)
+    for i in (pos // 32 * 2, pos // 32 * 2 + 1):  # and its neighbours' in a piece of 32
+        s.rv.values[s.table[0][i]] = 0
+    s.rv.values[block, 0, pos % 16, 9] = 448
+    _check_tight(s, _q_of_bits(BITS, D, 2.0 ** -7, torch.bfloat16), 1.0, copies)
+
+
+@pytest.mark.parametrize("copies", [1, 60, 240])
+@pytest.mark.parametrize("kind", [Setup, Wide], ids=["narrow", "wide"])
+@pytest.mark.parametrize("D,group,P", [(64, 8, 16), (128, 4, 16), (128, 12, 32), (256, 6, 128), (64, 20, 64)])
+def test_attend_scales_far_apart_tight(cuda, kind, D, group, P, copies):
+    """V scales of 2^-40 to 2^40 in no order, scores some tens apart: rows' references go up and down all the time."""
+    s = kind([900, 64, 333, 1, 40], 2, D, P, seed=D + P, exps=(-40, 40))
+    s.rk.scales[:] = np.exp2(np.random.default_rng(3).integers(-8, -3, s.rk.scales.shape))
+    _check_tight(s, _normal((5, 2 * group, D), 6, torch.bfloat16, 2.0).cuda(), 0.09, copies)
+
+
+@pytest.mark.parametrize("copies", [1, 450, 1800])
+def test_attend_tail_beyond_the_sums_range(cuda, copies):
+    """Blocks of zeros have the smallest scale; here all have it, and the tail lies up to 2^-300 below the sharp key:
+    nothing overflows, and what is lost is below any value that the cache can hold."""
+    s = Wide([3000], 1, 128, 16, seed=1, exps=(-40, -40))
+    s.rk.scales[:] = 2.0 ** -7
+    _sink(s, 0, 700, 0, 128)
+    _check_tight(s, _q_of_bits([1.0, 20.0, 45.0, 70.0, 100.0, 120.0, 126.0, 300.0], 128, 2.0 ** -7, torch.bfloat16), 1.0,
+                 copies)

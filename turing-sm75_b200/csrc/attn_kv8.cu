@@ -6,9 +6,16 @@
 //
 // Mathematics.  For a query row r and key j, with the codes c and the scales sK, sV of j's block:
 //   x = scale log2(e) sK (q . cK) + log2(sV),  p = 2^(x - m),  O = sum p cV,  l = sum p / sV,
-// m a running maximum of x, and o = O / l.  The scale of V rides in the exponent of the weights,
-// so codes are multiplied as they are, whatever the blocks' scales.  (Scales are 2^e, |e| <= 40:
-// a weight that underflows to 0 in p counts less than 2^-46 of l.)
+// m a reference of the row's, and o = O / l.  The scale of V rides in the exponent of the weights,
+// so codes are multiplied as they are, whatever the blocks' scales.
+// The products take p in fp16, which has 40 powers of two where a long row's weights, times scales of
+// 2^-40 to 2^40, span any number.  So m is no running maximum: it follows the keys in hand, up and down.
+// p stays below 2^15, and the largest p of a piece (the 16 or 32 keys a warp takes at a time) above 2^-8, so that
+// a rounding to fp16 is off by 2^-11 of the weight or 2^-17 of its piece's largest, however small the piece's
+// weights are beside the row's others: many small weights together count in full.  (With a running maximum for
+// m, a warp that met a key 2^26 above its others lost all of those; 0.5 to 4 % of a call's time is what it costs.)  m
+// goes no lower than where l, in fp32, would pass 2^60; what fp16 loses of a weight there moves an output
+// by less than 448 x 2^-83.
 //
 // What bounds it: the bytes of the cache; a code is used by the few rows of its kv group only
 // (2 x rows flop a byte).  Everything follows from streaming them:
@@ -31,7 +38,7 @@
 //   * The channel and key order inside a product is free: each thread takes 32 consecutive channels
 //     of a K row (two 16-byte shared loads, conflict-free as the chunks are swizzled) and 16 of four V
 //     rows, whose bytes it pairs by key with one PRMT for two conversions.
-//   * No lane asks the others for a row's maximum until a score lies 2^8 above the one in use.
+//   * No lane asks the others for a row's largest score while each finds its own in the range of m.
 //   * Q is brought to fp16 with a power of two a row: exact, as bf16 and fp16 both have at most 11
 //     significant bits (below 2^-29 of the row's largest value, bits are lost).
 // Measured, 32 q-heads on 8 kv-heads of 128 unless said, calls back to back in a graph: B64 x 16k 345 us
@@ -53,7 +60,10 @@ constexpr int kWideWarps = 8;             // of a wide CTA of a cluster
 constexpr int kMostCluster = 8;           // CTAs of a cluster
 constexpr int kGroup = 16;                // keys of one product
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 8.f;              // the running maximum is moved when x exceeds it by 2^8
+// A row's reference m is moved when a score lies above m + kTop, to kRise below it, or when a piece has none as high
+// as m + kBottom, to kFall above its largest.
+constexpr float kTop = 15.f, kRise = 10.f, kBottom = -8.f, kFall = 4.f;
+constexpr int kMostSum = 60;              // and not to where its sum l would pass 2^60
 
 // What a variant's CTA works on and holds; `ctas` (of four warps) fill an SM's registers and shared
 // memory.  Two groups a piece halve what a piece costs beside its products where registers allow it
@@ -224,12 +234,12 @@ template <int D, int NT, int W> struct Smem {
     float qscale[8 * NT];
 };
 
-// The factor that brings a part's sums from its own maximum m to the common one M.  A part without
-// scores counts nothing, one whose scores are all NaN (l is NaN) everything.
+// The factor that brings a part's sums from its own level m to the largest one M.  A part without scores counts
+// nothing, one whose scores are all NaN (l is NaN) everything.  Every part has an l of 1 to 2 times the parts that it
+// is made of: what underflows counts less than 2^-126 of the sum.
 __device__ __forceinline__ float part_weight(float m, float l, float M) {
     return m == -INFINITY && l == l ? 0.f : ex2(m - M);
 }
-
 // Row n of a row tile -> query token of the sequence and head of the group.
 __device__ __forceinline__ void row_place(int row, int group, int& i, int& hg) {
     i = row / group;
@@ -729,7 +739,7 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                 // ---- softmax over the piece: thread (g, t) has keys key(g), key(g) + 8 of each group and rows
                 // 2t, 2t + 1
                 const bool edge = base + kPiece > all_see || !whole_piece;  // some key is masked for some row
-                bool moved = false;  // some score of this thread is far above its row's maximum so far
+                bool out = false;  // this thread's largest score of some row is not in the range of the row's m
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -754,25 +764,45 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                         float x = fmaxf(sc[0][nt][0][c], sc[0][nt][0][c + 2]);
 #pragma unroll
                         for (int u = 1; u < kH; ++u) x = fmaxf(x, fmaxf(sc[u][nt][0][c], sc[u][nt][0][c + 2]));
-                        moved |= x > m[nt][c] + kLazy;
+                        out |= !(fabsf(x - m[nt][c] - (kTop + kBottom) / 2) <= (kTop - kBottom) / 2);
                     }
                 }
-                // The maximum only has to keep 2^(x - m) in range, and fp16 has room for 2^kLazy: no lane asks
-                // the others for theirs until one lies beyond that.
-                if (__builtin_expect(__any_sync(0xffffffffu, moved), 0)) {
+                if (__builtin_expect(__any_sync(0xffffffffu, out), 0)) {
+                    float x[NT][2], to[NT][2];  // of each row: the largest score of all lanes, and the new m
+                    bool fall = false;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float x = fmaxf(sc[0][nt][0][c], sc[0][nt][0][c + 2]);
+                            x[nt][c] = fmaxf(sc[0][nt][0][c], sc[0][nt][0][c + 2]);
 #pragma unroll
-                            for (int u = 1; u < kH; ++u) x = fmaxf(x, fmaxf(sc[u][nt][0][c], sc[u][nt][0][c + 2]));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                            const float to = fmaxf(m[nt][c], x);
-                            const float f = to == -INFINITY ? 1.f : ex2(m[nt][c] - to);
-                            m[nt][c] = to;
+                            for (int u = 1; u < kH; ++u) x[nt][c] = fmaxf(x[nt][c], fmaxf(sc[u][nt][0][c], sc[u][nt][0][c + 2]));
+#pragma unroll
+                            for (int k = 4; k <= 16; k <<= 1) x[nt][c] = fmaxf(x[nt][c], __shfl_xor_sync(0xffffffffu, x[nt][c], k));
+                            to[nt][c] = x[nt][c] > m[nt][c] + kTop ? x[nt][c] - kRise : m[nt][c];
+                            fall |= x[nt][c] > -INFINITY && x[nt][c] < m[nt][c] + kBottom;
+                        }
+                    if (__any_sync(0xffffffffu, fall)) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                float sum = l[nt][c];
+#pragma unroll
+                                for (int k = 4; k <= 16; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+                                // (a sum that is NaN has the largest exponent: m stays)
+                                const int room = kMostSum - 1 - ((int)(__float_as_uint(sum) >> 23) - 127);
+                                if (x[nt][c] > -INFINITY && x[nt][c] < m[nt][c] + kBottom)
+                                    to[nt][c] = fmaxf(x[nt][c] + kFall, m[nt][c] - (float)max(room, 0));
+                            }
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (!__any_sync(0xffffffffu, to[nt][0] != m[nt][0] || to[nt][1] != m[nt][1])) continue;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float f = to[nt][c] == m[nt][c] ? 1.f : ex2(m[nt][c] - to[nt][c]);
+                            m[nt][c] = to[nt][c];
                             l[nt][c] *= f;
 #pragma unroll
                             for (int i = 0; i < D / 16; ++i) {
@@ -793,8 +823,8 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                         const float p2 = ex2(sc[u][nt][0][2] - m0), p3 = ex2(sc[u][nt][0][3] - m1);
                         l[nt][0] = fmaf(p0 + p2, gi[u], l[nt][0]);
                         l[nt][1] = fmaf(p1 + p3, gi[u], l[nt][1]);
-                        // the weights are rounded to fp16 (2^-11 relative); the sum l takes them before: a
-                        // weight that is small because its block's scale is counts in l all the same
+                        // the weights are rounded to fp16, of which the head of this file says how much it costs; the
+                        // sum l takes them before
                         pb[u][nt][0] = transpose8x8(pack_h2(p0, p1));
                         pb[u][nt][1] = transpose8x8(pack_h2(p2, p3));
                     }
@@ -846,6 +876,25 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int x = 4; x <= 16; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+        const bool whole = first == 0 && run == s.tiles;
+        if (W > 1 || !whole) {
+            // to be joined: m lies anywhere below the weights that make l; here it becomes their level, by a power of two
+            // that brings l to [1, 2) (no scores: l is 0 and m -infinity, and both stay)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t field = min(__float_as_uint(l[nt][c]) >> 23, 253u);
+                    const float f = __uint_as_float((254u - field) << 23);
+                    m[nt][c] += (float)((int)field - 127);
+                    l[nt][c] *= f;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        o[nt][i][c] *= f;
+                        o[nt][i][c + 2] *= f;
+                    }
+                }
+        }
         constexpr int kOwn = kBox / 8;  // consecutive channels a thread has in a box, of rows 2t and 2t + 1
         if constexpr (kCluster) {
             // every warp leaves its sums in its own ring, from which nothing is read any more: a row's
@@ -922,7 +971,6 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
             cluster_sync();  // the others have read this CTA's sums
             continue;
         }
-        const bool whole = first == 0 && run == s.tiles;
         const int part = blockIdx.x * 2 + (first == 0 ? 1 : 0);
         float2* part_ml = reinterpret_cast<float2*>(a.part + (size_t)gridDim.x * 2 * kRows * D) + (size_t)part * kRows;
         if constexpr (W == 1) {
