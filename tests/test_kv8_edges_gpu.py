@@ -1,12 +1,12 @@
 """GPU tests of calls at the edge of what the 8-bit key/value cache documents: blocks outside the pool between
-good ones, weights far below a row's largest."""
+good ones, weights far below a row's largest, padding entries."""
 import numpy as np
 import pytest
 import torch
 
 import b200lab
 import kv8_ref
-from test_kv8_gpu import UNIT, Setup, Wide, _normal
+from test_kv8_gpu import UNIT, Setup, Wide, _normal, _prefix
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +168,35 @@ def test_attend_tail_beyond_the_sums_range(cuda, copies):
     _sink(s, 0, 700, 0, 128)
     _check_tight(s, _q_of_bits([1.0, 20.0, 45.0, 70.0, 100.0, 120.0, 126.0, 300.0], 128, 2.0 ** -7, torch.bfloat16), 1.0,
                  copies)
+
+
+# ---- rows that see no key --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,D,Hkv,group,lens,new", [
+    (Setup, 128, 2, 4, [0, 70, 0, 5], [1, 1, 1, 1]),                          # clusters
+    (Setup, 64, 2, 5, [3, 0, 200], [7, 2, 2]),
+    (Wide, 128, 2, 4, [0, 70, 0, 5], [1, 1, 1, 1]),                           # the plan, four warps a CTA
+    (Wide, 256, 2, 3, [3, 0, 200], [7, 2, 2]),
+    (Wide, 64, 8, 2, [(i * 7) % 40 if i % 3 else 0 for i in range(300)], [1] * 300),  # a warp a CTA
+    (Setup, 128, 8, 2, [(i * 7) % 40 if i % 3 else 0 for i in range(300)], [1] * 300),
+    (Wide, 128, 1, 4, [300], [310]),                                          # cut segments, a warp a row joins them
+    (Wide, 128, 1, 1, [129], [130]),                                          # cut segments, a block a row
+    (Wide, 256, 1, 1, [129], [133])])
+def test_rows_without_keys_are_zero_whatever_their_gate(cuda, kind, D, Hkv, group, lens, new):
+    """A padded batch's unwritten activations: q and the gate are NaN or infinite in the rows that see no key."""
+    s = kind(lens, Hkv, D, 16, seed=D, garbage=True)
+    q, gate = (_normal((sum(new), Hkv * group, D), i, torch.bfloat16) for i in (5, 6))
+    none = torch.tensor([n - m + i < 0 for n, m in zip(lens, new) for i in range(m)])
+    assert bool(none.any())
+    ref, bound = kv8_ref.attend(q.double().numpy(), s.rk, s.rv, s.table, lens, new, 1 / np.sqrt(D), True,
+                                gate.double().numpy(), UNIT[q.dtype])
+    assert not ref[none.numpy()].any()
+    q[none] = float("nan")
+    gate[none] = float("nan")
+    gate[none, 0, 1] = float("inf")
+    one = max(new) == 1
+    out = torch.full(q.shape, 55.0, dtype=q.dtype, device="cuda")
+    b200lab.attn_fwd_kv8(q.cuda(), *s.cache, s.l, cu_seqlens_q=None if one else _prefix(new), max_seqlen_q=max(new),
+                         gate=gate.cuda(), out=out)
+    assert b200lab.device_status() == b200lab.OK
+    assert bool((out[none.cuda()] == 0).all())
+    _within(out, ref, bound)

@@ -265,12 +265,18 @@ template <typename T, int kPer> struct Channels {
         }
     }
 };
+// Stores channels of a row whose sums are x and `sum`.  A row that sees no key (sum 0) is 0 whatever its gate: a padding
+// entry's may be NaN.
 template <typename T, int kPer>
 __device__ __forceinline__ void store_row(const Args& a, size_t token, int head, int D, int d0, const float (&x)[kPer],
-                                          const Channels<T, kPer>& gate) {
+                                          float sum, const Channels<T, kPer>& gate) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     float y[kPer];
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) y[u] = a.g ? x[u] / (1.f + __expf(-Elem<T>::to_f(gate.v[u]))) : x[u];
+    for (int u = 0; u < kPer; ++u) {
+        y[u] = x[u] * inv;
+        if (a.g && sum != 0.f) y[u] = y[u] / (1.f + __expf(-Elem<T>::to_f(gate.v[u])));
+    }
     uint32_t w[kPer / 2];
 #pragma unroll
     for (int u = 0; u < kPer; u += 2) w[u / 2] = Elem<T>::pack2(y[u], y[u + 1]);
@@ -962,10 +968,7 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                     for (int u = 0; u < 4; ++u) x[u] += __shfl_xor_sync(0xffffffffu, x[u], k);
                 }
                 if (from == 0) {
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key: 0
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) x[u] *= inv;
-                    store_row<T, 4>(a, token, head, D, d, x, gate);
+                    store_row<T, 4>(a, token, head, D, d, x, sum, gate);
                 }
             }
             cluster_sync();  // the others have read this CTA's sums
@@ -981,7 +984,6 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                 for (int c = 0; c < 2; ++c) {
                     const int n = nt * 8 + 2 * t + c;
                     if (n >= rows) continue;
-                    const float inv = l[nt][c] == 0.f ? 0.f : 1.f / l[nt][c];  // a row that sees no key: 0
                     int i, hg;
                     row_place(row0 + n, a.group, i, hg);
                     const size_t token = (size_t)(s.t0 + i);
@@ -997,11 +999,9 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                             x[2 * u + 1] = o[nt][box * (kBox / 16) + from / 2 + u][c + 2];
                         }
                         if (whole) {
-#pragma unroll
-                            for (int u = 0; u < 8; ++u) x[u] *= inv;
                             Channels<T, 8> gate;
                             if (a.g) gate.load_gate(a, token, head, ch);
-                            store_row<T, 8>(a, token, head, D, ch, x, gate);
+                            store_row<T, 8>(a, token, head, D, ch, x, l[nt][c], gate);
                         } else {
                             float4* p = reinterpret_cast<float4*>(a.part + ((size_t)part * kRows + n) * D + ch);
                             p[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -1067,16 +1067,13 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
 #pragma unroll
                         for (int u = 0; u < kPer; ++u) x[u] += sm.join[w][jr][jd + u];
                     if (whole) {
-                        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key: 0
-#pragma unroll
-                        for (int u = 0; u < kPer; ++u) x[u] *= inv;
                         int i, hg;
                         row_place(row0 + n, a.group, i, hg);
                         const size_t token = (size_t)(s.t0 + i);
                         const int head = cur.h * a.group + hg;
                         Channels<T, kPer> gate;
                         if (a.g) gate.load_gate(a, token, head, d * kRow + jd);
-                        store_row<T, kPer>(a, token, head, D, d * kRow + jd, x, gate);
+                        store_row<T, kPer>(a, token, head, D, d * kRow + jd, x, sum, gate);
                     } else {
                         float* p = a.part + ((size_t)part * kRows + n) * D + d * kRow + jd;
 #pragma unroll
@@ -1216,10 +1213,7 @@ __global__ void __launch_bounds__(kFew ? 512 : 256) attn_kv8_join_kernel(const A
         }
     }
     if (n >= rows) return;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int u = 0; u < kVec; ++u) x[u] *= inv;
-    store_row<T, kVec>(a, token, head, D, lane * kVec, x, gate);
+    store_row<T, kVec>(a, token, head, D, lane * kVec, x, sum, gate);
 }
 
 // Column tiles of 8 query rows a CTA works on at once; rows beyond take further passes over the keys,
