@@ -314,7 +314,8 @@ int gdn_decode_sm100_state16(const void* q, const void* k, const void* v,
  *   seq_lens counts the new tokens too.
  *   cu_seqlens : [B+1] device int32 prefix sums of the n_b; NULL: one token a
  *          sequence (total_tokens == B, max_seqlen 1), and a sequence with
- *          seq_lens[b] <= 0 is a padding entry, of which nothing is written.
+ *          seq_lens[b] == 0 is a padding entry, of which nothing is written (a
+ *          negative length is reported, as attn_fwd_sm100_kv8 reports it).
  *   max_seqlen : the most new tokens a sequence has (bounds the grid).
  * The scale of a (block, head) is the smallest power of two in range with
  * max |x| <= 448 * scale over the finite values written to it; a block begun by
@@ -351,8 +352,8 @@ int kv8_read_sm100(const void* k_cache, const void* v_cache, const float* k_scal
  *   cu_seqlens_q : [B+1] device int32 prefix sums of the query tokens n_b; NULL:
  *       one token a sequence (total_q == B, max_seqlen_q 1).
  *   causal: query i of n_b sees the keys j <= i + seq_lens[b] - n_b.  A row that
- *       sees no key (seq_lens[b] == 0, a padding entry) is written as 0.  Rows
- *       behind the last sequence are left as they were.
+ *       sees no key (seq_lens[b] == 0, a padding entry) is written as 0, whatever
+ *       Q and G hold there.  Rows behind the last sequence are left as they were.
  * GQA as attn_fwd_sm100.  Any number of query tokens is right, but the kernel is
  * made for few: it reads the cache once for every 8 or 16 rows of a kv group,
  * so from about 64 new tokens a sequence on they are faster through

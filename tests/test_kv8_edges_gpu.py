@@ -1,12 +1,12 @@
 """GPU tests of calls at the edge of what the 8-bit key/value cache documents: blocks outside the pool between
-good ones, weights far below a row's largest, padding entries."""
+good ones, padding entries, weights far below a row's largest."""
 import numpy as np
 import pytest
 import torch
 
 import b200lab
 import kv8_ref
-from test_kv8_gpu import UNIT, Setup, Wide, _normal, _prefix
+from test_kv8_gpu import UNIT, Setup, Wide, _ints, _normal, _prefix
 
 pytestmark = pytest.mark.gpu
 
@@ -200,3 +200,22 @@ def test_rows_without_keys_are_zero_whatever_their_gate(cuda, kind, D, Hkv, grou
     assert b200lab.device_status() == b200lab.OK
     assert bool((out[none.cuda()] == 0).all())
     _within(out, ref, bound)
+
+
+# ---- padding entries -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bad", [-1, -5, -2 ** 31])
+def test_append_reports_a_negative_length(cuda, bad):
+    """A padding entry of a step has length 0; the step's append and its attention both report a negative one."""
+    s = Setup([20, 30, 40], 2, 128, 16, seed=1)
+    k, v = (_normal((3, 2, 128), i, torch.bfloat16) for i in (1, 2))
+    lens = _ints([20, bad, 40])
+    b200lab.kv8_append(k.cuda(), v.cuda(), *s.cache, lens)
+    assert b200lab.device_status() == b200lab.ERR_INVALID
+    for r, x in ((s.rk, k), (s.rv, v)):
+        r.append(x.double().numpy()[[0, 2]], [s.table[0], s.table[2]], [20, 40], [1, 1])
+    s.same()
+    b200lab.attn_fwd_kv8(_normal((3, 4, 128), 3, torch.bfloat16).cuda(), *s.cache, lens)
+    assert b200lab.device_status() == b200lab.ERR_INVALID
+    b200lab.kv8_append(k.cuda(), v.cuda(), *s.cache, _ints([0, 0, 0]))
+    assert b200lab.device_status() == b200lab.OK
+    s.same()

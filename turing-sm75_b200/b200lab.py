@@ -503,7 +503,7 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, 
     (fp16/bf16/fp32; strided views of a fused projection are taken as they are); k_cache, v_cache
     [n_blocks,Hkv,block_size,D] float8_e4m3fn; k_scale, v_scale [n_blocks,Hkv] fp32 powers of two;
     block_table int32 [B,max_blocks]; seq_lens int32 [B], the new tokens counted; cu_seqlens int32
-    [B+1] of the new tokens (None: one a sequence, seq_lens <= 0 marking padding) with max_seqlen
+    [B+1] of the new tokens (None: one a sequence, a length of 0 marking padding) with max_seqlen
     the most of one sequence."""
     args = (k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, max_seqlen)
     f = _native().append

@@ -122,7 +122,7 @@ __device__ __forceinline__ AppendItem append_item(const AppendArgs& a, long long
     const int L = a.lens[b];
     const int t0 = a.cu ? a.cu[b] : b;
     const long long n = a.cu ? (long long)a.cu[b + 1] - t0 : 1;
-    if (n == 0 || (!a.cu && L <= 0)) return it;  // nothing new, or a padding entry of a step
+    if (n == 0 || (!a.cu && L == 0)) return it;  // nothing new, or a padding entry of a step
     if (t0 < 0 || n < 0 || t0 + n > a.total || n > a.max_seqlen || L < n || L > ((long long)a.max_blocks << a.log2P)) {
         if (local == 0) report_invalid();
         return it;
