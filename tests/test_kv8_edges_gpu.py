@@ -219,3 +219,33 @@ def test_append_reports_a_negative_length(cuda, bad):
     b200lab.kv8_append(k.cuda(), v.cuda(), *s.cache, _ints([0, 0, 0]))
     assert b200lab.device_status() == b200lab.OK
     s.same()
+
+
+# ---- the host's side -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", [Setup, Wide], ids=["narrow", "wide"])
+def test_calls_after_a_failed_call_of_the_program(cuda, kind):
+    """The runtime remembers the last error of a thread, here that of selecting a device that there is not; it
+    is not the following calls'."""
+    import ctypes
+    s, t = kind([900, 33], 2, 128, 16, seed=1), kind([900, 33], 2, 128, 16, seed=1)
+    x = _normal((2, 2, 128), 1, torch.bfloat16).cuda()
+    q = _normal((2, 8, 128), 2, torch.bfloat16).cuda()
+    cu = _ints([0, 900, 933])
+    b200lab.kv8_append(x, x, *t.cache, t.l)
+    want, (wk, wv) = b200lab.attn_fwd_kv8(q, *t.cache, t.l), b200lab.kv8_read(*t.cache, cu, 900, 933)
+    runtime = ctypes.CDLL("libcudart.so.12")
+    # every buffer given: torch's allocator looks at the last error, too, where it takes new memory
+    out, k, v = torch.empty_like(want), torch.empty_like(wk), torch.empty_like(wv)
+    ws = torch.empty(b200lab.attn_fwd_kv8_workspace_bytes(8, 2, 1, 128), dtype=torch.uint8, device="cuda")
+    calls = (lambda: b200lab.kv8_append(x, x, *s.cache, s.l),
+             lambda: b200lab.attn_fwd_kv8(q, *s.cache, s.l, out=out, workspace=ws),
+             lambda: b200lab.kv8_read(*s.cache, cu, 900, 933, k_out=k, v_out=v))
+    got = []
+    try:
+        for call in calls:
+            assert runtime.cudaSetDevice(4096) != 0
+            got.append(call())
+    finally:
+        runtime.cudaGetLastError()
+    assert b200lab.device_status() == b200lab.OK
+    assert torch.equal(got[1], want) and torch.equal(got[2][0], wk) and torch.equal(got[2][1], wv)

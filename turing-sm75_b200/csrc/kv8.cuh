@@ -115,9 +115,14 @@ int kv8_launch_clusters(int cluster, Kern kern, dim3 grid, int threads, size_t s
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return B200LAB_ERR_CUDA;
+    // The launch's own status alone: the thread's last error may be an earlier call's, and a call that reported it
+    // would have written the cache, or stopped between its two kernels.
+    if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) {
+        (void)cudaGetLastError();  // it is reported here, and not again by the program's next check
+        return B200LAB_ERR_CUDA;
+    }
     count_launch(1);
-    return cudaGetLastError() == cudaSuccess ? B200LAB_OK : B200LAB_ERR_CUDA;
+    return B200LAB_OK;
 }
 template <typename Kern, typename... Args>
 int kv8_launch(Kern kern, dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
