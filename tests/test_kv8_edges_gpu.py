@@ -249,3 +249,26 @@ def test_calls_after_a_failed_call_of_the_program(cuda, kind):
         runtime.cudaGetLastError()
     assert b200lab.device_status() == b200lab.OK
     assert torch.equal(got[1], want) and torch.equal(got[2][0], wk) and torch.equal(got[2][1], wv)
+
+
+# ---- strides ---------------------------------------------------------------------------------------------------------
+def test_strides_of_dimensions_of_one(cuda):
+    """One token, or one kv-head, cut out of rows of any length: the stride that is never taken does not matter."""
+    D = 128
+    wide = torch.zeros((1, 3 * 2 * D + 4), dtype=torch.bfloat16, device="cuda")  # a projection with four values more
+    wide.copy_(_normal(tuple(wide.shape), 3))
+    st = (3 * 2 * D + 4, D, 1)
+    q, k, v = (wide.as_strided((1, 2, D), st, i * 2 * D) for i in range(3))
+    s, t = (Setup([40], 2, D, 16, seed=1) for _ in range(2))
+    for c, args in ((s, (q, k, v, q)), (t, tuple(x.clone(memory_format=torch.contiguous_format) for x in (q, k, v, q)))):
+        b200lab.kv8_append(args[1], args[2], *c.cache, c.l)
+        c.o = b200lab.attn_fwd_kv8(args[0], *c.cache, c.l, gate=args[3])
+    assert torch.equal(s.o, t.o) and torch.equal(s.k.view(torch.uint8), t.k.view(torch.uint8))
+    rows = _normal((3, D + 8), 4, torch.bfloat16).cuda()
+    one = rows.as_strided((3, 1, D), (D + 8, 5, 1))
+    s, t = (Setup([40, 7, 19], 1, D, 16, seed=2) for _ in range(2))
+    for c, x in ((s, one), (t, one.clone(memory_format=torch.contiguous_format))):
+        b200lab.kv8_append(x, x, *c.cache, c.l)
+        c.o = b200lab.attn_fwd_kv8(x, *c.cache, c.l, gate=x)
+    assert b200lab.device_status() == b200lab.OK
+    assert torch.equal(s.o, t.o) and torch.equal(s.v.view(torch.uint8), t.v.view(torch.uint8))

@@ -92,6 +92,9 @@ struct Cache {
     }
 };
 
+// The stride of a dimension; 0 where it has one entry and is never stepped over, when torch lets it be any number.
+int64_t stride(const Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
 Tensor empty(at::IntArrayRef sizes, at::ScalarType dtype, c10::Device device) {
     return at::empty(sizes, at::TensorOptions().dtype(dtype).device(device));
 }
@@ -115,7 +118,7 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
     const int code = dtype_code(k), most = integer(o[9], "max_seqlen");
     if (total == 0 && (cu || c.B == 0)) return status(B200LAB_OK);
     const c10::cuda::CUDAGuard guard(c.device);
-    return status(kv8_append_sm100(kp, k.stride(0), k.stride(1), vp, v.stride(0), v.stride(1), c.k.data_ptr(),
+    return status(kv8_append_sm100(kp, stride(k, 0), stride(k, 1), vp, stride(v, 0), stride(v, 1), c.k.data_ptr(),
                                    c.v.data_ptr(), static_cast<float*>(c.ks.data_ptr()),
                                    static_cast<float*>(c.vs.data_ptr()), static_cast<const int*>(c.table.data_ptr()), lens,
                                    cu, most, total, c.B, c.max_blocks, c.n_blocks, c.block_size, c.Hkv, c.D, code,
@@ -187,7 +190,7 @@ PyObject* attend(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const Tensor& g = tensor(o[9], "gate");
         TORCH_CHECK_TYPE(g.scalar_type() == q.scalar_type(), "gate must have q's dtype");
         gp = c.rows(g, total, Hq, "gate");
-        gt = g.stride(0), gh = g.stride(1);
+        gt = stride(g, 0), gh = stride(g, 1);
     }
     double scale = 1.0 / std::sqrt((double)c.D);
     if (o[10] != Py_None) {
@@ -217,7 +220,7 @@ PyObject* attend(PyObject*, PyObject* const* o, Py_ssize_t n) {
                           "workspace must be contiguous, on the cache's device");
     }
     const int st = attn_fwd_sm100_kv8(
-        qp, q.stride(0), q.stride(1), gp, gt, gh, c.k.data_ptr(), c.v.data_ptr(),
+        qp, stride(q, 0), stride(q, 1), gp, gt, gh, c.k.data_ptr(), c.v.data_ptr(),
         static_cast<const float*>(c.ks.data_ptr()), static_cast<const float*>(c.vs.data_ptr()),
         static_cast<const int*>(c.table.data_ptr()), lens, cu, most, total, out.data_ptr(), c.B, c.max_blocks, c.n_blocks,
         c.block_size, Hq, c.Hkv, c.D, (float)scale, causal, code, ws.data_ptr(), (size_t)ws.numel() * ws.element_size(),
