@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libb200lab.so")
@@ -477,11 +478,17 @@ def _native():
     if _NATIVE is None:
         import importlib.machinery
         import importlib.util
-        _torch()  # its libraries first
+        import sysconfig
+        torch = _torch()  # its libraries first
         lib()
         path = os.path.join(_HERE, "lib", "_b200torch.so")
         if not os.path.exists(path):
             raise FileNotFoundError(f"{path} is missing: build it with `make -C {_HERE}`")
+        fits = f"{sysconfig.get_config_var('SOABI')} {torch.__version__}"
+        with open(os.path.join(_HERE, "lib", "_b200torch.txt")) as f:
+            built = f.read().strip()
+        if built != fits:  # another Python's or torch's layout of objects: it would crash, not raise
+            raise ImportError(f"{path} was built for {built}, this is {fits}: `make -C {_HERE} PYTHON={sys.executable}`")
         loader = importlib.machinery.ExtensionFileLoader("_b200torch", path)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_b200torch", loader))
         loader.exec_module(module)
