@@ -272,3 +272,29 @@ def test_strides_of_dimensions_of_one(cuda):
         c.o = b200lab.attn_fwd_kv8(x, *c.cache, c.l, gate=x)
     assert b200lab.device_status() == b200lab.OK
     assert torch.equal(s.o, t.o) and torch.equal(s.v.view(torch.uint8), t.v.view(torch.uint8))
+
+
+# ---- NaN that some rows do not see -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,D,group,B", [(Setup, 64, 4, 3), (Setup, 256, 4, 3), (Wide, 64, 4, 3), (Wide, 256, 4, 3),
+                                            (Wide, 128, 4, 3), (Setup, 64, 12, 3), (Wide, 128, 12, 3),
+                                            (Wide, 64, 2, 300), (Wide, 128, 2, 230), (Wide, 256, 2, 150), (Wide, 128, 5, 230)])
+def test_attend_masked_nan_in_every_channel(cuda, kind, D, group, B):
+    """NaN in V at new tokens, each in channels of its own (all of them over the batch, and over the tokens of the
+    first sequence): it reaches those channels of the rows that see the key, and no other."""
+    new = [4 if B < 100 else 2] * B
+    lens = [(b * 31) % 90 + 8 for b in range(B)]
+    s = kind(lens, 2 if B < 100 else 8, D, 16, seed=D + group, garbage=True)
+    for b in range(B):
+        for i in range(1, new[b]):
+            pos = lens[b] - new[b] + i
+            blk, slot = s.table[b][pos // 16], pos % 16
+            for d in range((b * 5 + i) % 7, D, 7):
+                s.v.view(torch.uint8)[blk, 1, slot, d] = 0x7f if d % 2 else 0xff
+                s.rv.values[blk, 1, slot, d] = np.nan
+    q = _normal((sum(new), s.Hkv * group, D), 9, torch.bfloat16)
+    o = b200lab.attn_fwd_kv8(q.cuda(), *s.cache, s.l, cu_seqlens_q=_prefix(new), max_seqlen_q=max(new))
+    assert b200lab.device_status() == b200lab.OK
+    ref, bound = kv8_ref.attend(q.double().numpy(), s.rk, s.rv, s.table, lens, new, 1 / np.sqrt(D), True,
+                                unit=UNIT[q.dtype])
+    assert np.isnan(ref).any() and not np.isnan(ref[::new[0]]).any()
+    _within(o, ref, bound)
