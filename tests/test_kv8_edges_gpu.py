@@ -6,7 +6,7 @@ import torch
 
 import b200lab
 import kv8_ref
-from test_kv8_gpu import UNIT, Setup, Wide, _ints, _normal, _prefix
+from test_kv8_gpu import UNIT, Setup, Wide, _check_attend, _ints, _normal, _prefix
 
 pytestmark = pytest.mark.gpu
 
@@ -298,3 +298,24 @@ def test_attend_masked_nan_in_every_channel(cuda, kind, D, group, B):
                                 unit=UNIT[q.dtype])
     assert np.isnan(ref).any() and not np.isnan(ref[::new[0]]).any()
     _within(o, ref, bound)
+
+
+# ---- one long sequence among short ones ------------------------------------------------------------------------------
+@pytest.mark.parametrize("D,Hkv,group,B,new", [(128, 1, 1, 64, 1), (128, 1, 3, 64, 1), (128, 1, 4, 64, 1), (128, 1, 8, 64, 1),
+                                               (64, 1, 2, 64, 1), (64, 2, 5, 40, 3), (128, 1, 4, 40, 5), (256, 1, 6, 64, 1),
+                                               (256, 1, 4, 30, 3), (128, 8, 2, 230, 1), (64, 8, 1, 300, 1)])
+def test_attend_one_long_sequence_among_short_ones(cuda, D, Hkv, group, B, new):
+    """Nearly all parts are one segment's, of one to sixteen rows: the warps of its join share them.  The largest
+    values lie in one part, rows that see no key and padding in the short ones."""
+    lens = [(i * 13) % 29 for i in range(B)]
+    lens[B // 3] = 20000
+    counts = [(i * 7) % (new + 1) if new > 1 else 1 for i in range(B)]
+    counts[B // 3] = new
+    s = Wide(lens, Hkv, D, 32, seed=D + B, garbage=True)
+    s.rv.scales[s.table[B // 3][400]] *= 64
+    s.vs.copy_(torch.from_numpy(s.rv.scales).float())
+    q = _normal((sum(counts), Hkv * group, D), 5, torch.bfloat16).cuda()
+    gate = _normal(tuple(q.shape), 6, torch.bfloat16).cuda()
+    _check_attend(s, q, counts, gate=gate)
+    first = b200lab.attn_fwd_kv8(q, *s.cache, s.l, cu_seqlens_q=_prefix(counts), max_seqlen_q=new, gate=gate)
+    assert torch.equal(first, b200lab.attn_fwd_kv8(q, *s.cache, s.l, cu_seqlens_q=_prefix(counts), max_seqlen_q=new, gate=gate))

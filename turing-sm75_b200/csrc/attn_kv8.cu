@@ -111,7 +111,7 @@ struct Args {
     const float* k_scale;
     const float* v_scale;
     float* part;    // [grid][2][rows][D] sums, [grid][2][rows] (m, l)
-    int* meta;      // [grid][4]
+    int* meta;      // [grid][4]: what a CTA says of its last segment (end of attn_kv8_kernel)
     int rts;        // row tiles that a sequence can have
     int log2C;      // CTAs of a cluster that has a segment; negative: the segments are cut by a plan
     int max_seqlen_q, total_q, B, max_blocks, n_blocks, log2P, Hq, Hkv, group, causal;
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
     int slot = 0;  // the next piece's
     for (int i = 0; i < kDepth; ++i) pro.issue(a, sm.ring[warp][i], sm.meta[warp][i], warp, lane);
 
-    bool has_tail = false;  // whether the run's last segment goes on in the next CTA's
+    int said = -1;  // whether the run's last segment goes on in the next CTA's, and where it begins
     for (bool once = kCluster; once || cur.left > 0; once = false, cur.next(a)) {
         const int first = cur.first(), run = cur.count();
         if (!kCluster && run <= 0) continue;  // the cut lies in the segment's start: the next CTA has it
@@ -1086,33 +1086,40 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
             }
         }
         }
-        if (first == 0 && run < s.tiles) {
-            has_tail = true;
-            if (tid == 0) {
-                const long long end = u1 - cur.left + (s.tiles - cur.tile);  // the segment's end
-                a.meta[4 * blockIdx.x] = deal.holder(end - 1);  // the CTA whose run holds its last tile
+        // A CTA that has the first tiles of a segment, and not the last, owns it and describes it: the CTA that has its
+        // last tile, its place, its rows.  One with tiles of its middle alone names the owner, one without either says -1.
+        if (tid == 0 && first + run < s.tiles) {
+            const long long at = u1 - cur.left - cur.tile;  // tile 0 in the plan's numbering
+            if (first == 0) {
+                said = deal.holder(at + s.tiles - 1);
                 a.meta[4 * blockIdx.x + 1] = s.t0;
                 a.meta[4 * blockIdx.x + 2] = cur.h * a.group;
                 a.meta[4 * blockIdx.x + 3] = row0 | rows << 24;
+            } else {
+                said = -2 - deal.holder(at);
             }
         }
     }
-    if (!kCluster && !has_tail && tid == 0) a.meta[4 * blockIdx.x] = -1;
+    if (!kCluster && tid == 0) a.meta[4 * blockIdx.x] = said;
 }
 
 // Joins the segments that were cut: part 0 of each is its owner's second one, the others are the first
 // ones of the CTAs that follow, up to `last`.  Two forms, by how many segments there are:
 //   many (kFew false): block (c, y), rows 8 y .. of the segment that CTA c owns, if it owns one; a warp a
-//     row, as there are few parts (B4 x 8k, 4 tokens, eleven parts: 24.5 us so, 27.3 the other way).
+//     row, as segments of like lengths have few parts (B4 x 8k, 4 tokens, eleven parts: 25.4 us so, 28.4 the other
+//     way).  One far longer than the others has nearly all CTAs' parts: from kLong parts on, its rows go to the
+//     blocks of its first CTAs, which own no segment, a row a block, whose warps share its parts (B64, one of
+//     128k keys and 63 of 10, 4 heads on 1: 73 us with a warp a row, 23 so; B256, 128k and 255 of 500: 120, 101).
 //   few: block (i, n), row n of the i-th segment that was cut, which the block looks up among the owners;
 //     sixteen warps share the parts, of which there can be as many as CTAs.  (A block for every CTA and row
 //     is a thousand blocks more to start: B1 x 64k, 16 heads on 1, 21.8 us with them, 17 without.)
-// Either way a warp has all its loads under way at once behind the one of the segment's description.
-constexpr int kJoinAhead = 4;  // parts a warp loads at a time
+// Either way a warp has the loads of kJoinAhead parts under way at once, behind the one of the segment's description.
+constexpr int kJoinAhead = 4;
+constexpr int kLong = 16;  // at least 8: the owner and seven that are neither it nor the last
 template <int D, int NT, typename T, bool kFew>
 __global__ void __launch_bounds__(kFew ? 512 : 256) attn_kv8_join_kernel(const Args a, int grid) {
     constexpr int kRows = 8 * NT, kVec = D / 32;  // channels of a lane
-    constexpr int kSharers = kFew ? 16 : 1, kPerBlock = kFew ? 1 : 8;
+    constexpr int kWarps = kFew ? 16 : 8;
     grid_dependency_wait();
     allow_dependent_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1139,10 +1146,20 @@ __global__ void __launch_bounds__(kFew ? 512 : 256) attn_kv8_join_kernel(const A
         c = found;
         if (c < 0) return;
     }
-    const int4 desc = reinterpret_cast<const int4*>(a.meta)[c];
+    int4 desc = reinterpret_cast<const int4*>(a.meta)[c];
+    int ahead_of = 0;  // which of the segment's CTAs this block stands for
+    if (!kFew && desc.x < -1) {
+        ahead_of = c + 2 + desc.x;
+        if (ahead_of >= 8) return;
+        c -= ahead_of;
+        desc = reinterpret_cast<const int4*>(a.meta)[c];
+    }
     const int last = desc.x, row0 = desc.w & 0xffffff, rows = desc.w >> 24;
     if (last < 0) return;
-    const int n = blockIdx.y * kPerBlock + (kFew ? 0 : warp);
+    const bool shared = kFew || last - c >= kLong;  // all warps have one row
+    if (!shared && ahead_of > 0) return;
+    const int n = kFew ? blockIdx.y : blockIdx.y * 8 + (shared ? ahead_of : warp);
+    const int sharers = shared ? kWarps : 1, share = shared ? warp : 0;
     const int parts = n < rows ? last - c + 1 : 0;
     int i, hg;
     row_place(row0 + n, a.group, i, hg);
@@ -1154,15 +1171,15 @@ __global__ void __launch_bounds__(kFew ? 512 : 256) attn_kv8_join_kernel(const A
     float M = -INFINITY, sum = 0.f, x[kVec];
 #pragma unroll
     for (int u = 0; u < kVec; ++u) x[u] = 0.f;
-    for (int p0 = warp % kSharers; p0 < parts; p0 += kSharers * kJoinAhead) {
+    for (int p0 = share; p0 < parts; p0 += sharers * kJoinAhead) {
         float2 st[kJoinAhead];
         float y[kJoinAhead][kVec];
 #pragma unroll
         for (int j = 0; j < kJoinAhead; ++j) {
-            const int p = min(p0 + j * kSharers, parts - 1);  // past the end: the last one, not counted
+            const int p = min(p0 + j * sharers, parts - 1);  // past the end: the last one, not counted
             const size_t at = (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * kRows + n;
             st[j] = ml[at];
-            if (p0 + j * kSharers >= parts) st[j] = make_float2(-INFINITY, 0.f);
+            if (p0 + j * sharers >= parts) st[j] = make_float2(-INFINITY, 0.f);
             const float* src = a.part + at * D + lane * kVec;
 #pragma unroll
             for (int u = 0; u < kVec; u += 2) {
@@ -1180,7 +1197,7 @@ __global__ void __launch_bounds__(kFew ? 512 : 256) attn_kv8_join_kernel(const A
         for (int u = 0; u < kVec; ++u) x[u] *= f;
 #pragma unroll
         for (int j = 0; j < kJoinAhead; ++j) {
-            if (p0 + j * kSharers >= parts) continue;
+            if (p0 + j * sharers >= parts) continue;
             const float w = part_weight(st[j].x, st[j].y, to);
             sum = fmaf(w, st[j].y, sum);
 #pragma unroll
@@ -1188,28 +1205,28 @@ __global__ void __launch_bounds__(kFew ? 512 : 256) attn_kv8_join_kernel(const A
         }
         M = to;
     }
-    if constexpr (kSharers > 1) {
-        __shared__ float acc[kSharers][D];
-        __shared__ float2 stat[kSharers];
+    if (shared) {
+        __shared__ float acc[kWarps][D];
+        __shared__ float2 stat[kWarps];
         if (lane == 0) stat[warp] = make_float2(M, sum);
 #pragma unroll
         for (int u = 0; u < kVec; ++u) acc[warp][lane * kVec + u] = x[u];
         __syncthreads();
-        if (warp % kSharers != 0 || n >= rows) return;
+        if (warp != 0) return;
         float all = M;
 #pragma unroll
-        for (int w = 1; w < kSharers; ++w) all = fmaxf(all, stat[warp + w].x);
+        for (int w = 1; w < kWarps; ++w) all = fmaxf(all, stat[w].x);
         const float f = part_weight(M, sum, all);
         sum *= f;
 #pragma unroll
         for (int u = 0; u < kVec; ++u) x[u] *= f;
 #pragma unroll
-        for (int w = 1; w < kSharers; ++w) {
-            const float2 st = stat[warp + w];
+        for (int w = 1; w < kWarps; ++w) {
+            const float2 st = stat[w];
             const float g = part_weight(st.x, st.y, all);
             sum = fmaf(g, st.y, sum);
 #pragma unroll
-            for (int u = 0; u < kVec; ++u) x[u] = fmaf(g, acc[warp + w][lane * kVec + u], x[u]);
+            for (int u = 0; u < kVec; ++u) x[u] = fmaf(g, acc[w][lane * kVec + u], x[u]);
         }
     }
     if (n >= rows) return;
