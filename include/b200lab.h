@@ -296,7 +296,7 @@ int gdn_decode_sm100_state16(const void* q, const void* k, const void* v,
  *   block_table : [B][max_blocks] device int32; token p of sequence b is slot
  *           p % block_size of block block_table[b][p / block_size].  Entries past
  *           a sequence's last block are not read.  Sequences may share blocks
- *           that no call writes.
+ *           that no call writes; one that is written is one place of one sequence.
  *   seq_lens : [B] device int32, tokens of each sequence in the cache
  *   block_size 16, 32, 64 or 128; D 64, 128 or 256.  Caches 16-byte aligned.
  * Nothing needs to be initialised: a block's first token sets its scale, and
@@ -334,7 +334,9 @@ int kv8_append_sm100(const void* k, long long k_stride_token, long long k_stride
 /* Reads the first cu_seqlens[b+1] - cu_seqlens[b] tokens of each sequence back:
  *   k, v : [total_tokens][Hkv][D] contiguous, out_dtype F16, BF16 or F32, 16-byte
  *          aligned; packed as attn_fwd_sm100_varlen takes them, which is how the
- *          queries of a long prompt attend over a cached context.
+ *          queries of a long prompt attend over a cached context (D 64 and 128; at
+ *          D 256 the dense kernel, attn_gated_fwd_sm100, takes them a head after the
+ *          other, so they have to be transposed first).
  * code * scale is exact in BF16 and F32 and rounded in F16 (values above 65504
  * become infinite).  Rows behind the last sequence are left as they were. */
 int kv8_read_sm100(const void* k_cache, const void* v_cache, const float* k_scale,
@@ -356,12 +358,16 @@ int kv8_read_sm100(const void* k_cache, const void* v_cache, const float* k_scal
  *       Q and G hold there.  Rows behind the last sequence are left as they were.
  * GQA as attn_fwd_sm100.  Any number of query tokens is right, but the kernel is
  * made for few: it reads the cache once for every 8 or 16 rows of a kv group,
- * so from about 64 new tokens a sequence on they are faster through
- * kv8_read_sm100 and attn_fwd_sm100_varlen (8 sequences of 4096 keys, 32 q-heads on
- * 8 of 128: 64 tokens 139 us against 147, 256 tokens 478 against 167).  Few short
+ * so from about 48 new tokens a sequence on (150 for a lone sequence) they are
+ * faster through kv8_read_sm100 and attn_fwd_sm100_varlen (8 sequences of 4096 keys,
+ * 32 q-heads on 8 of 128: 16 tokens 58 us against 146, 64 tokens 202 against 146, 256
+ * tokens 771 against 170).  attn_fwd_sm100_varlen takes D 64 and 128: at D 256, through
+ * kv8_read_sm100, transposes and attn_gated_fwd_sm100 (24 heads on 4, 8 sequences: 16
+ * tokens 105 us against 348, 64 tokens 376 / 359, 256 tokens 1490 / 474).  Few short
  * sequences take one kernel instead of two (B1 x 1000 6.2 us against 9.1); the call knows
  * them by the width of the block table (max_blocks * block_size tokens), so one that
- * is no wider than the batch needs is faster.  Calls that may overlap need
+ * is no wider than the batch needs is faster, and a step captured once with a table for
+ * long texts takes two kernels whatever the lengths are.  Calls that may overlap need
  * workspaces of their own. */
 int attn_fwd_sm100_kv8(const void* Q, long long q_stride_token, long long q_stride_head,
                        const void* G, long long g_stride_token, long long g_stride_head,

@@ -12,10 +12,10 @@
 // 2^-40 to 2^40, span any number.  So m is no running maximum: it follows the keys in hand, up and down.
 // p stays below 2^15, and the largest p of a piece (the 16 or 32 keys a warp takes at a time) above 2^-8, so that
 // a rounding to fp16 is off by 2^-11 of the weight or 2^-17 of its piece's largest, however small the piece's
-// weights are beside the row's others: many small weights together count in full.  (With a running maximum for
-// m, a warp that met a key 2^26 above its others lost all of those; 0.5 to 4 % of a call's time is what it costs.)  m
-// goes no lower than where l, in fp32, would pass 2^60; what fp16 loses of a weight there moves an output
-// by less than 448 x 2^-83.
+// weights are beside the row's others: many small weights together count in full.  m goes no lower than where
+// l, in fp32, would pass 2^60; what fp16 loses of a weight there moves an output by less than 448 x 2^-83.
+// (With a running maximum for m, a warp that met a key 2^26 above its others lost all of those.  What following the
+// keys costs: 0.5 % of long streams, 3 to 6 % of short calls, 7 % of many rows at D 256.)
 //
 // What bounds it: the bytes of the cache; a code is used by the few rows of its kv group only
 // (2 x rows flop a byte).  Everything follows from streaming them:
@@ -42,11 +42,13 @@
 //   * Q is brought to fp16 with a power of two a row: exact, as bf16 and fp16 both have at most 11
 //     significant bits (below 2^-29 of the row's largest value, bits are lost).
 // Measured, 32 q-heads on 8 kv-heads of 128 unless said, calls back to back in a graph: B64 x 16k 345 us
-// (6.2 TB/s, 97 % of the measured copy rate), B64 x 400..8k 99 us (89 %), B1 x 16k 14.5 us, B1 x 1000
-// 6.2 us, 4 tokens x B16 x 2-4k 31 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 43 us, 8 heads of 64
-// B48 x 250..2500 22 us.  The longest streams are bound by memory; what the shorter ones add to that is
-// a call's own chain (lengths, block ids, codes; the part's join; the second kernel: 7 us in all, 4 with clusters) and,
-// with more rows or 64 channels, the instructions of converting (0.5 issued a cycle and scheduler).
+// (6.2 TB/s, 97 % of the measured copy rate), B64 x 400..8k 99.6 us (88 %), B1 x 16k 14.6 us, B1 x 1000
+// 6.2 us, 4 tokens x B16 x 2-4k 32 us, 24 q-heads on 4 of 256 with gate B32 x 2-4k 43 us, 8 heads of 64
+// B48 x 250..2500 23 us.  The longest streams are bound by memory; what the shorter ones add to that is
+// a call's own chain (lengths, block ids, codes; the part's join; the second kernel: 7 us in all, 4 with clusters).
+// With more rows or 64 channels it is latency: a piece is a chain of dependent conversions, products and
+// exponentials, and the two or four warps that a scheduler has cover a third or a half of it (issue 34 and 48 %
+// busy, half of the stalls waits for a fixed latency; neither a pipe nor memory is full).
 #include "errwords.h"
 #include "kv8.cuh"
 
@@ -1246,10 +1248,12 @@ int plan_grid(int D, int nt, int warps, int sms) {
 // Warps of a CTA.  Four share the tiles of a segment and join their sums in shared memory, which
 // leaves few cut segments; a warp on its own joins nothing, and while it starts or ends a segment the
 // SM's other warps go on: better where segments are short and many.  The lengths are on the device, so
-// the rule goes by what the host has, the segments and the most that the block table can hold (measured
-// by the plan, with four / with one, 32 q-heads on 8 kv-heads of 128 unless said: B64 x 200 tokens 14.8 / 14.0 us,
-// B128 x 200 24.9 / 21.6, B256 x 200 40.9 / 29.1, B512 x 64 52 / 31, B128 x 2k D 64 32 heads 148 / 136,
-// B256 x 1k 79 / 81, and the other way B256 x 200..4k 188 / 197, B32 x 200 11.0 / 16.6).
+// the rule goes by what the host has, the segments and the most that the block table can hold.  Measured
+// by the plan, inputs in turn beyond L2, with four / with one, 32 q-heads on 8 kv-heads of 128 unless said: B64 x 200
+// tokens 18.0 / 17.4 us, B128 x 200 27.0 / 23.6, B256 x 200 42.6 / 33.7, B512 x 64 51 / 30, B128 x 2k D 64 32 heads
+// 190 / 177, and the other way B32 x 200 11.7 / 13.8.  A wide table does not tell what lengths it holds: B256 in one for
+// 4k tokens is 42.6 / 33.7 where all have 200, 62.4 / 59.4 where they have 500, but 93 / 102 with 1000 and 180 / 192 with
+// 200 to 4k.  The rule takes one there: up to 9 % lost where sequences are long, up to 21 % won where they are short.
 int warps_of(long long segments, long long tokens, int D, int nt, int sms) {
     const long long alone = plan_grid(D, nt, 1, sms);
     return segments >= (tokens <= 512 ? alone / 2 : alone) ? 1 : 4;
@@ -1262,11 +1266,11 @@ int warps_of(long long segments, long long tokens, int D, int nt, int sms) {
 // an SM one CTA.  Where a CTA then has more than two tiles, eight warps share them, if the segments are so
 // many that the clusters are pairs at most (wider ones of such CTAs do not all find room at once: B2 x 4096
 // 16.4 us with eight CTAs of eight warps, 9.8 of four); else two CTAs an SM do, from four tiles on.
-// Measured, 32 q-heads on 8 kv-heads of 128, planned / by clusters: B1 x 64 7.2 / 4.2 us, B1 x 1000 9.1 / 6.4,
-// B1 x 4096 10.3 / 9.4, B1 x 8192 11.2 / 13.5 (so planned), B4 x 2000 12.1 / 9.0, B16 x 250 10.2 / 6.2, B32 x 250
-// 11.5 / 6.8, B64 x 250 15.7 / 12.8, B128 x 200 21.3 / 21.9 (so planned); with four warps / eight: B8 x 1000 8.9 /
-// 7.8, B16 x 500 8.4 / 7.0, B1 x 2000 7.1 / 7.8 (so four).  Two column tiles: 4 tokens x B16 x 250 planned 11.8, by
-// clusters 8.2, x B16 x 1000 15.8 / 12.2, x B1 x 2000 11.1 / 11.5 (so planned).
+// Measured, 32 q-heads on 8 kv-heads of 128, planned / by clusters: B1 x 64 7.4 / 4.4 us, B1 x 1000 9.3 / 6.6,
+// B1 x 4096 10.3 / 9.5, B1 x 8192 11.3 / 13.5 (so planned), B4 x 2000 12.5 / 9.5, B16 x 250 10.6 / 6.4, B32 x 250
+// 11.6 / 7.0, B64 x 250 19.9 / 16.6, B128 x 200 23.5 / 23.0 (about even from here on: planned); with four warps /
+// eight: B8 x 1000 9.2 / 8.3, B16 x 500 8.5 / 7.1, B1 x 2000 7.3 / 8.0 (so four).  Two column tiles: 4 tokens x B16 x 250
+// planned 13.1, by clusters 8.7, x B16 x 1000 19.9 / 14.8, x B1 x 2000 11.1 / 12.8 (so planned).
 struct Clusters {
     int log2C, warps;
 };
