@@ -149,20 +149,6 @@ def test_attend_sharp_key_in_a_block_of_large_values(cuda, kind, D, n, copies, f
     _check_tight(s, _q_of_bits(BITS, D, 2.0 ** -7, torch.bfloat16), 1.0, copies)
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("kind,D,n,copies", FORMS[:1] + FORMS[2:5] + FORMS[6:])
-def test_attend_references_that_move_at_every_piece(cuda, kind, D, n, copies, dtype):
-    """Every other 32 keys take nearly all of the weight, of values 0; the others make the output."""
-    s = kind([n], 1, D, 32, seed=n + D, exps=(-6, -6))
-    s.rk.scales[:] = 2.0 ** -7
-    s.rk.values[:] = 0
-    s.rv.values[:] = np.abs(s.rv.values)
-    for block in s.table[0][:-(-n // 32)][::2]:
-        s.rk.values[block, :, :, 0] = 448
-        s.rv.values[block] = 0
-    _check_tight(s, _q_of_bits([0.0, 13.0, 19.0, 24.5, 25.5, 30.0, 36.0, 47.0], D, 2.0 ** -7, dtype), 1.0, copies)
-
-
 @pytest.mark.parametrize("copies", [1, 60, 240])
 @pytest.mark.parametrize("kind", [Setup, Wide], ids=["narrow", "wide"])
 @pytest.mark.parametrize("D,group,P", [(64, 8, 16), (128, 4, 16), (128, 12, 32), (256, 6, 128), (64, 20, 64)])

@@ -63,8 +63,7 @@ constexpr int kMostCluster = 8;           // CTAs of a cluster
 constexpr int kGroup = 16;                // keys of one product
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's reference m is moved when a score lies above m + kTop, to kRise below it, or when a piece has none as high
-// as m + kBottom, to kFall above its largest; to whole numbers, so that the sums, which can be moved as often as a run
-// has pieces, are multiplied by exact powers of two.
+// as m + kBottom, to kFall above its largest.
 constexpr float kTop = 15.f, kRise = 10.f, kBottom = -8.f, kFall = 4.f;
 constexpr int kMostSum = 60;              // and not to where its sum l would pass 2^60
 
@@ -209,11 +208,6 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// 2^k for a whole k up to 127; 0 below -126.
-__device__ __forceinline__ float power_of_two(float k) {
-    return k < -126.f ? 0.f : __uint_as_float((uint32_t)((int)k + 127) << 23);
-}
-
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -248,7 +242,6 @@ template <int D, int NT, int W> struct Smem {
 __device__ __forceinline__ float part_weight(float m, float l, float M) {
     return m == -INFINITY && l == l ? 0.f : ex2(m - M);
 }
-
 // Row n of a row tile -> query token of the sequence and head of the group.
 __device__ __forceinline__ void row_place(int row, int group, int& i, int& hg) {
     i = row / group;
@@ -794,7 +787,7 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                             for (int u = 1; u < kH; ++u) x[nt][c] = fmaxf(x[nt][c], fmaxf(sc[u][nt][0][c], sc[u][nt][0][c + 2]));
 #pragma unroll
                             for (int k = 4; k <= 16; k <<= 1) x[nt][c] = fmaxf(x[nt][c], __shfl_xor_sync(0xffffffffu, x[nt][c], k));
-                            to[nt][c] = x[nt][c] > m[nt][c] + kTop ? rintf(x[nt][c]) - kRise : m[nt][c];
+                            to[nt][c] = x[nt][c] > m[nt][c] + kTop ? x[nt][c] - kRise : m[nt][c];
                             fall |= x[nt][c] > -INFINITY && x[nt][c] < m[nt][c] + kBottom;
                         }
                     if (__any_sync(0xffffffffu, fall)) {
@@ -808,7 +801,7 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                                 // (a sum that is NaN has the largest exponent: m stays)
                                 const int room = kMostSum - 1 - ((int)(__float_as_uint(sum) >> 23) - 127);
                                 if (x[nt][c] > -INFINITY && x[nt][c] < m[nt][c] + kBottom)
-                                    to[nt][c] = fmaxf(rintf(x[nt][c]) + kFall, m[nt][c] - (float)max(room, 0));
+                                    to[nt][c] = fmaxf(x[nt][c] + kFall, m[nt][c] - (float)max(room, 0));
                             }
                     }
 #pragma unroll
@@ -816,7 +809,7 @@ __global__ void __launch_bounds__(32 * W, Cfg<D, NT, W>::kCtas)
                         if (!__any_sync(0xffffffffu, to[nt][0] != m[nt][0] || to[nt][1] != m[nt][1])) continue;
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const float f = to[nt][c] == m[nt][c] ? 1.f : power_of_two(m[nt][c] - to[nt][c]);
+                            const float f = to[nt][c] == m[nt][c] ? 1.f : ex2(m[nt][c] - to[nt][c]);
                             m[nt][c] = to[nt][c];
                             l[nt][c] *= f;
 #pragma unroll
