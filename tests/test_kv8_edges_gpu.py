@@ -149,6 +149,47 @@ def test_attend_sharp_key_in_a_block_of_large_values(cuda, kind, D, n, copies, f
     _check_tight(s, _q_of_bits(BITS, D, 2.0 ** -7, torch.bfloat16), 1.0, copies)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind,D,n,copies", FORMS[:1] + FORMS[2:5] + FORMS[6:])
+def test_attend_references_that_move_at_every_piece(cuda, kind, D, n, copies, dtype):
+    """Every other 32 keys take nearly all of the weight, of values 0; the others make the output."""
+    s = kind([n], 1, D, 32, seed=n + D, exps=(-6, -6))
+    s.rk.scales[:] = 2.0 ** -7
+    s.rk.values[:] = 0
+    s.rv.values[:] = np.abs(s.rv.values)
+    for block in s.table[0][:-(-n // 32)][::2]:
+        s.rk.values[block, :, :, 0] = 448
+        s.rv.values[block] = 0
+    _check_tight(s, _q_of_bits([0.0, 13.0, 19.0, 24.5, 25.5, 30.0, 36.0, 47.0], D, 2.0 ** -7, dtype), 1.0, copies)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind,B,Hkv", [(Setup, 20, 2), (Wide, 20, 2), (Setup, 300, 8), (Wide, 300, 8)])
+@pytest.mark.parametrize("D,group", [(64, 3), (128, 4), (128, 12), (256, 6)])
+def test_attend_the_largest_weight_is_exact(cuda, kind, B, Hkv, D, group, dtype):
+    """A row whose first key has all of the weight gives that key's values, to the bit: the reference stands at a whole
+    number of powers of two below it, so fp16 holds its weight as it is (off by 2^-21 of the exponential, far from
+    half a step of the output).  A lone key's, and one's 60 powers of two above the others'."""
+    lens = [1 + 40 * (i % 2) for i in range(B)]
+    s = kind(lens, Hkv, D, 16, seed=D + group, exps=(-8, -5))
+    s.rk.scales[:] = 2.0 ** -7
+    q = _normal((B, Hkv * group, D), 7, torch.float32)
+    q[..., 0] = q[..., 0].abs() + 17  # scores of 17 * 3.5 = 59 and more with the first key, of 0 with the others
+    for b in range(1, B, 2):
+        for i in range(3):
+            s.rk.values[s.table[b][i]] = 0
+        s.rk.values[s.table[b][0], :, 0, 0] = 448
+    s.rv.values[s.rv.values == 0] = 1  # where the first key's were 0, the others' 2^-60 would be the answer
+    for t, r in ((s.k, s.rk), (s.v, s.rv)):
+        t.copy_(torch.from_numpy(r.values).float().to(t.dtype))
+    s.ks.copy_(torch.from_numpy(s.rk.scales).float())
+    o = b200lab.attn_fwd_kv8(q.to(dtype).cuda(), *s.cache, s.l, scale=1.0)
+    assert b200lab.device_status() == b200lab.OK
+    want = np.stack([s.rv.tokens(s.table[b], 1)[0] for b in range(B)]).repeat(group, axis=1)
+    off = (o.cpu() != torch.from_numpy(want).to(dtype)).nonzero().tolist()
+    assert not off, f"{len(off)} differ, the first at {off[0]}"
+
+
 @pytest.mark.parametrize("copies", [1, 60, 240])
 @pytest.mark.parametrize("kind", [Setup, Wide], ids=["narrow", "wide"])
 @pytest.mark.parametrize("D,group,P", [(64, 8, 16), (128, 4, 16), (128, 12, 32), (256, 6, 128), (64, 20, 64)])

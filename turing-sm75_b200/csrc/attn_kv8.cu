@@ -63,7 +63,9 @@ constexpr int kMostCluster = 8;           // CTAs of a cluster
 constexpr int kGroup = 16;                // keys of one product
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's reference m is moved when a score lies above m + kTop, to kRise below it, or when a piece has none as high
-// as m + kBottom, to kFall above its largest.
+// as m + kBottom, to kFall above its largest: whole powers of two away, so that fp16 holds the weight of the key that moved
+// it as it is.  (References that are whole numbers themselves, moved without a rounding, leave the largest weights rounded
+// where l is not: errors of fp16 outputs 3.0e-4 instead of 2.2e-4, and a lone key's values no longer exact.)
 constexpr float kTop = 15.f, kRise = 10.f, kBottom = -8.f, kFall = 4.f;
 constexpr int kMostSum = 60;              // and not to where its sum l would pass 2^60
 
@@ -242,6 +244,7 @@ template <int D, int NT, int W> struct Smem {
 __device__ __forceinline__ float part_weight(float m, float l, float M) {
     return m == -INFINITY && l == l ? 0.f : ex2(m - M);
 }
+
 // Row n of a row tile -> query token of the sequence and head of the group.
 __device__ __forceinline__ void row_place(int row, int group, int& i, int& hg) {
     i = row / group;
